@@ -195,8 +195,8 @@ def _own_run(st):
   cache = st["cache"] if case["kv"] in DTYPE else ops.BfpCache(st["cache"], case["kv"], 2 * kv, st["rows"], hd)
   if case["kind"] == "packed":
     if "ws" not in st: st["ws"] = ops.attention_packed_workspace(st["q"].shape[0], case["n"], heads, kv, hd, st["context"])
-    return ops.attention_prefill_packed(st["q"], cache, heads, kv, hd, st["starts"], st["p0"], st["first"], st["context"], prefix_row=st["prefix_row"],
-                                        shared=st["shared"], workspace=st["ws"], o=st["o"])
+    prefix = dict(prefix_row=st["prefix_row"], shared=st["shared"]) if case["prefix"] else {}
+    return ops.attention_prefill_packed(st["q"], cache, heads, kv, hd, st["starts"], st["p0"], st["first"], st["context"], workspace=st["ws"], o=st["o"], **prefix)
   if "ws" not in st: st["ws"] = ops.attention_shared_workspace(case["batch"], heads, kv, hd, st["prefix"], st["longest"])
   return ops.attention_decode_shared(st["q"], cache, heads, kv, hd, st["places"], st["first"], st["prefix_row"], st["shared"], st["prefix"], st["longest"],
                                      workspace=st["ws"], o=st["o"])
