@@ -60,6 +60,10 @@ SIGNATURES = {
   "fh_attention_decode": ([P, P, I, L, I, I, I, I, P, P, L, P, I, P, S, P], I),
   "fh_attention_decode_noalloc": ([P, P, I, L, I, I, I, I, P, P, L, P, I, P], I),
   "fh_attention_prefill": ([P, L, P, I, L, I, I, I, I, L, L, P, I, L, P], I),
+  "fh_attention_packed_workspace_bytes": ([L, I, I, I, I, L], S),
+  "fh_attention_prefill_packed": ([P, I, L, P, I, L, L, I, I, I, I, P, P, P, P, P, L, P, I, L, P, S, P], I),
+  "fh_attention_shared_workspace_bytes": ([I, I, I, I, L, L], S),
+  "fh_attention_decode_shared": ([P, I, P, I, L, I, I, I, I, P, P, P, P, L, L, P, I, P, S, P], I),
   "fh_rms_rows": ([P, L, L, L, P, ctypes.c_float, I, P, I, L, P], I),
   "fh_moe_route": ([P, L, I, L, P, ctypes.c_float, I, P, I, I, I, I, P, P, P, P], I),
   "fh_moe_workspace_bytes": ([I, I, L, L], S),
@@ -74,6 +78,7 @@ SIGNATURES = {
   "fh_lds_probe": ([I, P, I, P], I),
   "fh_heads_workspace_bytes": ([I, L, I], S),
   "fh_logit_heads": ([P, L, I, L, I, P, P, P, P, P, S, P], I),
+  "fh_logit_rules": ([P, L, L, L, P, L, L, P, P, P, P, P, P, P, L, L, P, L, P, L, P], I),
   "fh_gather_cols": ([P, L, L, P, L, L, L, P, L, P], I),
   "fh_gather_rows": ([P, L, L, L, P, L, L, L, P, L, L, P], I),
   "fh_moe_touched": ([P, L, P, L, I, I, I, P, P, P], I),

@@ -349,6 +349,104 @@ def attention_prefill(q, cache, heads, kv_heads, head_dim, p0, slot_row, o=None,
   return o
 
 
+def _rows_operand(what, q, cols):
+  """q [rows][cols] (fp32 or bf16, rows contiguous), its device the current one: what an entry point reads rows of."""
+  _dev(q)
+  if q.dim() != 2 or q.shape[0] < 1 or q.shape[1] != cols or q.dtype not in _TORCH or q.stride(1) != 1:
+    raise ValueError(f"{what}: q [rows][{cols}] fp32 or bf16 with contiguous rows, not {tuple(q.shape)} {q.dtype}")
+
+
+def _here(what, device, *ts):
+  """Each tensor (or None) on `device`, and that device the current one, whose stream the call goes to."""
+  if device.type != "cuda" or _device() not in (None, device.index): raise ValueError(f"{what}: tensors must be on the current GPU")
+  for t in ts:
+    if t is not None and t.device != device: raise ValueError(f"{what}: tensors must be on one GPU")
+
+
+def _int_vector(what, name, t, n):
+  if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or (n > 1 and t.stride(0) != 1):
+    raise ValueError(f"{what}: {name} is {n} contiguous int32 on the GPU")
+
+
+def _cache_of(what, cache, kv_heads, head_dim):
+  """cache_fields of a cache of kv_heads heads of head_dim, contiguous."""
+  data, dtype, length = cache_fields(cache)
+  if tuple(cache.shape) != (2 * kv_heads, length, head_dim) or not data.is_contiguous():
+    raise ValueError(f"{what}: a contiguous cache [{2 * kv_heads}][len][{head_dim}], not {tuple(cache.shape)}")
+  if isinstance(cache, BfpCache) and data.numel() < lib.load().fh_kv_cache_bytes(dtype, kv_heads, length, head_dim):
+    raise ValueError(f"{what}: the cache's buffer is smaller than its shape")
+  return data, dtype, length
+
+
+def attention_packed_workspace(rows, sequences, heads, kv_heads, head_dim, max_context, device="cuda"):
+  """fh_attention_prefill_packed's workspace, uninitialised (a workspace needs no clearing)."""
+  n = lib.load().fh_attention_packed_workspace_bytes(rows, sequences, heads, kv_heads, head_dim, max_context)
+  return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
+
+
+def attention_prefill_packed(q, cache, heads, kv_heads, head_dim, starts, p0, first_row, max_context, prefix_row=None, shared=None,
+                             workspace=None, o=None, out_dtype=torch.float32):
+  """The causal attention of packed prompts (fh_attention_prefill_packed): rows starts[s] .. starts[s + 1] - 1 of q
+  [T][heads*hd] (fp32 or bf16) are sequence s's, at places p0[s], p0[s] + 1, ... of it; place p lies at cache row
+  first_row[s] + p, or, given shared [sequences] and prefix_row [1], at prefix_row + p where p < shared[s] and at
+  first_row[s] + p - shared[s] behind them. starts [sequences + 1], p0, first_row, shared and prefix_row are int32 on the
+  GPU, read when the kernel runs. max_context bounds every place + 1. o (fp32 or bf16) keeps its rows that are no
+  sequence's; a new o has zeros there."""
+  what = "attention_prefill_packed"
+  _rows_operand(what, q, heads * head_dim)
+  data, dtype, length = _cache_of(what, cache, kv_heads, head_dim)
+  T, n = q.shape[0], p0.numel()
+  _int_vector(what, "starts", starts, n + 1)
+  for name, t in (("p0", p0), ("first_row", first_row)): _int_vector(what, name, t, n)
+  if (shared is None) != (prefix_row is None): raise ValueError(f"{what}: shared and prefix_row go together")
+  if shared is not None:
+    _int_vector(what, "shared", shared, n)
+    _int_vector(what, "prefix_row", prefix_row, 1)
+  if o is None: o = torch.zeros(T, heads * head_dim, dtype=out_dtype, device=q.device)
+  if o.shape != q.shape or o.dtype not in _TORCH or o.stride(1) != 1: raise ValueError(f"{what}: o is fp32 or bf16 rows of q's shape")
+  need = lib.load().fh_attention_packed_workspace_bytes(T, n, heads, kv_heads, head_dim, max_context)
+  if need and workspace is None: workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+  _here(what, q.device, data, starts, p0, first_row, prefix_row, shared, o, workspace)
+  lib.call("fh_attention_prefill_packed", _ptr(q), _TORCH[q.dtype], q.stride(0), _ptr(data), dtype, length, T, n, heads, kv_heads,
+           head_dim, _ptr(starts), _ptr(p0), _ptr(first_row), _ptr(prefix_row), _ptr(shared), max_context, _ptr(o), _TORCH[o.dtype],
+           o.stride(0), _ptr(workspace), workspace.numel() if workspace is not None else 0, _stream())
+  return o
+
+
+def attention_shared_workspace(batch, heads, kv_heads, head_dim, max_prefix, max_own, device="cuda"):
+  """fh_attention_decode_shared's workspace, uninitialised (a workspace needs no clearing)."""
+  n = lib.load().fh_attention_shared_workspace_bytes(batch, heads, kv_heads, head_dim, max_prefix, max_own)
+  return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
+
+
+def attention_decode_shared(q, cache, heads, kv_heads, head_dim, places, first_row, prefix_row, shared, max_prefix, max_own,
+                            workspace=None, o=None, out_dtype=torch.float32):
+  """The decode attention of a batch that shares a prefix (fh_attention_decode_shared): row b of q [batch][heads*hd] (fp32
+  or bf16) is at places[b] of its sequence, whose places below shared[b] lie at cache rows prefix_row + place (read once for
+  the batch) and the rest at first_row[b] + place - shared[b]. All int32 on the GPU, read when the kernels run; max_prefix
+  bounds shared, max_own the places behind it. A row at place -1 sees nothing and gives zeros. o: contiguous fp32 or bf16 of
+  q's shape, or Tiles16."""
+  what = "attention_decode_shared"
+  _rows_operand(what, q, heads * head_dim)
+  if not q.is_contiguous(): raise ValueError(f"{what}: q contiguous")
+  data, dtype, length = _cache_of(what, cache, kv_heads, head_dim)
+  batch = q.shape[0]
+  for name, t in (("places", places), ("first_row", first_row), ("shared", shared)): _int_vector(what, name, t, batch)
+  _int_vector(what, "prefix_row", prefix_row, 1)
+  if o is None: o = torch.empty(batch, heads * head_dim, dtype=out_dtype, device=q.device)
+  if isinstance(o, Tiles16):
+    if (o.rows, o.cols) != tuple(q.shape): raise ValueError(f"{what}: o tiles of q's shape")
+  elif o.dtype not in _TORCH or o.shape != q.shape or not o.is_contiguous(): raise ValueError(f"{what}: o is a contiguous fp32 or bf16 tensor of q's shape")
+  need = lib.load().fh_attention_shared_workspace_bytes(batch, heads, kv_heads, head_dim, max_prefix, max_own)
+  if need and workspace is None: workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+  _here(what, q.device, data, places, first_row, prefix_row, shared, o.data if isinstance(o, Tiles16) else o, workspace)
+  op, odt, _, _ = _layout(o)
+  lib.call("fh_attention_decode_shared", _ptr(q), _TORCH[q.dtype], _ptr(data), dtype, length, batch, heads, kv_heads, head_dim, _ptr(places),
+           _ptr(first_row), _ptr(prefix_row), _ptr(shared), max_prefix, max_own, op, odt, _ptr(workspace),
+           workspace.numel() if workspace is not None else 0, _stream())
+  return o
+
+
 def rms_rows(x, w, eps, centered=False, out=None, out_dtype=torch.bfloat16):
   """x * rsqrt(mean(x^2) + eps) * w, a row at a time (fh_rms_rows); bf16 out by default (a prefill GEMM's input), or
   bf16 Tiles16."""
@@ -425,6 +523,49 @@ def logit_heads(logits, k=64, inv_temp=None, ws=None):
   lib.call("fh_logit_heads", _ptr(logits), logits.stride(0), rows, vocab, k, _ptr(inv_temp), _ptr(values), _ptr(ids),
            _ptr(lse), _ptr(ws) if n else None, ws.numel() if n else 0, _stream())
   return (values, ids) if lse is None else (values, ids, lse)
+
+
+def logit_rules(logits, tokens=None, lengths=None, prompt_lengths=None, repetition=None, presence=None, frequency=None, bias_ids=None,
+                bias=None, allowed=None, out=None):
+  """Each request's rules on its row of logits [rows][vocab] (fp32), into out (a new tensor by default; logits itself for
+  in place): pen(x) - frequency n - presence [n > 0] + bias, -inf where not allowed (fh_logit_rules). tokens [rows][most]
+  int32, the prompt's first, each row's first lengths[row] (all by default; ids outside the vocabulary are padding);
+  repetition divides a positive logit of any of them and multiplies the others; n counts those from prompt_lengths[row] on.
+  repetition, presence, frequency [rows] fp32; bias_ids int32 and bias fp32 [rows][up to 1024]; allowed [rows][vocab / 32
+  rounded up] int32, bit c % 32 of word c / 32 for column c. Each may be left out."""
+  what = "logit_rules"
+  _dev(logits)
+  if logits.dtype != torch.float32 or logits.dim() != 2 or logits.shape[0] < 1 or logits.stride(1) != 1: raise ValueError(f"{what}: fp32 rows")
+  rows, vocab = logits.shape
+
+  def vector(name, t, dtype):
+    if t is not None and (t.dtype != dtype or t.dim() != 1 or t.numel() != rows or (rows > 1 and t.stride(0) != 1)):
+      raise ValueError(f"{what}: {name} is {rows} contiguous {dtype}")
+
+  def matrix(name, t, dtype, cols=0):
+    if t is not None and (t.dtype != dtype or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < cols or (t.shape[1] > 1 and t.stride(1) != 1)):
+      raise ValueError(f"{what}: {name} is [{rows}][{cols or 'any'}] {dtype} with contiguous rows")
+    # (rows that overlap, as one row expanded to all of them: each its own)
+    return t.contiguous() if t is not None and rows > 1 and t.stride(0) < t.shape[1] else t
+
+  for name, t in (("lengths", lengths), ("prompt_lengths", prompt_lengths)): vector(name, t, torch.int32)
+  for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)): vector(name, t, torch.float32)
+  logits = matrix("logits", logits, torch.float32)
+  tokens, bias_ids, bias = matrix("tokens", tokens, torch.int32), matrix("bias_ids", bias_ids, torch.int32), matrix("bias", bias, torch.float32)
+  allowed = matrix("allowed", allowed, torch.int32, -(-vocab // 32))
+  if (bias is None) != (bias_ids is None) or (bias is not None and bias.shape != bias_ids.shape): raise ValueError(f"{what}: bias_ids and bias of one shape")
+  if bias is not None and bias.stride(0) != bias_ids.stride(0): bias, bias_ids = bias.contiguous(), bias_ids.contiguous()
+  if tokens is None and (lengths is not None or prompt_lengths is not None): raise ValueError(f"{what}: lengths without tokens")
+  if out is None: out = torch.empty(rows, vocab, dtype=torch.float32, device=logits.device)
+  if out.dtype != torch.float32 or out.shape != logits.shape or out.stride(1) != 1 or (rows > 1 and out.stride(0) < vocab):
+    raise ValueError(f"{what}: out is fp32 rows of logits' shape")
+  _here(what, logits.device, tokens, lengths, prompt_lengths, repetition, presence, frequency, bias_ids, bias, allowed, out)
+  nt, nb = (tokens.shape[1] if tokens is not None else 0), (bias.shape[1] if bias is not None else 0)
+  ld = lambda t: max(t.stride(0), t.shape[1]) if t is not None else 0  # (one row's stride may be anything)
+  lib.call("fh_logit_rules", _ptr(logits), ld(logits), rows, vocab, _ptr(tokens) if nt else None, ld(tokens), nt, _ptr(lengths) if nt else None,
+           _ptr(prompt_lengths) if nt else None, _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias_ids) if nb else None,
+           _ptr(bias) if nb else None, ld(bias), nb, _ptr(allowed), ld(allowed), _ptr(out), ld(out), _stream())
+  return out
 
 
 def argmax_rows(x, ids=None):

@@ -263,6 +263,40 @@ int fh_attention_prefill(const float* q, int64_t ldq, const void* cache, int cac
                          int heads, int kv_heads, int head_dim, int64_t p0, int64_t slot_row, void* o, int o_dtype,
                          int64_t ldo, void* stream);
 
+/* ---- many sequences at once: packed prompts, a shared prefix ------------------------------------------------------
+ * Both calls below address a sequence's places the same way: place p of sequence s lies at cache row prefix_row[0] + p
+ * where p < shared[s], and at first_row[s] + p - shared[s] behind them, so that many sequences read one copy of a prefix
+ * (shared NULL with prefix_row NULL: no prefix, place p at first_row[s] + p). A query at place p sees places 0 .. p, and
+ * one that sees none (a place below 0) gives zeros. All of it is device data, read when the kernels run (a captured call
+ * replays with what the arrays hold then); a cache row outside the cache is read at its nearest row, never outside. q is
+ * FH_F32 or FH_BF16, the cache any of fh_kv_cache_bytes' formats, head_dim 64 or 128; query head h reads kv head
+ * h / (heads / kv_heads). q's rows and the cache are 16-byte aligned, o's rows aligned to 4 values. Rows and cache values
+ * that a query does not see have no part in its result, NaN and infinities included. A workspace (16-byte aligned) as
+ * everywhere: no clearing, no state, not shared by calls that overlap. No counterpart in the reference, whose prompts are
+ * prefilled one at a time (models/llama.py:498-504) and whose rows each read their own slot (models/llama.py:429-452). */
+
+/* The causal attention of packed prompts: rows starts[s] .. starts[s + 1] - 1 of q [rows][ldq] are sequence s's, at places
+ * p0[s], p0[s] + 1, ..., their keys and values already in the cache; starts [sequences + 1] does not decrease (a sequence
+ * may have no rows), and rows of o before starts[0] or from starts[sequences] on are left as they were. max_context: a bound of every
+ * place + 1 (keys past it are not read). */
+size_t fh_attention_packed_workspace_bytes(int64_t rows, int sequences, int heads, int kv_heads, int head_dim,
+                                           int64_t max_context);
+int fh_attention_prefill_packed(const void* q, int q_dtype, int64_t ldq, const void* cache, int cache_dtype, int64_t cache_len,
+                                int64_t rows, int sequences, int heads, int kv_heads, int head_dim, const int32_t* starts,
+                                const int32_t* p0, const int32_t* first_row, const int32_t* prefix_row, const int32_t* shared,
+                                int64_t max_context, void* o, int o_dtype, int64_t ldo, void* workspace, size_t ws_bytes,
+                                void* stream);
+
+/* The decode attention of a batch that shares a prefix: row b of q [batch][heads*head_dim] is at places[b] of its sequence,
+ * whose first shared[b] places are the prefix's (each row its own count, 0 for none). The prefix's rows are read once for
+ * the whole batch. max_prefix bounds shared, max_own the places behind it (keys past either are not read). o: FH_F32,
+ * FH_BF16 or FH_BF16_T16, rows of heads * head_dim. */
+size_t fh_attention_shared_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int64_t max_prefix, int64_t max_own);
+int fh_attention_decode_shared(const void* q, int q_dtype, const void* cache, int cache_dtype, int64_t cache_len, int batch,
+                               int heads, int kv_heads, int head_dim, const int32_t* places, const int32_t* first_row,
+                               const int32_t* prefix_row, const int32_t* shared, int64_t max_prefix, int64_t max_own, void* o,
+                               int o_dtype, void* workspace, size_t ws_bytes, void* stream);
+
 /* out[rows][dim] = x * rsqrt(mean(x^2) + eps) * w (w + 1 when centered), fp32 or bf16 out: the RMSNorm before a
  * prefill GEMM (models/llama.py:82-85), which then takes bf16 rows. */
 int fh_rms_rows(const float* x, int64_t ldx, int64_t rows, int64_t dim, const float* norm_w, float eps, int centered,
@@ -344,6 +378,20 @@ int fh_argmax_parts(const void* parts, int64_t rows, int64_t nparts, int32_t* id
 size_t fh_heads_workspace_bytes(int rows, int64_t vocab, int k);
 int fh_logit_heads(const float* logits, int64_t ldl, int rows, int64_t vocab, int k, const float* inv_temp,
                    float* values, int32_t* ids, float* lse, void* workspace, size_t ws_bytes, void* stream);
+
+/* Each request's rules on its row of logits [rows][ldl] (fp32), before its head: out = pen(x) - frequency n - presence
+ * [n > 0] + bias, and -inf where the row's bit in `allowed` is 0. tokens [rows][ldt]: a row's tokens so far, its prompt's
+ * first, the first lengths[row] of at most max_tokens (lengths NULL: all); a token outside 0 .. vocab - 1 (padding) counts
+ * nowhere. pen(x) = x / repetition for x > 0, else x repetition, where the column is among them; n: its count among those
+ * from prompt_lengths[row] on (NULL: all). repetition, presence, frequency [rows] (NULL: 1, 0, 0). bias_ids and bias
+ * [rows][ldb]: up to 1024 columns a row and what is added to them, an id outside the vocabulary ignored, one given twice
+ * added twice, in the list's order. allowed [rows][ldm]: bit c % 32 of word c / 32 for column c (NULL: all). Each
+ * argument may be NULL. out may be logits itself (ldo = ldl); otherwise they do not overlap. Every sum has one order:
+ * a call repeats its bits. No counterpart in the reference (models/serve.py samples from the plain heads, 31-47). */
+int fh_logit_rules(const float* logits, int64_t ldl, int64_t rows, int64_t vocab, const int32_t* tokens, int64_t ldt,
+                   int64_t max_tokens, const int32_t* lengths, const int32_t* prompt_lengths, const float* repetition,
+                   const float* presence, const float* frequency, const int32_t* bias_ids, const float* bias, int64_t ldb,
+                   int64_t biases, const int32_t* allowed, int64_t ldm, float* out, int64_t ldo, void* stream);
 
 /* out[r][j] = src[r][idx[r][j]] (4-byte elements: int32 or fp32; rows lds, ldi, ldo apart), an index outside
  * [0, cols) read at the nearest column: Tensor.topk's labels, each pick's label instead of its column
