@@ -3,29 +3,151 @@
 // prefix_row + p where p < shared (rows that other sequences read too) and at first_row + p - shared behind them, and a
 // query at place p sees places 0 .. p: o = sum_k softmax_k(q k / sqrt(hd)) v. A query that sees no place gives zeros.
 //
-// A wave a query row and head: 64 keys a round, a lane a key's score, the running max and sum of the softmax (each
-// round rescales what is there), then a lane HD / 64 dimensions of p v.
+// The query heads of a key head read the same keys, so a workgroup takes rows of pairs (query row, head of the group): 32 a
+// wave, 4 waves, one key head; a prompt of 20 rows of 4 heads a key head is one tile of 80 pairs, and a decode step's rows
+// behind one prefix are 32 pairs to 8 rows. It walks the keys its pairs see in tiles staged in LDS, the next tile's loads in
+// flight meanwhile. Scores transposed, S^T = K Q^T, keys down and pairs across: a lane holds one pair's scores, so the
+// softmax's statistics need one exchange between the wave's halves; and P^T is the next product's operand as it lies, O^T +=
+// V^T P^T. The running max of a softmax moves only when a tile's lies more than 2^8 above it: exponents up to 256 lose
+// nothing in fp32 sums or bf16 products, and the output is rescaled a few times a row rather than every tile.
+//
+// Two forms. bf16 (a bf16 or block-float cache, bf16 output): v_mfma_f32_32x32x16_bf16, an fp32 q as two bf16 terms (off by
+// 2^-16 of itself at most; a bf16 q is exact in one), the softmax's weights rounded to bf16 (2^-8 at most, what the output's
+// own rounding adds; their sum is taken before it). fp32 (an fp32 cache or output): v_mfma_f32_32x32x2_f32, nothing rounded.
+//
+// Where tiles are few, the keys are split among workgroups, each leaving its weighted sum, max and sum of weights in the
+// workspace, and a second kernel joins them; a shared prefix is always one of two parts or more, the rows' own keys others.
+//
+// A key that a pair does not see has the weight 0, but 0 times an infinite or NaN value is NaN: a wave whose result is not
+// finite takes its pairs again one at a time over the keys each sees alone (attend_again).
 #include <math.h>
+#include <algorithm>
 #include "fh_common.h"
 
 namespace fh {
 
+typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float floatx16;
+typedef __attribute__((__vector_size__(4 * sizeof(short)))) short short4v;
+#define SEQ_LDS __attribute__((address_space(3)))
+
+constexpr int SQ_NW = 4;               // waves a workgroup
+constexpr int SQ_BQ = 32 * SQ_NW;      // pairs a workgroup
+constexpr float SQ_SLACK = 8.f;        // how far a score may lie above the running max, in base 2
+
 struct SeqArgs {
   const void* q; int q_bf16; int64_t ldq;
   const void* cache; int64_t cache_len; const uint8_t* cache_exps;
-  int heads, kv_heads; float scale;
+  int heads, kv_heads, rep; float scale;
   int64_t rows; int n;          // query rows; sequences
-  const int32_t* starts;        // [n + 1] each sequence's first row (NULL: row b is sequence b)
+  const int32_t* starts;        // [n + 1] each sequence's first row (NULL: a decode step, row b is sequence b)
   const int32_t* places;        // [n] the place of a sequence's first row
   const int32_t* first_row; const int32_t* prefix_row; const int32_t* shared;
   int64_t max_prefix, max_own;  // bounds of shared, and of the places behind it
+  int splits, own_splits;       // workgroups the keys are split among (a decode step's prefix; each row's own keys)
+  int tiles;                    // tiles of pairs (a decode step's prefix)
+  int parts;                    // parts a pair (1: the kernel writes o)
+  float* part;                  // [rows][heads][parts][hd + 2]: weighted sum, max (in base 2), sum of weights
   void* o; int o_bf16, o_tiles; int64_t ldo;
 };
 
-__device__ inline void put_out(const SeqArgs& a, int64_t row, int64_t col, float v) {
+// what a workgroup does: pairs pair0 .. of `pairs` of the rows from row0 on, keys of tiles first .. last of those they see
+struct SeqItem {
+  int64_t row0; int pair0, pairs;   // pair p: row row0 + p / rep, head p % rep of the group
+  int kvh, split, splits, part;
+  int64_t prefix, own; int shared;  // key k's cache row: prefix + k below shared, own + k from there on
+  int place0, step;                 // pair p sees keys 0 .. place0 + step (p / rep) of them; step -1: each row's own count
+};
+
+__device__ inline int clampi(int64_t v, int64_t lo, int64_t hi) { return (int)(v < lo ? lo : v > hi ? hi : v); }
+
+// A row of a decode step: its prefix's places and its own that it sees
+__device__ inline void row_counts(const SeqArgs& a, int64_t b, int& shared, int& in_prefix, int& own) {
+  shared = clampi(a.shared[b], 0, a.max_prefix);
+  const int64_t seen = (int64_t)a.places[b] + 1;
+  in_prefix = clampi(seen, 0, shared);
+  own = clampi(seen - shared, 0, a.max_own);
+}
+
+// The workgroup's item (false: none). Blocks of one key head lie kv_heads apart: with 8 key heads they share an XCD's L2.
+__device__ inline bool seq_item(const SeqArgs& a, SeqItem& it) {
+  int blk = blockIdx.x;
+  it.kvh = blk % a.kv_heads;
+  blk /= a.kv_heads;
+  if (!a.starts) {
+    if (blk < a.tiles * a.splits) {  // the prefix: tiles of all rows' pairs
+      it.split = blk % a.splits; it.splits = a.splits; it.part = it.split;
+      it.row0 = 0; it.pair0 = (blk / a.splits) * SQ_BQ; it.pairs = (int)a.rows * a.rep;
+      it.prefix = a.prefix_row[0]; it.own = 0; it.shared = 0x7FFFFFFF;
+      it.place0 = 0; it.step = -1;
+      return true;
+    }
+    blk -= a.tiles * a.splits;       // a row's own keys
+    const int64_t b = blk / a.own_splits;
+    it.split = blk % a.own_splits; it.splits = a.own_splits; it.part = a.splits + it.split;
+    int sh, pre, own;
+    row_counts(a, b, sh, pre, own);
+    it.row0 = b; it.pair0 = 0; it.pairs = a.rep;
+    it.prefix = 0; it.own = a.first_row[b]; it.shared = 0;
+    it.place0 = own - 1; it.step = 0;
+    return true;
+  }
+  it.split = it.part = blk % a.splits; it.splits = a.splits;
+  const int tile = blk / a.splits, lane = threadIdx.x & 63;
+  int before = 0;
+  for (int s0 = 0; s0 < a.n; s0 += 64) {  // 64 sequences a round: the one whose tiles hold this one
+    const int s = s0 + lane;
+    int lo = 0, len = 0;
+    if (s < a.n) {
+      lo = clampi(a.starts[s], 0, a.rows);
+      len = clampi(a.starts[s + 1], lo, a.rows) - lo;
+    }
+    const int tiles = (int)(((int64_t)len * a.rep + SQ_BQ - 1) / SQ_BQ);
+    int incl = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(incl, d, 64);
+      if (lane >= d) incl += o;
+    }
+    const int total = __shfl(incl, 63, 64);
+    if (tile < before + total) {
+      const uint64_t has = __ballot(tile < before + incl);
+      const int at = __builtin_ctzll(has), sq = s0 + at;
+      const int l0 = __shfl(lo, at, 64), ln = __shfl(len, at, 64), nt = __shfl(tiles, at, 64), in = __shfl(incl, at, 64);
+      const int t = nt - 1 - (tile - (before + in - nt));  // (a sequence's longest tile first)
+      it.row0 = l0; it.pair0 = t * SQ_BQ; it.pairs = ln * a.rep;
+      it.shared = a.shared ? clampi(a.shared[sq], 0, a.max_prefix) : 0;
+      it.prefix = a.shared ? a.prefix_row[0] : 0;
+      it.own = (int64_t)a.first_row[sq] - it.shared;
+      it.place0 = a.places[sq]; it.step = 1;
+      return true;
+    }
+    before += total;
+  }
+  return false;
+}
+
+// how many keys pair p of the item sees
+__device__ inline int pair_limit(const SeqArgs& a, const SeqItem& it, int p) {
+  if (p >= it.pairs) return 0;
+  if (it.step >= 0) return clampi((int64_t)it.place0 + (int64_t)it.step * (p / a.rep) + 1, 0, it.step ? a.max_own : 0x7FFFFFFF);
+  int sh, pre, own;
+  row_counts(a, p / a.rep, sh, pre, own);
+  return pre;
+}
+
+__device__ inline int64_t key_row(const SeqArgs& a, const SeqItem& it, int k) {
+  const int64_t r = (k < it.shared ? it.prefix : it.own) + k;
+  return r < 0 ? 0 : r >= a.cache_len ? a.cache_len - 1 : r;
+}
+
+__device__ inline uint32_t pack2_rne(float lo, float hi) { return bf16_rne_f(lo) | (bf16_rne_f(hi) << 16); }
+
+// four values of a row of o, columns col .. col + 3
+__device__ inline void put4(const SeqArgs& a, int64_t row, int64_t col, float4 v) {
   const int64_t at = a.o_tiles ? tile16_at(row, col, a.ldo) : row * a.ldo + col;
-  if (a.o_bf16) ((uint16_t*)a.o)[at] = (uint16_t)bf16_rne_f(v);
-  else ((float*)a.o)[at] = v;
+  if (a.o_bf16) *(uint2*)((uint16_t*)a.o + at) = make_uint2(pack2_rne(v.x, v.y), pack2_rne(v.z, v.w));
+  else *(float4*)((float*)a.o + at) = v;
 }
 
 // a cache row's value, whatever the cache holds
@@ -42,70 +164,460 @@ __device__ inline float cache_value(const SeqArgs& a, int64_t row, int c) {
   }
 }
 
-// the sequence of row r: the last whose start is at most r, if r lies before its end (-1: none)
-__device__ inline int sequence_of(const SeqArgs& a, int64_t r) {
-  if (!a.starts) return (int)r;
-  for (int s = 0; s < a.n; ++s)
-    if (a.starts[s] <= r && r < a.starts[s + 1]) return s;
-  return -1;
+// 8 values of a cache row as loaded: 16 bytes of bf16, 32 of fp32, or a block float's magnitudes and exponent
+struct SeqRaw { uint4 a, b; uint32_t e; };
+template <int HD, int CF>
+__device__ inline SeqRaw seq_raw(const SeqArgs& a, int64_t row, int c) {
+  SeqRaw r;
+  if constexpr (CF == FH_BF16) r.a = *(const uint4*)((const uint16_t*)a.cache + row * HD + c);
+  else if constexpr (CF == FH_F32) {
+    const uint4* p = (const uint4*)((const float*)a.cache + row * HD + c);
+    r.a = p[0]; r.b = p[1];
+  } else {
+    if constexpr (CF == FH_BFP8) { const uint2 m = *(const uint2*)((const uint8_t*)a.cache + row * HD + c); r.a.x = m.x; r.a.y = m.y; }
+    else r.a.x = *(const uint32_t*)((const uint8_t*)a.cache + row * (HD / 2) + c / 2);
+    r.e = a.cache_exps[row * (HD / 16) + c / 16];
+  }
+  return r;
+}
+template <int CF>
+__device__ inline uint4 seq_bf16x8(const SeqRaw& r) {
+  static_assert(CF != FH_F32, "an fp32 cache goes in as fp32");
+  if constexpr (CF == FH_BF16) return r.a;
+  else {
+    float f[8];
+    uint32_t w[4];
+    if constexpr (CF == FH_BFP8) magnitudes8(make_uint2(r.a.x, r.a.y), f);
+    else magnitudes8(r.a.x, f);
+    bfp_run_bf16<8>(f, r.e, w);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+template <int CF>
+__device__ inline void seq_f32x8(const SeqRaw& r, float4& x, float4& y) {
+  if constexpr (CF == FH_F32) {
+    x = make_float4(__uint_as_float(r.a.x), __uint_as_float(r.a.y), __uint_as_float(r.a.z), __uint_as_float(r.a.w));
+    y = make_float4(__uint_as_float(r.b.x), __uint_as_float(r.b.y), __uint_as_float(r.b.z), __uint_as_float(r.b.w));
+  } else {
+    const uint4 w = seq_bf16x8<CF>(r);
+    x = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
+    y = make_float4(__uint_as_float(w.z << 16), __uint_as_float(w.z & 0xFFFF0000u), __uint_as_float(w.w << 16), __uint_as_float(w.w & 0xFFFF0000u));
+  }
+}
+
+__device__ inline float q_value(const SeqArgs& a, int64_t at) {
+  return a.q_bf16 ? bf16_to_f(((const uint16_t*)a.q)[at]) : ((const float*)a.q)[at];
+}
+// 8 of a row of q
+__device__ inline void q8(const SeqArgs& a, int64_t at, float (&f)[8]) {
+  if (a.q_bf16) {
+    const uint4 w = *(const uint4*)((const uint16_t*)a.q + at);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(u[i] << 16); f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u); }
+  } else {
+    const float4 u = *(const float4*)((const float*)a.q + at), v = *(const float4*)((const float*)a.q + at + 4);
+    f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w; f[4] = v.x; f[5] = v.y; f[6] = v.z; f[7] = v.w;
+  }
+}
+
+__device__ inline float* part_of(const SeqArgs& a, int64_t row, int h, int part, int hd) {
+  return a.part + (((row * a.heads + h) * a.parts) + part) * (hd + 2);
+}
+
+// The wave's pairs again, one at a time over the keys k0 .. k1 - 1 that each sees and no other: a lane a key's score, then a
+// lane HD / 64 dimensions of p v.
+template <int HD, int CF>
+__device__ void attend_again(const SeqArgs& a, const SeqItem& it, int wpair, int k0, int k1) {
+  const int lane = threadIdx.x & 63;
+  for (int i = 0; i < 32 && wpair + i < it.pairs; ++i) {
+    const int p = wpair + i, h = it.kvh * a.rep + p % a.rep, end = min(pair_limit(a, it, p), k1);
+    const int64_t row = it.row0 + p / a.rep, qat = row * a.ldq + (int64_t)h * HD;
+    float m = -INFINITY, l = 0.f, o[HD / 64];
+    for (int d = 0; d < HD / 64; ++d) o[d] = 0.f;
+    for (int k = k0; k < end; k += 64) {
+      float sc = -INFINITY;
+      if (k + lane < end) {
+        const int64_t r = (int64_t)it.kvh * a.cache_len + key_row(a, it, k + lane);
+        sc = 0.f;
+        for (int c = 0; c < HD; ++c) sc = fmaf(q_value(a, qat + c), cache_value<HD, CF>(a, r, c), sc);
+        sc *= a.scale * 1.44269504088896341f;
+      }
+      const float mn = fmaxf(m, wave_max(sc));
+      const float pr = k + lane < end ? exp2f(sc - (mn == -INFINITY ? 0.f : mn)) : 0.f, f = m == -INFINITY ? 0.f : exp2f(m - mn);
+      l = l * f + wave_sum(pr);
+      m = mn;
+      for (int d = 0; d < HD / 64; ++d) o[d] *= f;
+      for (int j = 0; j < min(64, end - k); ++j) {
+        const float pj = __shfl(pr, j, 64);
+        const int64_t r = (int64_t)(a.kv_heads + it.kvh) * a.cache_len + key_row(a, it, k + j);
+        for (int d = 0; d < HD / 64; ++d) o[d] = fmaf(pj, cache_value<HD, CF>(a, r, lane + 64 * d), o[d]);
+      }
+    }
+    if (a.parts > 1) {
+      float* pp = part_of(a, row, h, it.part, HD);
+      for (int d = 0; d < HD / 64; ++d) pp[lane + 64 * d] = o[d];
+      if (lane == 0) { pp[HD] = m; pp[HD + 1] = m == -INFINITY && end > k0 ? 1.f : l; }
+    } else {
+      for (int d = 0; d < HD / 64; ++d) {
+        const int64_t col = (int64_t)h * HD + lane + 64 * d, at = a.o_tiles ? tile16_at(row, col, a.ldo) : row * a.ldo + col;
+        const float v = end > k0 ? o[d] / l : 0.f;
+        if (a.o_bf16) ((uint16_t*)a.o)[at] = (uint16_t)bf16_rne_f(v);
+        else ((float*)a.o)[at] = v;
+      }
+    }
+  }
+}
+
+// A wave's result: lane (ql, hh) holds dimensions 32 d + 8 (r / 4) + 4 hh + r % 4 of pair wpair + ql
+template <int HD, int CF>
+__device__ inline void seq_finish(const SeqArgs& a, const SeqItem& it, int wpair, int limit, int k0, int k1, floatx16 (&acc)[HD / 32], float m, float l) {
+  const int lane = threadIdx.x & 63, ql = lane & 31, hh = lane >> 5, p = wpair + ql;
+  float big = l;  // (0 times a sum that is not finite: NaN)
+#pragma unroll
+  for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) big = fmaf(acc[d][r], 0.f, big);
+  if (__any(!(fabsf(big) < INFINITY))) { attend_again<HD, CF>(a, it, wpair, k0, k1); return; }
+  if (p >= it.pairs) return;
+  const int64_t row = it.row0 + p / a.rep;
+  const int h = it.kvh * a.rep + p % a.rep;
+  if (a.parts > 1) {
+    float* pp = part_of(a, row, h, it.part, HD);
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float2* to = (float2*)(pp + 32 * d + 8 * g + 4 * hh);  // (8-byte aligned: hd + 2 floats a part)
+        to[0] = make_float2(acc[d][4 * g], acc[d][4 * g + 1]);
+        to[1] = make_float2(acc[d][4 * g + 2], acc[d][4 * g + 3]);
+      }
+    // (a part whose keys all score -inf: no weight beside others, NaN alone; a part without keys: a sum of 0)
+    if (hh == 0) *(float2*)(pp + HD) = make_float2(m, m == -INFINITY && limit > k0 ? 1.f : l);
+    return;
+  }
+  const float inv = limit > 0 ? 1.f / l : 0.f;
+#pragma unroll
+  for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      put4(a, row, (int64_t)h * HD + 32 * d + 8 * g + 4 * hh,
+           make_float4(acc[d][4 * g] * inv, acc[d][4 * g + 1] * inv, acc[d][4 * g + 2] * inv, acc[d][4 * g + 3] * inv));
+}
+
+// The softmax of a tile's NB blocks of 32 keys from key k0: scores in, weights out; the running max (base 2), the sum and
+// the output's rescaling
+template <int HD, int NB>
+__device__ inline void seq_softmax(floatx16 (&s)[NB], int k0, int limit, int wave_min, int hh, float scale2, float& m, float& l, floatx16 (&acc)[HD / 32]) {
+  if (k0 + 32 * NB > wave_min) {  // (some pair of the wave does not see all of the tile)
+    const int left = limit - k0 - 4 * hh;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[b][r] = 32 * b + 8 * (r >> 2) + (r & 3) < left ? s[b][r] : -INFINITY;
+  }
+  float mt = -INFINITY;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[b][r]);
+  mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * scale2;
+  if (__any(mt > m + SQ_SLACK)) {
+    const float mn = fmaxf(m, mt), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= f;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+  }
+  const float shift = m == -INFINITY ? 0.f : m;  // (no key seen so far: every weight 0)
+  float sum = 0.f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(s[b][r], scale2, -shift));
+      s[b][r] = p;
+      sum += p;
+    }
+  l += sum;  // (this half's keys; the halves meet at the end)
+}
+
+// what both forms do around their tiles: the item, the pair of each lane, the tiles of its keys
+#define SEQ_BEGIN(BK) \
+  SeqItem it; \
+  if (!seq_item(a, it)) return; \
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ql = lane & 31, hh = lane >> 5; \
+  if (it.pair0 >= it.pairs) return; \
+  const int wpair = it.pair0 + 32 * wave, pair = min(wpair + ql, it.pairs - 1); \
+  const int limit = wpair + ql < it.pairs ? pair_limit(a, it, pair) : 0; \
+  int wave_max = limit, wave_min = wpair + ql < it.pairs ? limit : 0x7FFFFFFF; \
+  for (int d = 1; d < 32; d <<= 1) { wave_max = max(wave_max, __shfl_xor(wave_max, d, 64)); wave_min = min(wave_min, __shfl_xor(wave_min, d, 64)); } \
+  wave_max = __builtin_amdgcn_readfirstlane(wave_max); wave_min = __builtin_amdgcn_readfirstlane(wave_min); \
+  __shared__ int tops[SQ_NW]; \
+  if (lane == 0) tops[wave] = wave_max; \
+  __syncthreads(); \
+  int keys = tops[0]; \
+  for (int w = 1; w < SQ_NW; ++w) keys = max(keys, tops[w]); \
+  const int ntiles = (keys + BK - 1) / BK; \
+  const int t0 = (int)((int64_t)ntiles * it.split / it.splits), t1 = (int)((int64_t)ntiles * (it.split + 1) / it.splits); \
+  const int64_t qat = (it.row0 + pair / a.rep) * a.ldq + (int64_t)(it.kvh * a.rep + pair % a.rep) * HD; \
+  const float scale2 = a.scale * 1.44269504088896341f; \
+  const int64_t kplane = (int64_t)it.kvh * a.cache_len, vplane = (int64_t)(a.kv_heads + it.kvh) * a.cache_len; \
+  floatx16 acc[HD / 32]; \
+  for (int d = 0; d < HD / 32; ++d) for (int r = 0; r < 16; ++r) acc[d][r] = 0.f; \
+  float m = -INFINITY, l = 0.f;
+
+template <int HD, int CF, int QT>
+__global__ __launch_bounds__(64 * SQ_NW, 2) void seq_bf16_kernel(SeqArgs a) {
+  constexpr int BK = 64, KLD = HD + 8, VLD = HD + 32;  // (a row's 16-byte reads, and 4 rows' transposed reads, on distinct banks)
+  __shared__ __attribute__((aligned(16))) uint16_t Ks[2][BK * KLD];
+  __shared__ __attribute__((aligned(16))) uint16_t Vs[2][BK * VLD];
+  SEQ_BEGIN(BK)
+
+  // the lane's q as the product's B: step s holds dimensions 16 s + 8 hh .. + 7, each term
+  bf16x8 qf[HD / 16][QT];
+#pragma unroll
+  for (int s = 0; s < HD / 16; ++s) {
+    float f[8];
+    q8(a, qat + 16 * s + 8 * hh, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const __bf16 t = (__bf16)f[i];
+      qf[s][0][i] = t;
+      if (QT > 1) qf[s][QT - 1][i] = (__bf16)(f[i] - (float)t);
+    }
+  }
+
+  constexpr int NP = BK * HD / 8 / (64 * SQ_NW);  // pieces of 8 a thread
+  SeqRaw kraw[NP], vraw[NP];
+  auto load = [&](int t) {
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      const int i = tid + 64 * SQ_NW * j, r = i / (HD / 8), c = (i % (HD / 8)) * 8;
+      const int64_t row = key_row(a, it, min(t * BK + r, keys - 1));
+      kraw[j] = seq_raw<HD, CF>(a, kplane + row, c);
+      vraw[j] = seq_raw<HD, CF>(a, vplane + row, c);
+    }
+  };
+  auto store = [&](int b) {
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      const int i = tid + 64 * SQ_NW * j, r = i / (HD / 8), c = (i % (HD / 8)) * 8;
+      *(uint4*)(Ks[b] + r * KLD + c) = seq_bf16x8<CF>(kraw[j]);
+      *(uint4*)(Vs[b] + r * VLD + c) = seq_bf16x8<CF>(vraw[j]);
+    }
+  };
+  if (t0 < t1) { load(t0); store(0); }
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const int b = (t - t0) & 1, k0 = t * BK;
+    if (t + 1 < t1) load(t + 1);
+    if (k0 < wave_max) {
+      floatx16 s[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+#pragma unroll
+      for (int st = 0; st < HD / 16; ++st)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const bf16x8 kf = *(const bf16x8*)(Ks[b] + (32 * kb + ql) * KLD + 16 * st + 8 * hh);
+#pragma unroll
+          for (int u = 0; u < QT; ++u) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st][u], s[kb], 0, 0, 0);
+        }
+      seq_softmax<HD, 2>(s, k0, limit, wave_min, hh, scale2, m, l, acc);
+      // O^T += V^T P^T, 16 keys a step: the lane's weights 8 j .. 8 j + 7 of block kb are keys 32 kb + 16 j + {4 hh .. 4 hh + 3,
+      // 8 + 4 hh .. 8 + 4 hh + 3}; V's columns come transposed, 4 keys of 16 dimensions to 16 lanes
+      SEQ_LDS short4v* vt = (SEQ_LDS short4v*)(Vs[b] + (4 * hh + ((lane & 15) >> 2)) * VLD + (lane & 16) + 4 * (lane & 3));
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          bf16x8 pf;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pf[i] = (__bf16)s[kb][8 * j + i];
+          const int g = 32 * kb + 16 * j;
+#pragma unroll
+          for (int d = 0; d < HD / 32; ++d) {
+            const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(vt + (g * VLD + 32 * d) / 4);
+            const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(vt + ((g + 8) * VLD + 32 * d) / 4);
+            const short v8[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)v8, pf, acc[d], 0, 0, 0);
+          }
+        }
+    }
+    if (t + 1 < t1) store(1 - b);  // (the other buffer: its last readers passed the previous barrier)
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32, 64);
+  seq_finish<HD, CF>(a, it, wpair, limit, t0 * BK, min(t1 * BK, keys), acc, m, l);
+}
+
+// The same in fp32: 32 keys a tile. A lane's q holds dimensions HD / 2 hh .. of its half (the order of a sum's products is free),
+// so that K's row is read 16 bytes at a time; P's step r multiplies keys 8 (r / 4) + 4 hh + r % 4, V's rows as they lie.
+template <int HD, int CF>
+__global__ __launch_bounds__(64 * SQ_NW, 2) void seq_f32_kernel(SeqArgs a) {
+  constexpr int BK = 32, LD = HD + 4;
+  __shared__ __attribute__((aligned(16))) float Ks[2][BK * LD];
+  __shared__ __attribute__((aligned(16))) float Vs[2][BK * LD];
+  SEQ_BEGIN(BK)
+  float qf[HD / 2];
+#pragma unroll
+  for (int s = 0; s < HD / 16; ++s) {
+    float f[8];
+    q8(a, qat + (HD / 2) * hh + 8 * s, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) qf[8 * s + i] = f[i];
+  }
+  constexpr int NP = BK * HD / 8 / (64 * SQ_NW);
+  SeqRaw kraw[NP], vraw[NP];
+  auto load = [&](int t) {
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      const int i = tid + 64 * SQ_NW * j, r = i / (HD / 8), c = (i % (HD / 8)) * 8;
+      const int64_t row = key_row(a, it, min(t * BK + r, keys - 1));
+      kraw[j] = seq_raw<HD, CF>(a, kplane + row, c);
+      vraw[j] = seq_raw<HD, CF>(a, vplane + row, c);
+    }
+  };
+  auto store = [&](int b) {
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      const int i = tid + 64 * SQ_NW * j, r = i / (HD / 8), c = (i % (HD / 8)) * 8;
+      float4* k = (float4*)(Ks[b] + r * LD + c);
+      float4* v = (float4*)(Vs[b] + r * LD + c);
+      seq_f32x8<CF>(kraw[j], k[0], k[1]);
+      seq_f32x8<CF>(vraw[j], v[0], v[1]);
+    }
+  };
+  if (t0 < t1) { load(t0); store(0); }
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const int b = (t - t0) & 1, k0 = t * BK;
+    if (t + 1 < t1) load(t + 1);
+    if (k0 < wave_max) {
+      floatx16 s[1];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+      const float* kr = Ks[b] + ql * LD + (HD / 2) * hh;
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) {
+        const float4 kf = *(const float4*)(kr + 4 * c);
+        s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.x, qf[4 * c], s[0], 0, 0, 0);
+        s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.y, qf[4 * c + 1], s[0], 0, 0, 0);
+        s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.z, qf[4 * c + 2], s[0], 0, 0, 0);
+        s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.w, qf[4 * c + 3], s[0], 0, 0, 0);
+      }
+      seq_softmax<HD, 1>(s, k0, limit, wave_min, hh, scale2, m, l, acc);
+      const float* vr = Vs[b] + 4 * hh * LD + ql;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vr[(8 * (r >> 2) + (r & 3)) * LD + 32 * d], s[0][r], acc[d], 0, 0, 0);
+    }
+    if (t + 1 < t1) store(1 - b);
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32, 64);
+  seq_finish<HD, CF>(a, it, wpair, limit, t0 * BK, min(t1 * BK, keys), acc, m, l);
+}
+
+// A pair's parts joined, a wave a pair: lane p holds part p's statistics, then a lane HD / 64 dimensions of each part's sum,
+// times 2^(its max - the largest). A part that saw no key (its max -inf) has no weight; a pair with none gives zeros. Parts
+// of rows that are no sequence's were never written and are not read.
+template <int HD>
+__global__ __launch_bounds__(256) void seq_join(SeqArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= a.rows * a.heads) return;
+  const int64_t row = i / a.heads;
+  const int h = (int)(i % a.heads);
+  if (a.starts && (row < a.starts[0] || row >= a.starts[a.n])) return;
+  const float* pp = part_of(a, row, h, 0, HD);
+  const bool in = lane < a.parts;
+  const float2 st = in ? *(const float2*)(pp + (int64_t)lane * (HD + 2) + HD) : make_float2(-INFINITY, 0.f);
+  float o[HD / 64];
+  const float top = wave_max(st.x);
+  // (a max that is NaN or +inf makes the sum NaN, as one softmax over all keys would)
+  const bool none = st.y == 0.f && st.x == -INFINITY;
+  const float w = none ? 0.f : __builtin_amdgcn_exp2f(st.x - top);
+  const float den = wave_sum(none ? 0.f : w * st.y);
+#pragma unroll
+  for (int d = 0; d < HD / 64; ++d) o[d] = 0.f;
+  const uint64_t some = __ballot(!none && in);
+  for (int p0 = 0; p0 < a.parts; p0 += 8) {
+    float v[8][HD / 64];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int d = 0; d < HD / 64; ++d) v[u][d] = pp[(int64_t)min(p0 + u, a.parts - 1) * (HD + 2) + lane * (HD / 64) + d];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float wp = __shfl(w, (p0 + u) & 63, 64);
+      if (p0 + u < a.parts && (some >> (p0 + u) & 1))
+#pragma unroll
+        for (int d = 0; d < HD / 64; ++d) o[d] = fmaf(wp, v[u][d], o[d]);
+    }
+  }
+  const int64_t col = (int64_t)h * HD + lane * (HD / 64), at = a.o_tiles ? tile16_at(row, col, a.ldo) : row * a.ldo + col;
+  const float inv = some ? 1.f / den : 0.f;
+#pragma unroll
+  for (int d = 0; d < HD / 64; ++d) {
+    if (a.o_bf16) ((uint16_t*)a.o)[at + d] = (uint16_t)bf16_rne_f(o[d] * inv);
+    else ((float*)a.o)[at + d] = o[d] * inv;
+  }
 }
 
 template <int HD, int CF>
-__global__ __launch_bounds__(64) void seq_attention_kernel(SeqArgs a) {
-  __shared__ float qs[HD];
-  const int64_t row = blockIdx.x;
-  const int h = blockIdx.y, lane = threadIdx.x;
-  const int s = sequence_of(a, row);
-  if (s < 0) return;
-  const int64_t shared = a.shared ? min(max((int64_t)a.shared[s], (int64_t)0), a.max_prefix) : 0;
-  const int64_t place = a.places[s] + (a.starts ? row - a.starts[s] : 0);
-  const int64_t keys = min(place + 1, shared + a.max_own);
-  const int64_t first = (int64_t)a.first_row[s] - shared, prefix = a.prefix_row ? *a.prefix_row : 0;
-  const int kvh = h / (a.heads / a.kv_heads);
-  for (int i = lane; i < HD; i += 64) {
-    const int64_t at = row * a.ldq + (int64_t)h * HD + i;
-    qs[i] = a.q_bf16 ? bf16_to_f(((const uint16_t*)a.q)[at]) : ((const float*)a.q)[at];
-  }
-  __syncthreads();
-  auto cache_row = [&](int64_t k) {
-    const int64_t r = k < shared ? prefix + k : first + k;
-    return min(max(r, (int64_t)0), a.cache_len - 1);
-  };
-  float m = -INFINITY, l = 0.f, o[HD / 64];
-  for (int i = 0; i < HD / 64; ++i) o[i] = 0.f;
-  for (int64_t k0 = 0; k0 < keys; k0 += 64) {
-    const bool in = k0 + lane < keys;
-    float sc = -INFINITY;
-    if (in) {
-      const int64_t r = (int64_t)kvh * a.cache_len + cache_row(k0 + lane);
-      sc = 0.f;
-      for (int c = 0; c < HD; ++c) sc = fmaf(qs[c], cache_value<HD, CF>(a, r, c), sc);
-      sc *= a.scale;
+static void launch_seq(unsigned blocks, hipStream_t s, const SeqArgs& a) {
+  const dim3 g(blocks), b(64 * SQ_NW);
+  if constexpr (CF != FH_F32)
+    if (a.o_bf16) {
+      if (a.q_bf16) hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 1>), g, b, 0, s, a);
+      else hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 2>), g, b, 0, s, a);
+      return;
     }
-    const float mn = fmaxf(m, wave_max(sc));
-    const float p = in ? expf(sc - mn) : 0.f, f = m == -INFINITY ? 0.f : expf(m - mn);
-    l = l * f + wave_sum(p);
-    m = mn;
-    for (int i = 0; i < HD / 64; ++i) o[i] *= f;
-    const int n = (int)min((int64_t)64, keys - k0);
-    for (int j = 0; j < n; ++j) {
-      const float pj = __shfl(p, j, 64);
-      const int64_t r = (int64_t)(a.kv_heads + kvh) * a.cache_len + cache_row(k0 + j);
-      for (int i = 0; i < HD / 64; ++i) o[i] = fmaf(pj, cache_value<HD, CF>(a, r, lane + 64 * i), o[i]);
-    }
-  }
-  for (int i = 0; i < HD / 64; ++i) put_out(a, row, (int64_t)h * HD + lane + 64 * i, keys > 0 ? o[i] / l : 0.f);
+  hipLaunchKernelGGL((seq_f32_kernel<HD, CF>), g, b, 0, s, a);
 }
 
 template <int HD>
-static void launch_seq(int cf, hipStream_t s, const SeqArgs& a) {
-  const dim3 g((unsigned)a.rows, a.heads), b(64);
+static void launch_seq(int cf, unsigned blocks, hipStream_t s, const SeqArgs& a) {
   switch (cf) {
-    case FH_F32: hipLaunchKernelGGL((seq_attention_kernel<HD, FH_F32>), g, b, 0, s, a); break;
-    case FH_BF16: hipLaunchKernelGGL((seq_attention_kernel<HD, FH_BF16>), g, b, 0, s, a); break;
-    case FH_BFP8: hipLaunchKernelGGL((seq_attention_kernel<HD, FH_BFP8>), g, b, 0, s, a); break;
-    default: hipLaunchKernelGGL((seq_attention_kernel<HD, FH_BFP4>), g, b, 0, s, a); break;
+    case FH_F32: launch_seq<HD, FH_F32>(blocks, s, a); break;
+    case FH_BF16: launch_seq<HD, FH_BF16>(blocks, s, a); break;
+    case FH_BFP8: launch_seq<HD, FH_BFP8>(blocks, s, a); break;
+    default: launch_seq<HD, FH_BFP4>(blocks, s, a); break;
   }
+  if (a.parts > 1) hipLaunchKernelGGL(seq_join<HD>, dim3((unsigned)((a.rows * a.heads + 3) / 4)), dim3(256), 0, s, a);
+}
+
+static int launch_seq(const char* fn, int head_dim, int cf, int64_t blocks, hipStream_t s, const SeqArgs& a) {
+  if (blocks >= (1LL << 31) || (a.rows * a.heads + 3) / 4 >= (1LL << 31)) { set_error("%s: too many rows for one grid", fn); return FH_EUNSUP; }
+  if (head_dim == 128) launch_seq<128>(cf, (unsigned)blocks, s, a);
+  else launch_seq<64>(cf, (unsigned)blocks, s, a);
+  return check_launch(fn);
+}
+
+// Workgroups the keys of a tile are split among: enough that the grid has two a CU, each with 4 tiles of 64 keys or more,
+// at most 32 (a wave joins the parts, a lane each)
+constexpr int SQ_CUS = 256, SQ_SPLIT_KEYS = 256, SQ_MAX_SPLITS = 32;
+static int splits_for(int64_t groups, int64_t keys) {
+  if (groups >= SQ_CUS) return 1;
+  const int64_t s = (2 * SQ_CUS + groups - 1) / groups;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({s, keys / SQ_SPLIT_KEYS, SQ_MAX_SPLITS}));
+}
+static int64_t packed_tiles(int64_t rows, int n, int rep) { return rows * rep / SQ_BQ + std::min<int64_t>(n, rows); }
+static int packed_splits(int64_t rows, int n, int heads, int kv_heads, int64_t max_context) {
+  return splits_for(packed_tiles(rows, n, heads / kv_heads) * kv_heads, max_context);
+}
+static void shared_splits(int batch, int heads, int kv_heads, int64_t max_prefix, int64_t max_own, int& tiles, int& prefix, int& own) {
+  tiles = (int)(((int64_t)batch * (heads / kv_heads) + SQ_BQ - 1) / SQ_BQ);
+  prefix = splits_for((int64_t)tiles * kv_heads, max_prefix);
+  own = splits_for((int64_t)batch * kv_heads, max_own);
 }
 
 // what both entry points ask of their operands (fn: the name in the message)
@@ -118,6 +630,7 @@ static int seq_check(const char* fn, const SeqArgs& a, int q_dtype, int cache_dt
   if (q_dtype != FH_F32 && q_dtype != FH_BF16) return no(FH_EINVAL, "q is FH_F32 or FH_BF16");
   if (cache_dtype < FH_F32 || cache_dtype > FH_BFP4) return no(FH_EUNSUP, "cache is FH_F32, FH_BF16, FH_BFP8 or FH_BFP4");
   if (a.cache_len < 1) return no(FH_EINVAL, "cache_len at least 1");
+  if (a.rows * (a.heads / a.kv_heads) >= (1LL << 31) || a.cache_len >= (1LL << 31)) return no(FH_EUNSUP, "fewer than 2^31 cache rows and pairs of a row and a key head's heads");
   if ((a.shared == nullptr) != (a.prefix_row == nullptr)) return no(FH_EINVAL, "prefix_row and shared go together");
   const int64_t cols = (int64_t)a.heads * head_dim;
   if (a.ldq < cols || a.ldo < cols || a.ldq % (q_dtype == FH_F32 ? 4 : 8) || (o_dtype != FH_BF16_T16 && a.ldo % 4) ||
@@ -132,7 +645,9 @@ using namespace fh;
 
 extern "C" size_t fh_attention_packed_workspace_bytes(int64_t rows, int sequences, int heads, int kv_heads, int head_dim,
                                                       int64_t max_context) {
-  return 0;
+  if (rows < 1 || sequences < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || max_context < 1) return 0;
+  const int s = packed_splits(rows, sequences, heads, kv_heads, max_context);
+  return s == 1 ? 0 : (size_t)rows * heads * s * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int fh_attention_prefill_packed(const void* q, int q_dtype, int64_t ldq, const void* cache, int cache_dtype,
@@ -152,16 +667,22 @@ extern "C" int fh_attention_prefill_packed(const void* q, int q_dtype, int64_t l
     return fail(FH_EINVAL, "fh_attention_prefill_packed: need 1 <= rows < 2^31, sequences >= 1 and max_context >= 1");
   if (o_dtype != FH_F32 && o_dtype != FH_BF16) return fail(FH_EINVAL, "fh_attention_prefill_packed: o is FH_F32 or FH_BF16");
   if (int rc = seq_check(fn, a, q_dtype, cache_dtype, head_dim, o_dtype)) return rc;
+  a.rep = heads / kv_heads;
   a.cache_exps = (const uint8_t*)cache + kv_exps_at(cache_dtype, kv_heads, cache_len, head_dim);
   a.scale = 1.0f / sqrtf((float)head_dim);
-  if (head_dim == 128) launch_seq<128>(cache_dtype, as_stream(stream), a);
-  else launch_seq<64>(cache_dtype, as_stream(stream), a);
-  return check_launch(fn);
+  a.splits = a.parts = packed_splits(rows, sequences, heads, kv_heads, max_context);
+  a.part = (float*)workspace;
+  if (a.parts > 1 && (!workspace || ws_bytes < fh_attention_packed_workspace_bytes(rows, sequences, heads, kv_heads, head_dim, max_context) || ((uintptr_t)workspace & 15)))
+    return fail(FH_EINVAL, "fh_attention_prefill_packed: a 16-byte aligned workspace of fh_attention_packed_workspace_bytes");
+  return launch_seq(fn, head_dim, cache_dtype, packed_tiles(rows, sequences, a.rep) * a.splits * kv_heads, as_stream(stream), a);
 }
 
 extern "C" size_t fh_attention_shared_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int64_t max_prefix,
                                                       int64_t max_own) {
-  return 0;
+  if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || max_prefix < 0 || max_own < 0) return 0;
+  int tiles, prefix, own;
+  shared_splits(batch, heads, kv_heads, max_prefix, max_own, tiles, prefix, own);
+  return (size_t)batch * heads * (prefix + own) * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int fh_attention_decode_shared(const void* q, int q_dtype, const void* cache, int cache_dtype, int64_t cache_len,
@@ -182,9 +703,13 @@ extern "C" int fh_attention_decode_shared(const void* q, int q_dtype, const void
   if (o_dtype != FH_F32 && o_dtype != FH_BF16 && o_dtype != FH_BF16_T16)
     return fail(FH_EINVAL, "fh_attention_decode_shared: o is FH_F32, FH_BF16 or FH_BF16_T16");
   if (int rc = seq_check(fn, a, q_dtype, cache_dtype, head_dim, o_dtype)) return rc;
+  a.rep = heads / kv_heads;
   a.cache_exps = (const uint8_t*)cache + kv_exps_at(cache_dtype, kv_heads, cache_len, head_dim);
   a.scale = 1.0f / sqrtf((float)head_dim);
-  if (head_dim == 128) launch_seq<128>(cache_dtype, as_stream(stream), a);
-  else launch_seq<64>(cache_dtype, as_stream(stream), a);
-  return check_launch(fn);
+  shared_splits(batch, heads, kv_heads, max_prefix, max_own, a.tiles, a.splits, a.own_splits);
+  a.parts = a.splits + a.own_splits;
+  a.part = (float*)workspace;
+  if (!workspace || ws_bytes < fh_attention_shared_workspace_bytes(batch, heads, kv_heads, head_dim, max_prefix, max_own) || ((uintptr_t)workspace & 15))
+    return fail(FH_EINVAL, "fh_attention_decode_shared: a 16-byte aligned workspace of fh_attention_shared_workspace_bytes");
+  return launch_seq(fn, head_dim, cache_dtype, ((int64_t)a.tiles * a.splits + (int64_t)batch * a.own_splits) * kv_heads, as_stream(stream), a);
 }
