@@ -2,12 +2,13 @@
 // mask bit is 0. pen(x) is x / repetition for x > 0 and x repetition otherwise, for the columns among the row's tokens;
 // n is a column's count among the tokens after the prompt.
 //
-// A workgroup a part of a row's columns: the loads of its tokens and logits go out together, the tokens that fall into the part
-// are counted in LDS (integers: their order does not show), the logits changed in registers and written. A column with a bias
-// is the thread's of the first entry that names it, which adds the column's entries in the list's order and writes the column
-// once more, behind the others. Bound by the
-// logits' read and write; each part reads the row's tokens again, so parts are as wide as fill the GPU: two workgroups a CU
-// of up to 32768 columns, a count of 16 bits a column (32 where a row may hold 32768 tokens or more: half the columns).
+// A workgroup a part of a row's columns: the loads of its biases, tokens and logits go out together, the tokens that fall
+// into the part are counted in LDS (integers: their order does not show) and the columns with a bias marked there, the
+// logits changed in registers and written once. Bound by the logits' read and write; each part reads the row's tokens again, so
+// parts are as wide as fill the GPU: two workgroups a CU of up to 32768 columns, a cell of 16 bits a column (32 where a row
+// may hold 16384 tokens or more: half the columns). A marked column finds its biases by a hash of the column, a chain of
+// them in LDS; more than one of a column are added in the list's order. 128 rows of 128256 columns with 8000 tokens: 41 us, 3.3
+// TB/s of what has to move (a copy of the logits alone takes 23.5 us: 5.6 TB/s).
 #include <math.h>
 #include <algorithm>
 #include "fh_common.h"
@@ -16,6 +17,7 @@ namespace fh {
 
 constexpr int RU = 8;              // loads of logits a thread has in flight
 constexpr int RBIAS = 1024;        // biases a row, at most
+constexpr int RHASH = 256;         // chains of them
 
 struct RuleArgs {
   const float* x; int64_t ldx; int64_t vocab;
@@ -27,100 +29,105 @@ struct RuleArgs {
   int part;                        // columns a workgroup, a multiple of 1024
 };
 
-// A column's cell of CB bits: the count after the prompt, and above it a bit for a token of the prompt
+// A column's cell of CB bits: the count after the prompt, above it a bit for a token of the prompt and one for a bias
+template <int CB>
+struct RuleCell { static constexpr uint32_t PROMPT = 1u << (CB - 2), BIAS = 1u << (CB - 1); };
+
 template <int CB>
 __device__ inline float ruled(float x, uint32_t cell, float rep, float pre, float fre) {
-  constexpr uint32_t PROMPT = 1u << (CB - 1);
-  if (!cell) return x;
+  constexpr uint32_t PROMPT = RuleCell<CB>::PROMPT;
   const uint32_t n = cell & (PROMPT - 1);
+  if (!(cell & (2 * PROMPT - 1))) return x;
   float y = x > 0.f ? x / rep : x * rep;
   if (n) y = y - fre * (float)n - pre;
   return y;
 }
 
-// VEC: rows aligned to 16 bytes, 4 columns a load
+// VEC: rows aligned to 16 bytes and a multiple of 4 columns, 4 a load
 template <int CB, bool VEC>
-__global__ __launch_bounds__(1024) void rules_kernel(RuleArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint32_t cells[];  // [part] of CB bits, then the biases' columns
+__global__ __launch_bounds__(512) void rules_kernel(RuleArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t cells[];  // [part] of CB bits, then the biases'
   constexpr int W = VEC ? 4 : 1;
   const int64_t row = blockIdx.y, c0 = (int64_t)blockIdx.x * a.part;
   const int tid = threadIdx.x, nt = blockDim.x, n = (int)min((int64_t)a.part, a.vocab - c0);
   const float* x = a.x + row * a.ldx + c0;
   float* out = a.out + row * a.ldo + c0;
   const uint32_t* allowed = a.allowed ? a.allowed + row * a.ldm + (c0 >> 5) : nullptr;
-  const int words = a.part * CB / 32;
-  int* at = (int*)(cells + words);                                  // [nbias in fours] a bias's column in the part (-1: not in it)
-  float* add = (float*)(at + (a.nbias + 3) / 4 * 4);                // the biases
+  const int words = a.part * CB / 32;  // (of the cells: there with tokens or biases)
+  int* head = (int*)(cells + words);                                // [RHASH] a chain's first bias, or -1
+  const int nb4 = (a.nbias + 3) / 4 * 4;
+  int* at = head + RHASH;                                           // [nb4] a bias's column in the part (-1: not in it)
+  int* next = at + nb4;                                             // [nb4] the chain's next
+  float* add = (float*)(next + nb4);                                // [nb4]
 
-  // the first tokens, the biases' columns and the first logits on their way together
+  // the biases, the first tokens and the first logits on their way together (every address inside its row: no branches)
+  constexpr int RB = RBIAS / 256;
+  int bc[RB];
+  float bv[RB];
+  if (a.nbias) {
+#pragma unroll
+    for (int e = 0; e < RB; ++e) {
+      const int64_t i = row * a.ldb + min(e * nt + tid, a.nbias - 1);
+      bc[e] = a.bias_ids[i];
+      bv[e] = a.bias[i];
+    }
+  }
   const int len = !a.tokens ? 0 : a.lengths ? min(a.lengths[row], a.max_tokens) : a.max_tokens, prompt = a.prompts ? a.prompts[row] : 0;
   const int32_t* tok = a.tokens + row * a.ldt;
   int t[RU];
   auto load_tokens = [&](int i0) {
 #pragma unroll
-    for (int u = 0; u < RU; ++u) { const int i = i0 + u * nt + tid; t[u] = i < len ? tok[i] : -1; }
+    for (int u = 0; u < RU; ++u) t[u] = tok[min(i0 + u * nt + tid, len - 1)];
   };
+  if (len > 0) load_tokens(0);
   float v[RU][W];
+  uint32_t m[RU];
   auto load = [&](int j0) {
 #pragma unroll
     for (int u = 0; u < RU; ++u) {
-      const int c = W * (j0 + u * nt + tid);
-      if constexpr (VEC) {
-        if (c + 4 <= n) { const float4 f = *(const float4*)(x + c); v[u][0] = f.x; v[u][1] = f.y; v[u][2] = f.z; v[u][3] = f.w; }
-        else
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[u][i] = c + i < n ? x[c + i] : 0.f;
-      } else v[u][0] = c < n ? x[c] : 0.f;
+      const int c = min(W * (j0 + u * nt + tid), n - W);
+      if constexpr (VEC) { const float4 f = *(const float4*)(x + c); v[u][0] = f.x; v[u][1] = f.y; v[u][2] = f.z; v[u][3] = f.w; }
+      else v[u][0] = x[c];
     }
+    if (allowed)
+#pragma unroll
+      for (int u = 0; u < RU; ++u) {
+        const int c = min(W * (j0 + u * nt + tid), n - W);
+        m[u] = allowed[c >> 5] >> (c & 31);  // (4 columns lie in one word)
+      }
   };
-  load_tokens(0);
-  const int nb4 = (a.nbias + 3) / 4 * 4;
-  for (int i = tid; i < nb4; i += nt) {
-    const int64_t c = i < a.nbias ? a.bias_ids[row * a.ldb + i] - c0 : -1;
-    at[i] = c < 0 || c >= n ? -1 : (int)c;
-    add[i] = i < a.nbias ? a.bias[row * a.ldb + i] : 0.f;
-  }
   const float rep = a.repetition ? a.repetition[row] : 1.f, pre = a.presence ? a.presence[row] : 0.f, fre = a.frequency ? a.frequency[row] : 0.f;
   load(0);
-  if (a.tokens)
+  if (a.tokens || a.nbias)
     for (int i = tid; i < words / 4; i += nt) ((uint4*)cells)[i] = make_uint4(0, 0, 0, 0);
+  if (a.nbias)
+    for (int i = tid; i < RHASH; i += nt) head[i] = -1;
   __syncthreads();
   for (int i0 = 0; i0 < len; i0 += RU * nt) {
     if (i0) load_tokens(i0);
 #pragma unroll
     for (int u = 0; u < RU; ++u) {
       const int64_t c = t[u] - c0;
-      if (c < 0 || c >= n) continue;
+      if (c < 0 || c >= n || i0 + u * nt + tid >= len) continue;
       const int sh = CB == 16 ? 16 * (int)(c & 1) : 0;
       uint32_t* cell = cells + (CB == 16 ? c >> 1 : c);
-      if (i0 + u * nt + tid < prompt) atomicOr(cell, 1u << (sh + CB - 1));
+      if (i0 + u * nt + tid < prompt) atomicOr(cell, RuleCell<CB>::PROMPT << sh);
       else atomicAdd(cell, 1u << sh);
     }
   }
-  // this thread's columns with a bias: the logit (read before any is written), the biases' sum
-  constexpr int RB = RBIAS / 256;
-  int bc[RB];
-  float bx[RB], bs[RB];
+  if (a.nbias) {
 #pragma unroll
-  for (int e = 0; e < RB; ++e) {
-    const int i = e * nt + tid;
-    bc[e] = -1;
-    if (i >= a.nbias) continue;
-    const int c = at[i];
-    if (c < 0 || (allowed && !(allowed[c >> 5] >> (c & 31) & 1u))) continue;
-    bx[e] = x[c];
-    bool first = true;
-    float sum = 0.f;
-#pragma unroll 4
-    for (int j = 0; j < nb4; j += 4) {
-      const int4 k = *(const int4*)(at + j);
-      if (k.x != c && k.y != c && k.z != c && k.w != c) continue;
-      if (k.x == c) { first = first && j >= i; sum += add[j]; }
-      if (k.y == c) { first = first && j + 1 >= i; sum += add[j + 1]; }
-      if (k.z == c) { first = first && j + 2 >= i; sum += add[j + 2]; }
-      if (k.w == c) { first = first && j + 3 >= i; sum += add[j + 3]; }
+    for (int e = 0; e < RB; ++e) {
+      const int i = e * nt + tid;
+      if (i >= nb4) continue;
+      const int64_t at_c = bc[e] - c0;
+      const int c = at_c < 0 || at_c >= n || i >= a.nbias ? -1 : (int)at_c;
+      at[i] = c;
+      add[i] = bv[e];
+      if (c < 0) continue;
+      atomicOr(cells + (CB == 16 ? c >> 1 : c), RuleCell<CB>::BIAS << (CB == 16 ? 16 * (c & 1) : 0));
+      next[i] = atomicExch(head + c % RHASH, i);
     }
-    if (first) { bc[e] = c; bs[e] = sum; }
   }
   __syncthreads();
   for (int j0 = 0; W * j0 < n; j0 += RU * nt) {
@@ -129,7 +136,7 @@ __global__ __launch_bounds__(1024) void rules_kernel(RuleArgs a) {
     for (int u = 0; u < RU; ++u) {
       const int c = W * (j0 + u * nt + tid);
       if (c >= n) continue;
-      if (a.tokens) {
+      if (a.tokens || a.nbias) {
         uint32_t cell[W];
         if constexpr (CB == 16 && VEC) {
           const uint2 w = *(const uint2*)(cells + (c >> 1));
@@ -138,30 +145,48 @@ __global__ __launch_bounds__(1024) void rules_kernel(RuleArgs a) {
 #pragma unroll
           for (int i = 0; i < W; ++i) cell[i] = CB == 16 ? ((const uint16_t*)cells)[c + i] : cells[c + i];
         }
+        uint32_t marks = 0;
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[u][i] = ruled<CB>(v[u][i], cell[i], rep, pre, fre);
+        for (int i = 0; i < W; ++i) {
+          v[u][i] = ruled<CB>(v[u][i], cell[i], rep, pre, fre);
+          if (cell[i] & RuleCell<CB>::BIAS) marks |= 1u << i;
+        }
+        while (marks) {
+          const int i = __builtin_ctz(marks), col = c + i;
+          marks &= marks - 1;
+          int found = 0;
+          float sum = 0.f;
+          for (int j = head[col % RHASH]; j >= 0; j = next[j])
+            if (at[j] == col) { ++found; sum += add[j]; }
+          if (found > 2) {  // (two have one sum in either order)
+            sum = 0.f;
+#pragma unroll 4
+            for (int j = 0; j < nb4; j += 4) {
+              const int4 k = *(const int4*)(at + j);
+              if (k.x == col) sum += add[j];
+              if (k.y == col) sum += add[j + 1];
+              if (k.z == col) sum += add[j + 2];
+              if (k.w == col) sum += add[j + 3];
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < W; ++k) v[u][k] = k == i ? v[u][k] + sum : v[u][k];
+        }
       }
       if (allowed) {
-        const uint32_t m = allowed[c >> 5] >> (c & 31);  // (4 columns lie in one word)
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[u][i] = m >> i & 1u ? v[u][i] : -INFINITY;
+        for (int i = 0; i < W; ++i) v[u][i] = m[u] >> i & 1u ? v[u][i] : -INFINITY;
       }
-      if constexpr (VEC) {
-        if (c + 4 <= n) { *(float4*)(out + c) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]); continue; }
-      }
+    }
+    // (the writes apart: a marked column's chain of LDS reads would wait for those before it)
 #pragma unroll
-      for (int i = 0; i < W; ++i)
-        if (c + i < n) out[c + i] = v[u][i];
+    for (int u = 0; u < RU; ++u) {
+      const int c = W * (j0 + u * nt + tid);
+      if (c >= n) continue;
+      if constexpr (VEC) *(float4*)(out + c) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+      else out[c] = v[u][0];
     }
   }
-  if (!a.nbias) return;
-  __syncthreads();  // (the part is written)
-#pragma unroll
-  for (int e = 0; e < RB; ++e)
-    if (bc[e] >= 0) {
-      const uint32_t cell = !a.tokens ? 0u : CB == 16 ? ((const uint16_t*)cells)[bc[e]] : cells[bc[e]];
-      out[bc[e]] = ruled<CB>(bx[e], cell, rep, pre, fre) + bs[e];
-    }
 }
 
 template <int CB, bool VEC>
@@ -195,13 +220,14 @@ extern "C" int fh_logit_rules(const float* logits, int64_t ldl, int64_t rows, in
   a.lengths = lengths; a.prompts = prompt_lengths; a.repetition = repetition; a.presence = presence; a.frequency = frequency;
   a.bias_ids = bias_ids; a.bias = bias; a.ldb = ldb; a.nbias = bias_ids ? (int)biases : 0;
   a.allowed = (const uint32_t*)allowed; a.ldm = ldm; a.out = out; a.ldo = ldo;
-  // parts: two workgroups a CU of 256, at least 1024 columns, at most 64 KB of cells; 8 columns a thread up to 1024 threads
-  const bool wide = a.tokens && max_tokens >= 32768;
+  // parts: two workgroups a CU of 256, at least 1024 columns, at most 64 KB of cells. Threads by the part: 64 columns each, 256 to
+  // 512 (128 rows of 128256 with tokens, 300 biases and a mask: 41 us; 256 threads 47, 1024 46, parts of 16384 42 to 50)
+  const bool wide = a.tokens && max_tokens >= 16384;
   const int64_t most = wide ? 16384 : 32768, even = (vocab * rows / 512 + 1023) / 1024 * 1024;
   a.part = (int)std::min(most, std::max<int64_t>(1024, even));
-  const int threads = std::min(1024, std::max(256, a.part / 8));
-  const size_t lds = (size_t)a.part * (wide ? 4 : 2) + (size_t)(a.nbias + 3) / 4 * 32;
-  const bool vec = ldl % 4 == 0 && ldo % 4 == 0 && !((uintptr_t)logits & 15) && !((uintptr_t)out & 15);
+  const int threads = std::min(512, std::max(256, a.part / 64));
+  const size_t lds = (a.tokens || a.nbias ? (size_t)a.part * (wide ? 4 : 2) : 0) + (a.nbias ? (size_t)(a.nbias + 3) / 4 * 48 + RHASH * 4 : 0);
+  const bool vec = vocab % 4 == 0 && ldl % 4 == 0 && ldo % 4 == 0 && !((uintptr_t)logits & 15) && !((uintptr_t)out & 15);
   const dim3 g((unsigned)((vocab + a.part - 1) / a.part), (unsigned)rows);
   if (wide) {
     if (vec) launch_rules<32, true>(g, threads, lds, as_stream(stream), a);
