@@ -11,9 +11,10 @@
 // V^T P^T. The running max of a softmax moves only when a tile's lies more than 2^8 above it: exponents up to 256 lose
 // nothing in fp32 sums or bf16 products, and the output is rescaled a few times a row rather than every tile.
 //
-// Two forms. bf16 (a bf16 or block-float cache, bf16 output): v_mfma_f32_32x32x16_bf16, an fp32 q as two bf16 terms (off by
+// Two forms. A bf16 or block-float cache (whose values are bf16) and bf16 output: v_mfma_f32_32x32x16_bf16, an fp32 q as two bf16 terms (off by
 // 2^-16 of itself at most; a bf16 q is exact in one), the softmax's weights rounded to bf16 (2^-8 at most, what the output's
-// own rounding adds; their sum is taken before it). fp32 (an fp32 cache or output): v_mfma_f32_32x32x2_f32, nothing rounded.
+// own rounding adds; their sum is taken before it). With fp32 output q and the weights go in as three terms, off by 2^-24 at
+// most. An fp32 cache takes v_mfma_f32_32x32x2_f32, nothing rounded.
 //
 // Where tiles are few, the keys are split among workgroups, each leaving its weighted sum, max and sum of weights in the
 // workspace, and a second kernel joins them; a shared prefix is always one of two parts or more, the rows' own keys others.
@@ -22,6 +23,7 @@
 // finite takes its pairs again one at a time over the keys each sees alone (attend_again).
 #include <math.h>
 #include <algorithm>
+#include <type_traits>
 #include "fh_common.h"
 
 namespace fh {
@@ -344,13 +346,18 @@ __device__ inline void seq_softmax(floatx16 (&s)[NB], int k0, int limit, int wav
   l += sum;  // (this half's keys; the halves meet at the end)
 }
 
-// what both forms do around their tiles: the item, the pair of each lane, the tiles of its keys
-#define SEQ_BEGIN(BK) \
+// what both forms do around their tiles: the item, the pair of each lane, the tiles of its keys. A tile of at most 64 pairs
+// leaves waves over: of KG = 2 groups of waves each takes half of a tile's keys (blocks of 32), and the groups' results meet
+// at the end (seq_meet). KGMAX: how many groups the form knows.
+#define SEQ_BEGIN(BK, KGMAX) \
   SeqItem it; \
   if (!seq_item(a, it)) return; \
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ql = lane & 31, hh = lane >> 5; \
   if (it.pair0 >= it.pairs) return; \
-  const int wpair = it.pair0 + 32 * wave, pair = min(wpair + ql, it.pairs - 1); \
+  const int groups = KGMAX > 1 && it.pairs - it.pair0 <= SQ_BQ / 2 ? 2 : 1;  /* of keys */ \
+  const int pgroups = groups == 1 ? SQ_NW : it.pairs - it.pair0 <= 32 ? 1 : 2;  /* of pairs */ \
+  const int kg = groups == 1 ? 0 : wave / pgroups;   /* (2 and 3: a wave that only loads) */ \
+  const int wpair = it.pair0 + 32 * (groups == 1 ? wave : wave % pgroups), pair = min(wpair + ql, it.pairs - 1); \
   const int limit = wpair + ql < it.pairs ? pair_limit(a, it, pair) : 0; \
   int wave_max = limit, wave_min = wpair + ql < it.pairs ? limit : 0x7FFFFFFF; \
   for (int d = 1; d < 32; d <<= 1) { wave_max = max(wave_max, __shfl_xor(wave_max, d, 64)); wave_min = min(wave_min, __shfl_xor(wave_min, d, 64)); } \
@@ -360,6 +367,7 @@ __device__ inline void seq_softmax(floatx16 (&s)[NB], int k0, int limit, int wav
   __syncthreads(); \
   int keys = tops[0]; \
   for (int w = 1; w < SQ_NW; ++w) keys = max(keys, tops[w]); \
+  if (kg >= groups) wave_max = 0; \
   const int ntiles = (keys + BK - 1) / BK; \
   const int t0 = (int)((int64_t)ntiles * it.split / it.splits), t1 = (int)((int64_t)ntiles * (it.split + 1) / it.splits); \
   const int64_t qat = (it.row0 + pair / a.rep) * a.ldq + (int64_t)(it.kvh * a.rep + pair % a.rep) * HD; \
@@ -369,12 +377,52 @@ __device__ inline void seq_softmax(floatx16 (&s)[NB], int k0, int limit, int wav
   for (int d = 0; d < HD / 32; ++d) for (int r = 0; r < 16; ++r) acc[d][r] = 0.f; \
   float m = -INFINITY, l = 0.f;
 
-template <int HD, int CF, int QT>
+// The second key group's results into the first's, pair group by pair group, through LDS where the tiles were. False: the
+// wave has given its results away. (All waves of the workgroup call it: behind the last tile's barrier.)
+template <int HD>
+__device__ inline bool seq_meet(float* lds, int groups, int pgroups, int kg, int wave, float& m, float& l, floatx16 (&acc)[HD / 32]) {
+  if (groups == 1) return true;
+  const int lane = threadIdx.x & 63;
+  float* slot = lds + (wave % pgroups) * (HD / 2 + 2) * 64 + lane;
+  if (kg == 1) {
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) slot[(16 * d + r) * 64] = acc[d][r];
+    slot[(HD / 2) * 64] = m;
+    slot[(HD / 2 + 1) * 64] = l;
+  }
+  __syncthreads();
+  if (kg != 0) return false;
+  const float om = slot[(HD / 2) * 64], ol = slot[(HD / 2 + 1) * 64], top = fmaxf(m, om);
+  // (a max of -inf, no key seen: no weight; both: 0)
+  const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), g = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - top);
+  m = top;
+  l = l * f + ol * g;
+#pragma unroll
+  for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[d][r] = acc[d][r] * f + slot[(16 * d + r) * 64] * g;
+  return true;
+}
+
+// x's bf16 terms: the value to nearest, then what is left to nearest
+template <int N>
+__device__ inline void bf16_terms(const float (&x)[8], bf16x8 (&t)[N]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float left = x[i];
+#pragma unroll
+    for (int j = 0; j < N; ++j) { t[j][i] = (__bf16)left; left -= (float)t[j][i]; }
+  }
+}
+
+// QT, PT: the bf16 terms of q and of the weights
+template <int HD, int CF, int QT, int PT>
 __global__ __launch_bounds__(64 * SQ_NW, 2) void seq_bf16_kernel(SeqArgs a) {
   constexpr int BK = 64, KLD = HD + 8, VLD = HD + 32;  // (a row's 16-byte reads, and 4 rows' transposed reads, on distinct banks)
-  __shared__ __attribute__((aligned(16))) uint16_t Ks[2][BK * KLD];
-  __shared__ __attribute__((aligned(16))) uint16_t Vs[2][BK * VLD];
-  SEQ_BEGIN(BK)
+  __shared__ __attribute__((aligned(16))) uint16_t tiles[2 * BK * (KLD + VLD)];
+  SEQ_BEGIN(BK, 2)
 
   // the lane's q as the product's B: step s holds dimensions 16 s + 8 hh .. + 7, each term
   bf16x8 qf[HD / 16][QT];
@@ -382,12 +430,7 @@ __global__ __launch_bounds__(64 * SQ_NW, 2) void seq_bf16_kernel(SeqArgs a) {
   for (int s = 0; s < HD / 16; ++s) {
     float f[8];
     q8(a, qat + 16 * s + 8 * hh, f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const __bf16 t = (__bf16)f[i];
-      qf[s][0][i] = t;
-      if (QT > 1) qf[s][QT - 1][i] = (__bf16)(f[i] - (float)t);
-    }
+    bf16_terms<QT>(f, qf[s]);
   }
 
   constexpr int NP = BK * HD / 8 / (64 * SQ_NW);  // pieces of 8 a thread
@@ -402,57 +445,71 @@ __global__ __launch_bounds__(64 * SQ_NW, 2) void seq_bf16_kernel(SeqArgs a) {
     }
   };
   auto store = [&](int b) {
+    uint16_t* K = tiles + b * BK * (KLD + VLD);
+    uint16_t* V = K + BK * KLD;
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
       const int i = tid + 64 * SQ_NW * j, r = i / (HD / 8), c = (i % (HD / 8)) * 8;
-      *(uint4*)(Ks[b] + r * KLD + c) = seq_bf16x8<CF>(kraw[j]);
-      *(uint4*)(Vs[b] + r * VLD + c) = seq_bf16x8<CF>(vraw[j]);
+      *(uint4*)(K + r * KLD + c) = seq_bf16x8<CF>(kraw[j]);
+      *(uint4*)(V + r * VLD + c) = seq_bf16x8<CF>(vraw[j]);
     }
+  };
+  // blocks kb0 .. kb0 + NB - 1 of 32 keys of the tile in buffer b, whose first key is k0
+  auto work = [&](auto nb, int kb0, int b, int k0) {
+    constexpr int NB = decltype(nb)::value;
+    const uint16_t* K = tiles + b * BK * (KLD + VLD) + 32 * kb0 * KLD;
+    const uint16_t* V = tiles + b * BK * (KLD + VLD) + BK * KLD + 32 * kb0 * VLD;
+    floatx16 s[NB];
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+#pragma unroll
+    for (int st = 0; st < HD / 16; ++st)
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) {
+        const bf16x8 kf = *(const bf16x8*)(K + (32 * kb + ql) * KLD + 16 * st + 8 * hh);
+#pragma unroll
+        for (int u = 0; u < QT; ++u) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st][u], s[kb], 0, 0, 0);
+      }
+    seq_softmax<HD, NB>(s, k0 + 32 * kb0, limit, wave_min, hh, scale2, m, l, acc);
+    // O^T += V^T P^T, 16 keys a step: the lane's weights 8 j .. 8 j + 7 of block kb are keys 32 kb + 16 j + {4 hh .. 4 hh + 3,
+    // 8 + 4 hh .. 8 + 4 hh + 3}; V's columns come transposed, 4 keys of 16 dimensions to 16 lanes
+    SEQ_LDS short4v* vt = (SEQ_LDS short4v*)(V + (4 * hh + ((lane & 15) >> 2)) * VLD + (lane & 16) + 4 * (lane & 3));
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float p8[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p8[i] = s[kb][8 * j + i];
+        bf16x8 pf[PT];
+        bf16_terms<PT>(p8, pf);
+        const int g = 32 * kb + 16 * j;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) {
+          const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(vt + (g * VLD + 32 * d) / 4);
+          const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(vt + ((g + 8) * VLD + 32 * d) / 4);
+          const short v8[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+          for (int u = 0; u < PT; ++u) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)v8, pf[u], acc[d], 0, 0, 0);
+        }
+      }
   };
   if (t0 < t1) { load(t0); store(0); }
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const int b = (t - t0) & 1, k0 = t * BK;
     if (t + 1 < t1) load(t + 1);
-    if (k0 < wave_max) {
-      floatx16 s[2];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
-#pragma unroll
-      for (int st = 0; st < HD / 16; ++st)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const bf16x8 kf = *(const bf16x8*)(Ks[b] + (32 * kb + ql) * KLD + 16 * st + 8 * hh);
-#pragma unroll
-          for (int u = 0; u < QT; ++u) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st][u], s[kb], 0, 0, 0);
-        }
-      seq_softmax<HD, 2>(s, k0, limit, wave_min, hh, scale2, m, l, acc);
-      // O^T += V^T P^T, 16 keys a step: the lane's weights 8 j .. 8 j + 7 of block kb are keys 32 kb + 16 j + {4 hh .. 4 hh + 3,
-      // 8 + 4 hh .. 8 + 4 hh + 3}; V's columns come transposed, 4 keys of 16 dimensions to 16 lanes
-      SEQ_LDS short4v* vt = (SEQ_LDS short4v*)(Vs[b] + (4 * hh + ((lane & 15) >> 2)) * VLD + (lane & 16) + 4 * (lane & 3));
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          bf16x8 pf;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pf[i] = (__bf16)s[kb][8 * j + i];
-          const int g = 32 * kb + 16 * j;
-#pragma unroll
-          for (int d = 0; d < HD / 32; ++d) {
-            const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(vt + (g * VLD + 32 * d) / 4);
-            const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(vt + ((g + 8) * VLD + 32 * d) / 4);
-            const short v8[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)v8, pf, acc[d], 0, 0, 0);
-          }
-        }
-    }
+    if (groups == 1) {
+      if (k0 < wave_max) work(std::integral_constant<int, 2>(), 0, b, k0);
+    } else if (k0 + 32 * kg < wave_max) work(std::integral_constant<int, 1>(), kg, b, k0);
     if (t + 1 < t1) store(1 - b);  // (the other buffer: its last readers passed the previous barrier)
     __syncthreads();
   }
   l += __shfl_xor(l, 32, 64);
+  static_assert(2 * 64 * (HD / 2 + 2) * 4 <= (int)sizeof(tiles), "the key groups' place");
+  if (!seq_meet<HD>((float*)tiles, groups, pgroups, kg, wave, m, l, acc)) return;
   seq_finish<HD, CF>(a, it, wpair, limit, t0 * BK, min(t1 * BK, keys), acc, m, l);
 }
 
@@ -463,7 +520,7 @@ __global__ __launch_bounds__(64 * SQ_NW, 2) void seq_f32_kernel(SeqArgs a) {
   constexpr int BK = 32, LD = HD + 4;
   __shared__ __attribute__((aligned(16))) float Ks[2][BK * LD];
   __shared__ __attribute__((aligned(16))) float Vs[2][BK * LD];
-  SEQ_BEGIN(BK)
+  SEQ_BEGIN(BK, 1)
   float qf[HD / 2];
 #pragma unroll
   for (int s = 0; s < HD / 16; ++s) {
@@ -575,13 +632,15 @@ __global__ __launch_bounds__(256) void seq_join(SeqArgs a) {
 template <int HD, int CF>
 static void launch_seq(unsigned blocks, hipStream_t s, const SeqArgs& a) {
   const dim3 g(blocks), b(64 * SQ_NW);
-  if constexpr (CF != FH_F32)
+  if constexpr (CF != FH_F32) {
     if (a.o_bf16) {
-      if (a.q_bf16) hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 1>), g, b, 0, s, a);
-      else hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 2>), g, b, 0, s, a);
-      return;
+      if (a.q_bf16) hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 1, 1>), g, b, 0, s, a);
+      else hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 2, 1>), g, b, 0, s, a);
+    } else {
+      if (a.q_bf16) hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 1, 3>), g, b, 0, s, a);
+      else hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 3, 3>), g, b, 0, s, a);
     }
-  hipLaunchKernelGGL((seq_f32_kernel<HD, CF>), g, b, 0, s, a);
+  } else hipLaunchKernelGGL((seq_f32_kernel<HD, CF>), g, b, 0, s, a);
 }
 
 template <int HD>
