@@ -32,6 +32,8 @@ typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float floatx16;
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short short4v;
 #define SEQ_LDS __attribute__((address_space(3)))
+typedef const __attribute__((address_space(1))) uint32_t* seq_global;
+typedef SEQ_LDS uint32_t* seq_lds;
 
 constexpr int SQ_NW = 4;               // waves a workgroup
 constexpr int SQ_BQ = 32 * SQ_NW;      // pairs a workgroup
@@ -417,11 +419,26 @@ __device__ inline void bf16_terms(const float (&x)[8], bf16x8 (&t)[N]) {
   }
 }
 
+// Where a tile's values lie in LDS. A bf16 cache's rows go there straight from memory (global_load_lds_dwordx4: no registers, no
+// writes of ours): rows unpadded, 1 KB a wave's instruction in lane order, the banks spread by which 16 bytes of its row each
+// lane fetches: unit u of a row at unit u ^ f(row). A block float's runs are decoded on the way and written to padded rows.
+template <int HD, bool ASYNC>
+struct SeqTile {
+  static constexpr int KLD = ASYNC ? HD : HD + 8, VLD = ASYNC ? HD : HD + 32;  // (a row's 16-byte reads, and 4 rows' transposed ones, on distinct banks)
+  static constexpr int SIZE = 64 * (KLD + VLD);                                // uint16s: 64 keys' rows, then their values'
+  // tiles in LDS: a third saves one of two barriers a tile, where it fits two workgroups a CU
+  static constexpr int STAGES = ASYNC && HD == 64 ? 3 : 2;
+  __device__ static int kswap(int row) { return !ASYNC ? 0 : HD == 128 ? row & 15 : (row >> 1) & 7; }
+  __device__ static int vswap(int row) { return !ASYNC ? 0 : HD == 128 ? (row & 3) * 4 : ((row >> 1) & 1) * 4; }
+};
+
 // QT, PT: the bf16 terms of q and of the weights
 template <int HD, int CF, int QT, int PT>
-__global__ __launch_bounds__(64 * SQ_NW, 2) void seq_bf16_kernel(SeqArgs a) {
-  constexpr int BK = 64, KLD = HD + 8, VLD = HD + 32;  // (a row's 16-byte reads, and 4 rows' transposed reads, on distinct banks)
-  __shared__ __attribute__((aligned(16))) uint16_t tiles[2 * BK * (KLD + VLD)];
+__global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf16_kernel(SeqArgs a) {
+  constexpr bool ASYNC = CF == FH_BF16;
+  using Tile = SeqTile<HD, ASYNC>;
+  constexpr int BK = 64, KLD = Tile::KLD, VLD = Tile::VLD, NS = Tile::STAGES;
+  __shared__ __attribute__((aligned(256))) uint16_t tiles[NS * Tile::SIZE];
   SEQ_BEGIN(BK, 2)
 
   // the lane's q as the product's B: step s holds dimensions 16 s + 8 hh .. + 7, each term
@@ -434,31 +451,39 @@ __global__ __launch_bounds__(64 * SQ_NW, 2) void seq_bf16_kernel(SeqArgs a) {
   }
 
   constexpr int NP = BK * HD / 8 / (64 * SQ_NW);  // pieces of 8 a thread
-  SeqRaw kraw[NP], vraw[NP];
-  auto load = [&](int t) {
+  SeqRaw kraw[ASYNC ? 1 : NP], vraw[ASYNC ? 1 : NP];
+  auto load = [&](int t, int b) {  // tile t's loads: into buffer b, or into registers
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      const int i = tid + 64 * SQ_NW * j, r = i / (HD / 8), c = (i % (HD / 8)) * 8;
+      const int i = ASYNC ? 64 * (NP * wave + j) + lane : tid + 64 * SQ_NW * j, r = i / (HD / 8), u = i % (HD / 8);
       const int64_t row = key_row(a, it, min(t * BK + r, keys - 1));
-      kraw[j] = seq_raw<HD, CF>(a, kplane + row, c);
-      vraw[j] = seq_raw<HD, CF>(a, vplane + row, c);
+      if constexpr (ASYNC) {
+        uint16_t* to = tiles + b * Tile::SIZE + 512 * (NP * wave + j);
+        __builtin_amdgcn_global_load_lds((seq_global)((const uint16_t*)a.cache + (kplane + row) * HD + 8 * (u ^ Tile::kswap(r))), (seq_lds)to, 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((seq_global)((const uint16_t*)a.cache + (vplane + row) * HD + 8 * (u ^ Tile::vswap(r))), (seq_lds)(to + BK * HD), 16, 0, 0);
+      } else {
+        kraw[j] = seq_raw<HD, CF>(a, kplane + row, 8 * u);
+        vraw[j] = seq_raw<HD, CF>(a, vplane + row, 8 * u);
+      }
     }
   };
   auto store = [&](int b) {
-    uint16_t* K = tiles + b * BK * (KLD + VLD);
-    uint16_t* V = K + BK * KLD;
+    if constexpr (!ASYNC) {
+      uint16_t* K = tiles + b * Tile::SIZE;
+      uint16_t* V = K + BK * KLD;
 #pragma unroll
-    for (int j = 0; j < NP; ++j) {
-      const int i = tid + 64 * SQ_NW * j, r = i / (HD / 8), c = (i % (HD / 8)) * 8;
-      *(uint4*)(K + r * KLD + c) = seq_bf16x8<CF>(kraw[j]);
-      *(uint4*)(V + r * VLD + c) = seq_bf16x8<CF>(vraw[j]);
+      for (int j = 0; j < NP; ++j) {
+        const int i = tid + 64 * SQ_NW * j, r = i / (HD / 8), c = (i % (HD / 8)) * 8;
+        *(uint4*)(K + r * KLD + c) = seq_bf16x8<CF>(kraw[j]);
+        *(uint4*)(V + r * VLD + c) = seq_bf16x8<CF>(vraw[j]);
+      }
     }
   };
   // blocks kb0 .. kb0 + NB - 1 of 32 keys of the tile in buffer b, whose first key is k0
   auto work = [&](auto nb, int kb0, int b, int k0) {
     constexpr int NB = decltype(nb)::value;
-    const uint16_t* K = tiles + b * BK * (KLD + VLD) + 32 * kb0 * KLD;
-    const uint16_t* V = tiles + b * BK * (KLD + VLD) + BK * KLD + 32 * kb0 * VLD;
+    const uint16_t* K = tiles + b * Tile::SIZE + 32 * kb0 * KLD;
+    const uint16_t* V = tiles + b * Tile::SIZE + BK * KLD + 32 * kb0 * VLD;
     floatx16 s[NB];
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
@@ -468,14 +493,15 @@ __global__ __launch_bounds__(64 * SQ_NW, 2) void seq_bf16_kernel(SeqArgs a) {
     for (int st = 0; st < HD / 16; ++st)
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb) {
-        const bf16x8 kf = *(const bf16x8*)(K + (32 * kb + ql) * KLD + 16 * st + 8 * hh);
+        const bf16x8 kf = *(const bf16x8*)(K + (32 * kb + ql) * KLD + 8 * ((2 * st + hh) ^ Tile::kswap(ql)));
 #pragma unroll
         for (int u = 0; u < QT; ++u) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st][u], s[kb], 0, 0, 0);
       }
     seq_softmax<HD, NB>(s, k0 + 32 * kb0, limit, wave_min, hh, scale2, m, l, acc);
     // O^T += V^T P^T, 16 keys a step: the lane's weights 8 j .. 8 j + 7 of block kb are keys 32 kb + 16 j + {4 hh .. 4 hh + 3,
     // 8 + 4 hh .. 8 + 4 hh + 3}; V's columns come transposed, 4 keys of 16 dimensions to 16 lanes
-    SEQ_LDS short4v* vt = (SEQ_LDS short4v*)(V + (4 * hh + ((lane & 15) >> 2)) * VLD + (lane & 16) + 4 * (lane & 3));
+    const int vr = (lane & 15) >> 2, vu = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);  // the lane's row of 4, its 16 bytes of 64
+    const uint16_t* vl = V + (4 * hh + vr) * VLD + 4 * (lane & 1);
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
@@ -488,24 +514,54 @@ __global__ __launch_bounds__(64 * SQ_NW, 2) void seq_bf16_kernel(SeqArgs a) {
         const int g = 32 * kb + 16 * j;
 #pragma unroll
         for (int d = 0; d < HD / 32; ++d) {
-          const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(vt + (g * VLD + 32 * d) / 4);
-          const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(vt + ((g + 8) * VLD + 32 * d) / 4);
+          const uint16_t* vd = vl + g * VLD + 8 * ((4 * d + vu) ^ Tile::vswap(vr));
+          const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SEQ_LDS short4v*)vd);
+          const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SEQ_LDS short4v*)(vd + 8 * VLD));
           const short v8[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
           for (int u = 0; u < PT; ++u) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)v8, pf[u], acc[d], 0, 0, 0);
         }
       }
   };
-  if (t0 < t1) { load(t0); store(0); }
-  __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    const int b = (t - t0) & 1, k0 = t * BK;
-    if (t + 1 < t1) load(t + 1);
+  auto work_on = [&](int t, int b) {
     if (groups == 1) {
-      if (k0 < wave_max) work(std::integral_constant<int, 2>(), 0, b, k0);
-    } else if (k0 + 32 * kg < wave_max) work(std::integral_constant<int, 1>(), kg, b, k0);
-    if (t + 1 < t1) store(1 - b);  // (the other buffer: its last readers passed the previous barrier)
+      if (t * BK < wave_max) work(std::integral_constant<int, 2>(), 0, b, t * BK);
+    } else if (t * BK + 32 * kg < wave_max) work(std::integral_constant<int, 1>(), kg, b, t * BK);
+  };
+  if constexpr (ASYNC) {
+    // a ring of NS tiles: a tile's wait leaves the next one's loads in flight
+    constexpr int W = 2 * NP;
+    if (t0 < t1) load(t0, 0);
+    if (t0 + 1 < t1) load(t0 + 1, 1);
+    int b = 0;
+    for (int t = t0; t < t1; ++t) {
+      asm volatile("" ::: "memory");
+      if (t + 1 < t1) __builtin_amdgcn_s_waitcnt(0x0070 | (W & 15) | (W >> 4) << 14);
+      else __builtin_amdgcn_s_waitcnt(0x0070);
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (NS == 3 && t + 2 < t1) load(t + 2, b == 0 ? 2 : b - 1);  // (its last readers passed this barrier)
+      work_on(t, b);
+      if (NS == 2 && t + 2 < t1) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // (this wave's reads of the buffer are done)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        load(t + 2, b);
+      }
+      b = b + 1 == NS ? 0 : b + 1;
+    }
     __syncthreads();
+  } else {
+    if (t0 < t1) { load(t0, 0); store(0); }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+      const int b = (t - t0) & 1;
+      if (t + 1 < t1) load(t + 1, 0);
+      work_on(t, b);
+      if (t + 1 < t1) store(1 - b);  // (the other buffer: its last readers passed the previous barrier)
+      __syncthreads();
+    }
   }
   l += __shfl_xor(l, 32, 64);
   static_assert(2 * 64 * (HD / 2 + 2) * 4 <= (int)sizeof(tiles), "the key groups' place");
