@@ -31,9 +31,18 @@ namespace fh {
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float floatx16;
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short short4v;
+typedef __attribute__((__vector_size__(8 * sizeof(short)))) short short8v;
 #define SEQ_LDS __attribute__((address_space(3)))
-typedef const __attribute__((address_space(1))) uint32_t* seq_global;
-typedef SEQ_LDS uint32_t* seq_lds;
+// 16 bytes a lane from memory to LDS, the wave's 1 KB from `to` on in lane order. Written as an instruction so that the compiler
+// does not hold every transposed read of LDS for all the loads in flight, as it does behind the builtin (the ring's waits are
+// the kernel's own; a count that leaves these loads out only waits longer).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0 is nobody's here)
+__device__ __forceinline__ void load_to_lds(const void* from, uint16_t* to) {
+  const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uintptr_t)(SEQ_LDS uint16_t*)to);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(at) : "memory", "m0");
+}
+#pragma clang diagnostic pop
 
 constexpr int SQ_NW = 4;               // waves a workgroup
 constexpr int SQ_BQ = 32 * SQ_NW;      // pairs a workgroup
@@ -452,18 +461,38 @@ __global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf
 
   constexpr int NP = BK * HD / 8 / (64 * SQ_NW);  // pieces of 8 a thread
   SeqRaw kraw[ASYNC ? 1 : NP], vraw[ASYNC ? 1 : NP];
+  // a thread's pieces of a tile: rows pr + PR j, unit pu of each; where they lie from the tile's first row on
+  constexpr int PR = 64 * SQ_NW / (HD / 8);
+  const int pr = ASYNC ? (64 * NP * wave + lane) / (HD / 8) : tid / (HD / 8), pu = lane % (HD / 8);
+  constexpr int PSTEP = ASYNC ? 64 / (HD / 8) : PR;  // (a wave's instructions in order: its rows lie together)
   auto load = [&](int t, int b) {  // tile t's loads: into buffer b, or into registers
+    const int k0 = t * BK;
+    // the tile's rows run on from its first, as they are, unless the keys end or the prefix ends in it, or it leaves the cache
+    const int64_t first = (k0 < it.shared ? it.prefix : it.own) + k0;
+    const bool plain = k0 + BK <= keys && (k0 >= it.shared || k0 + BK <= it.shared) && first >= 0 && first + BK <= a.cache_len;
+    if (ASYNC && plain) {
+      const char* kb = (const char*)a.cache + (kplane + first) * (HD * 2);
+      const char* vb = (const char*)a.cache + (vplane + first) * (HD * 2);
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        const int r = pr + PSTEP * j;
+        uint16_t* to = tiles + b * Tile::SIZE + 512 * (NP * wave + j);
+        load_to_lds(kb + (uint32_t)(r * HD * 2 + 16 * (pu ^ Tile::kswap(r))), to);
+        load_to_lds(vb + (uint32_t)(r * HD * 2 + 16 * (pu ^ Tile::vswap(r))), to + BK * HD);
+      }
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      const int i = ASYNC ? 64 * (NP * wave + j) + lane : tid + 64 * SQ_NW * j, r = i / (HD / 8), u = i % (HD / 8);
-      const int64_t row = key_row(a, it, min(t * BK + r, keys - 1));
+      const int r = pr + PSTEP * j;
+      const int64_t row = plain ? first + r : key_row(a, it, min(k0 + r, keys - 1));
       if constexpr (ASYNC) {
         uint16_t* to = tiles + b * Tile::SIZE + 512 * (NP * wave + j);
-        __builtin_amdgcn_global_load_lds((seq_global)((const uint16_t*)a.cache + (kplane + row) * HD + 8 * (u ^ Tile::kswap(r))), (seq_lds)to, 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((seq_global)((const uint16_t*)a.cache + (vplane + row) * HD + 8 * (u ^ Tile::vswap(r))), (seq_lds)(to + BK * HD), 16, 0, 0);
+        load_to_lds((const uint16_t*)a.cache + (kplane + row) * HD + 8 * (pu ^ Tile::kswap(r)), to);
+        load_to_lds((const uint16_t*)a.cache + (vplane + row) * HD + 8 * (pu ^ Tile::vswap(r)), to + BK * HD);
       } else {
-        kraw[j] = seq_raw<HD, CF>(a, kplane + row, 8 * u);
-        vraw[j] = seq_raw<HD, CF>(a, vplane + row, 8 * u);
+        kraw[j] = seq_raw<HD, CF>(a, kplane + row, 8 * pu);
+        vraw[j] = seq_raw<HD, CF>(a, vplane + row, 8 * pu);
       }
     }
   };
@@ -473,9 +502,9 @@ __global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf
       uint16_t* V = K + BK * KLD;
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
-        const int i = tid + 64 * SQ_NW * j, r = i / (HD / 8), c = (i % (HD / 8)) * 8;
-        *(uint4*)(K + r * KLD + c) = seq_bf16x8<CF>(kraw[j]);
-        *(uint4*)(V + r * VLD + c) = seq_bf16x8<CF>(vraw[j]);
+        const int r = pr + PSTEP * j;
+        *(uint4*)(K + r * KLD + 8 * pu) = seq_bf16x8<CF>(kraw[j]);
+        *(uint4*)(V + r * VLD + 8 * pu) = seq_bf16x8<CF>(vraw[j]);
       }
     }
   };
@@ -517,9 +546,9 @@ __global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf
           const uint16_t* vd = vl + g * VLD + 8 * ((4 * d + vu) ^ Tile::vswap(vr));
           const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SEQ_LDS short4v*)vd);
           const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SEQ_LDS short4v*)(vd + 8 * VLD));
-          const short v8[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          const short8v vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-          for (int u = 0; u < PT; ++u) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)v8, pf[u], acc[d], 0, 0, 0);
+          for (int u = 0; u < PT; ++u) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)&vf, pf[u], acc[d], 0, 0, 0);
         }
       }
   };
