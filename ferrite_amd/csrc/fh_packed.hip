@@ -45,7 +45,6 @@ __device__ __forceinline__ void load_to_lds(const void* from, uint16_t* to) {
 #pragma clang diagnostic pop
 
 constexpr int SQ_NW = 4;               // waves a workgroup
-constexpr int SQ_BQ = 32 * SQ_NW;      // pairs a workgroup
 constexpr float SQ_SLACK = 8.f;        // how far a score may lie above the running max, in base 2
 
 struct SeqArgs {
@@ -83,14 +82,15 @@ __device__ inline void row_counts(const SeqArgs& a, int64_t b, int& shared, int&
 }
 
 // The workgroup's item (false: none). Blocks of one key head lie kv_heads apart: with 8 key heads they share an XCD's L2.
+template <int BQ, bool PACKED>
 __device__ inline bool seq_item(const SeqArgs& a, SeqItem& it) {
   int blk = blockIdx.x;
   it.kvh = blk % a.kv_heads;
   blk /= a.kv_heads;
-  if (!a.starts) {
+  if constexpr (!PACKED) {
     if (blk < a.tiles * a.splits) {  // the prefix: tiles of all rows' pairs
       it.split = blk % a.splits; it.splits = a.splits; it.part = it.split;
-      it.row0 = 0; it.pair0 = (blk / a.splits) * SQ_BQ; it.pairs = (int)a.rows * a.rep;
+      it.row0 = 0; it.pair0 = (blk / a.splits) * BQ; it.pairs = (int)a.rows * a.rep;
       it.prefix = a.prefix_row[0]; it.own = 0; it.shared = 0x7FFFFFFF;
       it.place0 = 0; it.step = -1;
       return true;
@@ -104,40 +104,38 @@ __device__ inline bool seq_item(const SeqArgs& a, SeqItem& it) {
     it.prefix = 0; it.own = a.first_row[b]; it.shared = 0;
     it.place0 = own - 1; it.step = 0;
     return true;
-  }
-  it.split = it.part = blk % a.splits; it.splits = a.splits;
-  const int tile = blk / a.splits, lane = threadIdx.x & 63;
-  int before = 0;
-  for (int s0 = 0; s0 < a.n; s0 += 64) {  // 64 sequences a round: the one whose tiles hold this one
-    const int s = s0 + lane;
-    int lo = 0, len = 0;
-    if (s < a.n) {
-      lo = clampi(a.starts[s], 0, a.rows);
-      len = clampi(a.starts[s + 1], lo, a.rows) - lo;
-    }
-    const int tiles = (int)(((int64_t)len * a.rep + SQ_BQ - 1) / SQ_BQ);
-    int incl = tiles;
+  } else {
+    it.split = it.part = blk % a.splits; it.splits = a.splits;
+    const int tile = blk / a.splits, lane = threadIdx.x & 63;
+    const int prefix = a.shared ? a.prefix_row[0] : 0;
+    int before = 0;
+    for (int s0 = 0; s0 < a.n; s0 += 64) {  // 64 sequences a round: the one whose tiles hold this one
+      const int s = min(s0 + lane, a.n - 1);
+      const int st = a.starts[s], en = a.starts[s + 1], place = a.places[s], first = a.first_row[s], shd = a.shared ? a.shared[s] : 0;
+      const int lo = clampi(st, 0, a.rows), len = s0 + lane < a.n ? clampi(en, lo, a.rows) - lo : 0;
+      const int tiles = (int)(((int64_t)len * a.rep + BQ - 1) / BQ);
+      int incl = tiles;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(incl, d, 64);
-      if (lane >= d) incl += o;
-    }
-    const int total = __shfl(incl, 63, 64);
-    if (tile < before + total) {
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(incl, d, 64);
+        if (lane >= d) incl += o;
+      }
       const uint64_t has = __ballot(tile < before + incl);
-      const int at = __builtin_ctzll(has), sq = s0 + at;
-      const int l0 = __shfl(lo, at, 64), ln = __shfl(len, at, 64), nt = __shfl(tiles, at, 64), in = __shfl(incl, at, 64);
-      const int t = nt - 1 - (tile - (before + in - nt));  // (a sequence's longest tile first)
-      it.row0 = l0; it.pair0 = t * SQ_BQ; it.pairs = ln * a.rep;
-      it.shared = a.shared ? clampi(a.shared[sq], 0, a.max_prefix) : 0;
-      it.prefix = a.shared ? a.prefix_row[0] : 0;
-      it.own = (int64_t)a.first_row[sq] - it.shared;
-      it.place0 = a.places[sq]; it.step = 1;
-      return true;
+      if (has) {
+        const int at = __builtin_ctzll(has);
+        const int nt = __builtin_amdgcn_readlane(tiles, at), in = __builtin_amdgcn_readlane(incl, at);
+        const int t = nt - 1 - (tile - (before + in - nt));  // (a sequence's longest tile first)
+        it.row0 = __builtin_amdgcn_readlane(lo, at); it.pair0 = t * BQ; it.pairs = __builtin_amdgcn_readlane(len, at) * a.rep;
+        it.shared = a.shared ? clampi(__builtin_amdgcn_readlane(shd, at), 0, a.max_prefix) : 0;
+        it.prefix = prefix;
+        it.own = (int64_t)__builtin_amdgcn_readlane(first, at) - it.shared;
+        it.place0 = __builtin_amdgcn_readlane(place, at); it.step = 1;
+        return true;
+      }
+      before += __builtin_amdgcn_readlane(incl, 63);
     }
-    before += total;
+    return false;
   }
-  return false;
 }
 
 // how many keys pair p of the item sees
@@ -147,6 +145,13 @@ __device__ inline int pair_limit(const SeqArgs& a, const SeqItem& it, int p) {
   int sh, pre, own;
   row_counts(a, p / a.rep, sh, pre, own);
   return pre;
+}
+
+// the largest of a value over the wave
+__device__ inline int wave_most(int v) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) v = max(v, __shfl_xor(v, d, 64));
+  return __builtin_amdgcn_readfirstlane(v);
 }
 
 __device__ inline int64_t key_row(const SeqArgs& a, const SeqItem& it, int k) {
@@ -321,7 +326,7 @@ __device__ inline void seq_finish(const SeqArgs& a, const SeqItem& it, int wpair
 // The softmax of a tile's NB blocks of 32 keys from key k0: scores in, weights out; the running max (base 2), the sum and
 // the output's rescaling
 template <int HD, int NB>
-__device__ inline void seq_softmax(floatx16 (&s)[NB], int k0, int limit, int wave_min, int hh, float scale2, float& m, float& l, floatx16 (&acc)[HD / 32]) {
+__device__ inline void seq_softmax(floatx16* s, int k0, int limit, int wave_min, int hh, float scale2, float& m, float& l, floatx16 (&acc)[HD / 32]) {
   if (k0 + 32 * NB > wave_min) {  // (some pair of the wave does not see all of the tile)
     const int left = limit - k0 - 4 * hh;
 #pragma unroll
@@ -357,28 +362,28 @@ __device__ inline void seq_softmax(floatx16 (&s)[NB], int k0, int limit, int wav
   l += sum;  // (this half's keys; the halves meet at the end)
 }
 
-// what both forms do around their tiles: the item, the pair of each lane, the tiles of its keys. A tile of at most 64 pairs
-// leaves waves over: of KG = 2 groups of waves each takes half of a tile's keys (blocks of 32), and the groups' results meet
-// at the end (seq_meet). KGMAX: how many groups the form knows.
-#define SEQ_BEGIN(BK, KGMAX) \
+// What the forms do around their tiles: the item, the pair of each lane, the tiles of its keys. A workgroup takes BQ pairs: 32 a
+// wave, or with KG = 2 groups of waves half of that, each group half of a tile's keys, and the groups' results meet at the end
+// (seq_meet).
+#define SEQ_BEGIN(BK, KG, PACKED) \
+  constexpr int BQ = 32 * SQ_NW / KG, PG = SQ_NW / KG; \
   SeqItem it; \
-  if (!seq_item(a, it)) return; \
+  if (!seq_item<BQ, PACKED>(a, it)) return; \
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ql = lane & 31, hh = lane >> 5; \
   if (it.pair0 >= it.pairs) return; \
-  const int groups = KGMAX > 1 && it.pairs - it.pair0 <= SQ_BQ / 2 ? 2 : 1;  /* of keys */ \
-  const int pgroups = groups == 1 ? SQ_NW : it.pairs - it.pair0 <= 32 ? 1 : 2;  /* of pairs */ \
-  const int kg = groups == 1 ? 0 : wave / pgroups;   /* (2 and 3: a wave that only loads) */ \
-  const int wpair = it.pair0 + 32 * (groups == 1 ? wave : wave % pgroups), pair = min(wpair + ql, it.pairs - 1); \
+  const int kg = wave / PG, wpair = it.pair0 + 32 * (wave % PG), pair = min(wpair + ql, it.pairs - 1); \
   const int limit = wpair + ql < it.pairs ? pair_limit(a, it, pair) : 0; \
-  int wave_max = limit, wave_min = wpair + ql < it.pairs ? limit : 0x7FFFFFFF; \
-  for (int d = 1; d < 32; d <<= 1) { wave_max = max(wave_max, __shfl_xor(wave_max, d, 64)); wave_min = min(wave_min, __shfl_xor(wave_min, d, 64)); } \
-  wave_max = __builtin_amdgcn_readfirstlane(wave_max); wave_min = __builtin_amdgcn_readfirstlane(wave_min); \
-  __shared__ int tops[SQ_NW]; \
-  if (lane == 0) tops[wave] = wave_max; \
-  __syncthreads(); \
-  int keys = tops[0]; \
-  for (int w = 1; w < SQ_NW; ++w) keys = max(keys, tops[w]); \
-  if (kg >= groups) wave_max = 0; \
+  /* what the wave's pairs see at least and at most, and the tile's: a sequence's rows see more and more */ \
+  int wave_min, wave_max, keys; \
+  if (PACKED || it.step >= 0) { \
+    wave_min = pair_limit(a, it, wpair); wave_max = pair_limit(a, it, min(wpair + 31, it.pairs - 1)); \
+    keys = pair_limit(a, it, min(it.pair0 + BQ, it.pairs) - 1); \
+  } else { \
+    wave_max = wave_most(limit); wave_min = -wave_most(wpair + ql < it.pairs ? -limit : -0x7FFFFFFF); \
+    keys = wave_most(max(pair_limit(a, it, it.pair0 + lane), BQ > 64 ? pair_limit(a, it, it.pair0 + 64 + lane) : 0)); \
+  } \
+  wave_min = __builtin_amdgcn_readfirstlane(wave_min); wave_max = __builtin_amdgcn_readfirstlane(wave_max); keys = __builtin_amdgcn_readfirstlane(keys); \
+  if (wpair >= it.pairs) wave_max = 0; \
   const int ntiles = (keys + BK - 1) / BK; \
   const int t0 = (int)((int64_t)ntiles * it.split / it.splits), t1 = (int)((int64_t)ntiles * (it.split + 1) / it.splits); \
   const int64_t qat = (it.row0 + pair / a.rep) * a.ldq + (int64_t)(it.kvh * a.rep + pair % a.rep) * HD; \
@@ -391,8 +396,7 @@ __device__ inline void seq_softmax(floatx16 (&s)[NB], int k0, int limit, int wav
 // The second key group's results into the first's, pair group by pair group, through LDS where the tiles were. False: the
 // wave has given its results away. (All waves of the workgroup call it: behind the last tile's barrier.)
 template <int HD>
-__device__ inline bool seq_meet(float* lds, int groups, int pgroups, int kg, int wave, float& m, float& l, floatx16 (&acc)[HD / 32]) {
-  if (groups == 1) return true;
+__device__ inline bool seq_meet(float* lds, int pgroups, int kg, int wave, float& m, float& l, floatx16 (&acc)[HD / 32]) {
   const int lane = threadIdx.x & 63;
   float* slot = lds + (wave % pgroups) * (HD / 2 + 2) * 64 + lane;
   if (kg == 1) {
@@ -441,14 +445,14 @@ struct SeqTile {
   __device__ static int vswap(int row) { return !ASYNC ? 0 : HD == 128 ? (row & 3) * 4 : ((row >> 1) & 1) * 4; }
 };
 
-// QT, PT: the bf16 terms of q and of the weights
-template <int HD, int CF, int QT, int PT>
+// QT, PT: the bf16 terms of q and of the weights; KG: the groups of waves that share a tile's keys; PACKED: which entry point's
+template <int HD, int CF, int QT, int PT, int KG, bool PACKED>
 __global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf16_kernel(SeqArgs a) {
   constexpr bool ASYNC = CF == FH_BF16;
   using Tile = SeqTile<HD, ASYNC>;
   constexpr int BK = 64, KLD = Tile::KLD, VLD = Tile::VLD, NS = Tile::STAGES;
   __shared__ __attribute__((aligned(256))) uint16_t tiles[NS * Tile::SIZE];
-  SEQ_BEGIN(BK, 2)
+  SEQ_BEGIN(BK, KG, PACKED)
 
   // the lane's q as the product's B: step s holds dimensions 16 s + 8 hh .. + 7, each term
   bf16x8 qf[HD / 16][QT];
@@ -508,16 +512,31 @@ __global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf
       }
     }
   };
-  // blocks kb0 .. kb0 + NB - 1 of 32 keys of the tile in buffer b, whose first key is k0
-  auto work = [&](auto nb, int kb0, int b, int k0) {
-    constexpr int NB = decltype(nb)::value;
+  // this wave's blocks of 32 keys of the tile in buffer b, whose first key is k0
+  constexpr int NB = 2 / KG;
+  auto work = [&](int b, int k0) {
+    const int kb0 = KG == 1 ? 0 : kg;
     const uint16_t* K = tiles + b * Tile::SIZE + 32 * kb0 * KLD;
     const uint16_t* V = tiles + b * Tile::SIZE + BK * KLD + 32 * kb0 * VLD;
-    floatx16 s[NB];
+    floatx16 s[2];
 #pragma unroll
-    for (int kb = 0; kb < NB; ++kb)
+    for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+    if constexpr (NB == 1) {
+      // one block: every read of its keys at once, and two chains of products
+      bf16x8 kf[HD / 16];
+#pragma unroll
+      for (int st = 0; st < HD / 16; ++st) kf[st] = *(const bf16x8*)(K + ql * KLD + 8 * ((2 * st + hh) ^ Tile::kswap(ql)));
+#pragma unroll
+      for (int st = 0; st < HD / 16; st += 2)
+#pragma unroll
+        for (int u = 0; u < QT; ++u)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[st + c], qf[st + c][u], s[c], 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[0][r] += s[1][r];
+    } else {
 #pragma unroll
     for (int st = 0; st < HD / 16; ++st)
 #pragma unroll
@@ -526,6 +545,7 @@ __global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf
 #pragma unroll
         for (int u = 0; u < QT; ++u) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st][u], s[kb], 0, 0, 0);
       }
+    }
     seq_softmax<HD, NB>(s, k0 + 32 * kb0, limit, wave_min, hh, scale2, m, l, acc);
     // O^T += V^T P^T, 16 keys a step: the lane's weights 8 j .. 8 j + 7 of block kb are keys 32 kb + 16 j + {4 hh .. 4 hh + 3,
     // 8 + 4 hh .. 8 + 4 hh + 3}; V's columns come transposed, 4 keys of 16 dimensions to 16 lanes
@@ -553,9 +573,7 @@ __global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf
       }
   };
   auto work_on = [&](int t, int b) {
-    if (groups == 1) {
-      if (t * BK < wave_max) work(std::integral_constant<int, 2>(), 0, b, t * BK);
-    } else if (t * BK + 32 * kg < wave_max) work(std::integral_constant<int, 1>(), kg, b, t * BK);
+    if (t * BK + (KG == 1 ? 0 : 32 * kg) < wave_max) work(b, t * BK);
   };
   if constexpr (ASYNC) {
     // a ring of NS tiles: a tile's wait leaves the next one's loads in flight
@@ -593,19 +611,21 @@ __global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf
     }
   }
   l += __shfl_xor(l, 32, 64);
-  static_assert(2 * 64 * (HD / 2 + 2) * 4 <= (int)sizeof(tiles), "the key groups' place");
-  if (!seq_meet<HD>((float*)tiles, groups, pgroups, kg, wave, m, l, acc)) return;
+  static_assert(KG == 1 || PG * 64 * (HD / 2 + 2) * 4 <= (int)sizeof(tiles), "the key groups' place");
+  if constexpr (KG > 1)
+    if (!seq_meet<HD>((float*)tiles, PG, kg, wave, m, l, acc)) return;
   seq_finish<HD, CF>(a, it, wpair, limit, t0 * BK, min(t1 * BK, keys), acc, m, l);
 }
 
 // The same in fp32: 32 keys a tile. A lane's q holds dimensions HD / 2 hh .. of its half (the order of a sum's products is free),
 // so that K's row is read 16 bytes at a time; P's step r multiplies keys 8 (r / 4) + 4 hh + r % 4, V's rows as they lie.
-template <int HD, int CF>
+template <int HD, bool PACKED>
 __global__ __launch_bounds__(64 * SQ_NW, 2) void seq_f32_kernel(SeqArgs a) {
+  constexpr int CF = FH_F32;
   constexpr int BK = 32, LD = HD + 4;
   __shared__ __attribute__((aligned(16))) float Ks[2][BK * LD];
   __shared__ __attribute__((aligned(16))) float Vs[2][BK * LD];
-  SEQ_BEGIN(BK, 1)
+  SEQ_BEGIN(BK, 1, PACKED)
   float qf[HD / 2];
 #pragma unroll
   for (int s = 0; s < HD / 16; ++s) {
@@ -714,35 +734,41 @@ __global__ __launch_bounds__(256) void seq_join(SeqArgs a) {
   }
 }
 
-template <int HD, int CF>
+template <int HD, int CF, int KG, bool PACKED>
 static void launch_seq(unsigned blocks, hipStream_t s, const SeqArgs& a) {
   const dim3 g(blocks), b(64 * SQ_NW);
-  if constexpr (CF != FH_F32) {
-    if (a.o_bf16) {
-      if (a.q_bf16) hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 1, 1>), g, b, 0, s, a);
-      else hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 2, 1>), g, b, 0, s, a);
-    } else {
-      if (a.q_bf16) hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 1, 3>), g, b, 0, s, a);
-      else hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 3, 3>), g, b, 0, s, a);
-    }
-  } else hipLaunchKernelGGL((seq_f32_kernel<HD, CF>), g, b, 0, s, a);
+  if constexpr (CF == FH_F32) hipLaunchKernelGGL((seq_f32_kernel<HD, PACKED>), g, b, 0, s, a);
+  else if (a.o_bf16) {
+    if (a.q_bf16) hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 1, 1, KG, PACKED>), g, b, 0, s, a);
+    else hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 2, 1, KG, PACKED>), g, b, 0, s, a);
+  } else {
+    if (a.q_bf16) hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 1, 3, KG, PACKED>), g, b, 0, s, a);
+    else hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 3, 3, KG, PACKED>), g, b, 0, s, a);
+  }
+}
+
+template <int HD, int CF>
+static void launch_seq(int pairs, unsigned blocks, hipStream_t s, const SeqArgs& a) {
+  if (!a.starts) launch_seq<HD, CF, 2, false>(blocks, s, a);
+  else if (pairs == 64) launch_seq<HD, CF, 2, true>(blocks, s, a);
+  else launch_seq<HD, CF, 1, true>(blocks, s, a);
 }
 
 template <int HD>
-static void launch_seq(int cf, unsigned blocks, hipStream_t s, const SeqArgs& a) {
+static void launch_seq(int cf, int pairs, unsigned blocks, hipStream_t s, const SeqArgs& a) {
   switch (cf) {
-    case FH_F32: launch_seq<HD, FH_F32>(blocks, s, a); break;
-    case FH_BF16: launch_seq<HD, FH_BF16>(blocks, s, a); break;
-    case FH_BFP8: launch_seq<HD, FH_BFP8>(blocks, s, a); break;
-    default: launch_seq<HD, FH_BFP4>(blocks, s, a); break;
+    case FH_F32: launch_seq<HD, FH_F32>(pairs, blocks, s, a); break;
+    case FH_BF16: launch_seq<HD, FH_BF16>(pairs, blocks, s, a); break;
+    case FH_BFP8: launch_seq<HD, FH_BFP8>(pairs, blocks, s, a); break;
+    default: launch_seq<HD, FH_BFP4>(pairs, blocks, s, a); break;
   }
   if (a.parts > 1) hipLaunchKernelGGL(seq_join<HD>, dim3((unsigned)((a.rows * a.heads + 3) / 4)), dim3(256), 0, s, a);
 }
 
-static int launch_seq(const char* fn, int head_dim, int cf, int64_t blocks, hipStream_t s, const SeqArgs& a) {
+static int launch_seq(const char* fn, int head_dim, int cf, int pairs, int64_t blocks, hipStream_t s, const SeqArgs& a) {
   if (blocks >= (1LL << 31) || (a.rows * a.heads + 3) / 4 >= (1LL << 31)) { set_error("%s: too many rows for one grid", fn); return FH_EUNSUP; }
-  if (head_dim == 128) launch_seq<128>(cf, (unsigned)blocks, s, a);
-  else launch_seq<64>(cf, (unsigned)blocks, s, a);
+  if (head_dim == 128) launch_seq<128>(cf, pairs, (unsigned)blocks, s, a);
+  else launch_seq<64>(cf, pairs, (unsigned)blocks, s, a);
   return check_launch(fn);
 }
 
@@ -754,12 +780,16 @@ static int splits_for(int64_t groups, int64_t keys) {
   const int64_t s = (2 * SQ_CUS + groups - 1) / groups;
   return (int)std::max<int64_t>(1, std::min<int64_t>({s, keys / SQ_SPLIT_KEYS, SQ_MAX_SPLITS}));
 }
-static int64_t packed_tiles(int64_t rows, int n, int rep) { return rows * rep / SQ_BQ + std::min<int64_t>(n, rows); }
+// Pairs a workgroup: 128, or 64 with two groups of waves on a tile's keys: for a decode step (one row a sequence) and prompts of
+// few rows. An fp32 cache's form has no second group.
+static int packed_pairs(int64_t rows, int n, int rep, int cf) { return cf != FH_F32 && rows * rep <= (int64_t)64 * n ? 64 : 128; }
+static int64_t packed_tiles(int64_t rows, int n, int rep, int pairs) { return rows * rep / pairs + std::min<int64_t>(n, rows); }
 static int packed_splits(int64_t rows, int n, int heads, int kv_heads, int64_t max_context) {
-  return splits_for(packed_tiles(rows, n, heads / kv_heads) * kv_heads, max_context);
+  return splits_for(packed_tiles(rows, n, heads / kv_heads, 128) * kv_heads, max_context);
 }
-static void shared_splits(int batch, int heads, int kv_heads, int64_t max_prefix, int64_t max_own, int& tiles, int& prefix, int& own) {
-  tiles = (int)(((int64_t)batch * (heads / kv_heads) + SQ_BQ - 1) / SQ_BQ);
+static void shared_splits(int batch, int heads, int kv_heads, int cf, int64_t max_prefix, int64_t max_own, int& tiles, int& prefix, int& own) {
+  const int pairs = cf == FH_F32 ? 128 : 64;
+  tiles = (int)(((int64_t)batch * (heads / kv_heads) + pairs - 1) / pairs);
   prefix = splits_for((int64_t)tiles * kv_heads, max_prefix);
   own = splits_for((int64_t)batch * kv_heads, max_own);
 }
@@ -818,14 +848,15 @@ extern "C" int fh_attention_prefill_packed(const void* q, int q_dtype, int64_t l
   a.part = (float*)workspace;
   if (a.parts > 1 && (!workspace || ws_bytes < fh_attention_packed_workspace_bytes(rows, sequences, heads, kv_heads, head_dim, max_context) || ((uintptr_t)workspace & 15)))
     return fail(FH_EINVAL, "fh_attention_prefill_packed: a 16-byte aligned workspace of fh_attention_packed_workspace_bytes");
-  return launch_seq(fn, head_dim, cache_dtype, packed_tiles(rows, sequences, a.rep) * a.splits * kv_heads, as_stream(stream), a);
+  const int pairs = packed_pairs(rows, sequences, a.rep, cache_dtype);
+  return launch_seq(fn, head_dim, cache_dtype, pairs, packed_tiles(rows, sequences, a.rep, pairs) * a.splits * kv_heads, as_stream(stream), a);
 }
 
 extern "C" size_t fh_attention_shared_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int64_t max_prefix,
                                                       int64_t max_own) {
   if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || max_prefix < 0 || max_own < 0) return 0;
   int tiles, prefix, own;
-  shared_splits(batch, heads, kv_heads, max_prefix, max_own, tiles, prefix, own);
+  shared_splits(batch, heads, kv_heads, FH_F32, max_prefix, max_own, tiles, prefix, own);  // (the most splits of any cache)
   return (size_t)batch * heads * (prefix + own) * (head_dim + 2) * sizeof(float);
 }
 
@@ -850,10 +881,10 @@ extern "C" int fh_attention_decode_shared(const void* q, int q_dtype, const void
   a.rep = heads / kv_heads;
   a.cache_exps = (const uint8_t*)cache + kv_exps_at(cache_dtype, kv_heads, cache_len, head_dim);
   a.scale = 1.0f / sqrtf((float)head_dim);
-  shared_splits(batch, heads, kv_heads, max_prefix, max_own, a.tiles, a.splits, a.own_splits);
+  shared_splits(batch, heads, kv_heads, cache_dtype, max_prefix, max_own, a.tiles, a.splits, a.own_splits);
   a.parts = a.splits + a.own_splits;
   a.part = (float*)workspace;
   if (!workspace || ws_bytes < fh_attention_shared_workspace_bytes(batch, heads, kv_heads, head_dim, max_prefix, max_own) || ((uintptr_t)workspace & 15))
     return fail(FH_EINVAL, "fh_attention_decode_shared: a 16-byte aligned workspace of fh_attention_shared_workspace_bytes");
-  return launch_seq(fn, head_dim, cache_dtype, ((int64_t)a.tiles * a.splits + (int64_t)batch * a.own_splits) * kv_heads, as_stream(stream), a);
+  return launch_seq(fn, head_dim, cache_dtype, 64, ((int64_t)a.tiles * a.splits + (int64_t)batch * a.own_splits) * kv_heads, as_stream(stream), a);
 }
