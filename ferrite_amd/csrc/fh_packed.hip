@@ -371,7 +371,8 @@ __device__ inline void seq_softmax(floatx16* s, int k0, int limit, int wave_min,
   if (!seq_item<BQ, PACKED>(a, it)) return; \
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ql = lane & 31, hh = lane >> 5; \
   if (it.pair0 >= it.pairs) return; \
-  const int kg = wave / PG, wpair = it.pair0 + 32 * (wave % PG), pair = min(wpair + ql, it.pairs - 1); \
+  [[maybe_unused]] const int kg = wave / PG; \
+  const int wpair = it.pair0 + 32 * (wave % PG), pair = min(wpair + ql, it.pairs - 1); \
   const int limit = wpair + ql < it.pairs ? pair_limit(a, it, pair) : 0; \
   /* what the wave's pairs see at least and at most, and the tile's: a sequence's rows see more and more */ \
   int wave_min, wave_max, keys; \
@@ -772,13 +773,14 @@ static int launch_seq(const char* fn, int head_dim, int cf, int pairs, int64_t b
   return check_launch(fn);
 }
 
-// Workgroups the keys of a tile are split among: enough that the grid has two a CU, each with 4 tiles of 64 keys or more,
-// at most 32 (a wave joins the parts, a lane each)
-constexpr int SQ_CUS = 256, SQ_SPLIT_KEYS = 256, SQ_MAX_SPLITS = 32;
+// Workgroups the keys of a tile are split among: enough that the grid has two a CU, each with 4 tiles of 64 keys or more, or
+// 8 of fewer keys where there are not so many, at most 32 (a wave joins the parts, a lane each)
+constexpr int SQ_CUS = 256, SQ_SPLIT_KEYS = 256, SQ_SHORT_KEYS = 64, SQ_MAX_SPLITS = 32;
 static int splits_for(int64_t groups, int64_t keys) {
   if (groups >= SQ_CUS) return 1;
   const int64_t s = (2 * SQ_CUS + groups - 1) / groups;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({s, keys / SQ_SPLIT_KEYS, SQ_MAX_SPLITS}));
+  const int64_t most = std::max(keys / SQ_SPLIT_KEYS, std::min<int64_t>(8, keys / SQ_SHORT_KEYS));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({s, most, SQ_MAX_SPLITS}));
 }
 // Pairs a workgroup: 128, or 64 with two groups of waves on a tile's keys: for a decode step (one row a sequence) and prompts of
 // few rows. An fp32 cache's form has no second group.
@@ -791,7 +793,7 @@ static void shared_splits(int batch, int heads, int kv_heads, int cf, int64_t ma
   const int pairs = cf == FH_F32 ? 128 : 64;
   tiles = (int)(((int64_t)batch * (heads / kv_heads) + pairs - 1) / pairs);
   prefix = splits_for((int64_t)tiles * kv_heads, max_prefix);
-  own = splits_for((int64_t)batch * kv_heads, max_own);
+  own = splits_for((int64_t)batch * kv_heads * 2, max_own);  // (the prefix has the other half of the GPU)
 }
 
 // what both entry points ask of their operands (fn: the name in the message)
