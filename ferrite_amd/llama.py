@@ -22,6 +22,10 @@ the residual stream fp32 and each GEMM's input bf16 (as ferrite's chip feeds its
   gate_up fh_gemm_bfp  silu(gate) * up (bf16 out)
   down    fh_gemm_bfp  + the residual, with x's sums of squares
 then the final norm and the output layer for the last row only (fh_gemv_bfp), and its argmax.
+
+Many prompts go in together (prefill_batch): their rows packed one after another through the same matmuls, the attention
+fh_attention_prefill_packed. A batch whose sequences begin alike keeps that prefix once (share_prefix): its rows' attention is
+fh_attention_decode_shared, their own slots hold what follows the prefix.
 """
 import math
 from types import SimpleNamespace
@@ -168,7 +172,11 @@ class Decoder:
     self.parts = torch.zeros(B, c.vocab // 16, dtype=torch.int64, device=self.device)  # each run of 16 logits' best
     self.ws = ops.attention_workspace(B, c.heads, hd, context, self.device)
     self.graph = None
-    self.top = 0  # the largest place of the rows set (set_rows), which advance raises
+    # the shared prefix (share_prefix): its slot, its places, each row's of them, the same on the GPU; none at first
+    self.prefix_slot, self.prefix_len, self.shared_host = None, 0, np.zeros(B, np.int32)
+    self.prefix_row, self.shared = (torch.zeros(n, dtype=torch.int32, device=self.device) for n in (1, B))
+    self.top = 0  # the largest place of the rows set (set_rows), which advance raises,
+    self.top_own = 0  # and the largest behind the prefix: the row of its slot
 
   def weight_bytes(self):
     """Bytes of the weights one decode step reads: every matrix, a row of the embedding, the norms."""
@@ -176,8 +184,37 @@ class Decoder:
     return n + self.c.dim * 2 + (2 * self.c.layers + 1) * self.c.dim * 4
 
   def set_rows(self, places, slots=None):
-    """Each row's place, and the cache rows: slot s's sequence keeps rows s * context .. (models/llama.py:429-452)."""
+    """Each row's place, and the cache rows: slot s's sequence keeps rows s * context .. (models/llama.py:429-452), from the
+    first place behind the prefix on where the row shares one (share_prefix)."""
     self._put(places=places, slots=slots)
+
+  def share_prefix(self, slot=None, length=0, rows=None):
+    """The first `length` places of slot `slot` (a prompt prefilled there) become the prefix of the batch's sequences: row b
+    shares the first rows[b] of them (all of them by default), kept once and read once a step, and its own slot holds its
+    places from rows[b] on. A sequence may then have rows[b] + context places. The prefix's slot is not a row's while one
+    shares it. share_prefix() ends it. The rows are set again afterwards (set_rows, step's places)."""
+    if slot is None:
+      slot, length, rows = None, 0, np.zeros(self.batch, np.int32)
+    else:
+      if not 0 <= slot < self.slots: raise ValueError(f"share_prefix: slot {slot} outside 0..{self.slots - 1}")
+      if not 1 <= length <= min(self.context, self.c.places): raise ValueError(f"share_prefix: {length} places of a slot of {self.context}")
+      rows = np.full(self.batch, length, np.int32) if rows is None else np.asarray(rows, np.int32)
+      if rows.shape != (self.batch,) or (rows < 0).any() or (rows > length).any(): raise ValueError(f"share_prefix: {self.batch} rows' counts in 0..{length}")
+      ops.attention_heads_ok(self.c.heads, self.c.kv, self.hd)
+    self.prefix_slot, self.prefix_len, self.shared_host = slot, int(length), rows
+    ops.put_i32(rows, self.shared)
+    ops.put_i32([(slot or 0) * self.part], self.prefix_row)
+    self.ws_shared = ops.attention_shared_workspace(self.batch, self.c.heads, self.c.kv, self.hd, length, self.context, self.device) if slot is not None else None
+    self.graph = None  # (the step is captured again)
+
+  def _attend(self, l, out):
+    """A step's attention over block l's cache."""
+    c = self.c
+    if self.prefix_slot is None:
+      ops.attention_decode(self.q, self.cache[l], c.heads, c.kv, self.hd, self.places, self.first, self.context, self.ws, o=out)
+    else:
+      ops.attention_decode_shared(self.q, self.cache[l], c.heads, c.kv, self.hd, self.places, self.first, self.prefix_row, self.shared,
+                                  self.prefix_len, self.context, workspace=self.ws_shared, o=out)
 
   def _put(self, ids=None, places=None, slots=None):
     """The rows' tokens, and their places and slots where places is given: what the host holds by one launch whose
@@ -194,18 +231,21 @@ class Decoder:
     if places.shape != (self.batch,) or slots.shape != (self.batch,): raise ValueError(f"set_rows: {self.batch} places and slots")
     host = not (places.is_cuda or slots.is_cuda)
     p, s = (places.numpy(), slots.numpy()) if host else (places, slots)
-    if (p < 0).any() or (p >= min(self.context, self.c.places)).any(): raise ValueError("a place past the cache or RoPE's tables")
+    sh = self.shared_host if host else self.shared
+    if not host: p, s = p.to(self.device), s.to(self.device)
+    if (p < sh).any() or (p - sh >= self.context).any() or (p >= self.c.places).any(): raise ValueError("a place inside the shared prefix, or past the cache or RoPE's tables")
     if (s < 0).any() or (s >= self.slots).any(): raise ValueError(f"a slot outside 0..{self.slots - 1}")
-    self.top = int(p.max())  # (the largest place, kept on the host for advance's check)
+    if self.prefix_slot is not None and (s == self.prefix_slot).any(): raise ValueError(f"slot {self.prefix_slot} holds the shared prefix")
+    self.top, self.top_own = int(p.max()), int((p - sh).max())  # (kept on the host for advance's check)
     if host:
       first = s * np.int32(self.part)
-      v = [p, first, first + p]
+      v = [p, first, first + p - sh]
       ops.put_i32(np.concatenate(v if ids is None else [ids.numpy(), *v]), self._int[1 if ids is None else 0:])
       return
     if ids is not None: ops.put_i32(ids.numpy(), self.ids)
-    self.places.copy_(places)
-    self.first.copy_(slots * self.part)
-    self.rows.copy_(slots * self.part + places)
+    self.places.copy_(p)
+    self.first.copy_(s * self.part)
+    self.rows.copy_(s * self.part + p - sh)
 
   def _cache(self, l):
     data, dtype, length = ops.cache_fields(self.cache[l])
@@ -220,7 +260,7 @@ class Decoder:
                         heads=c.heads, kv_heads=c.kv, head_dim=hd, cos_tab=self.cos, sin_tab=self.sin, rope_rows=self.cos.shape[0],
                         places=self.places, cache_rows=self.rows, **self._cache(l))
       ops.gemv(self.x, L.qkv, ep, out=self.q)
-      ops.attention_decode(self.q, self.cache[l], c.heads, c.kv, hd, self.places, self.first, self.context, self.ws, o=self.att)
+      self._attend(l, self.att)
       ep = ops.epilogue(lib.EP_RESIDUAL, residual=self.x, ssq_out=self.ssq)
       ops.gemv(self.att, L.o, ep, out=self.x)
       ep = ops.epilogue(lib.EP_SILU_GATE, norm_w=L.norm2, ssq_in=self.ssq, eps=c.eps, centered=int(c.centered), split=c.ffn)
@@ -257,7 +297,7 @@ class Decoder:
         ops.gemm(self.xn, L.qkv, ops.epilogue(lib.EP_ROPE_KV, **rope), out=self.q)
       else:
         ops.gemm(self.xn, L.qkv, ops.epilogue(lib.EP_ROPE_KV, **rs, **rope), out=self.q)
-      ops.attention_decode(self.q, self.cache[l], c.heads, c.kv, hd, self.places, self.first, self.context, self.ws, o=self.attb)
+      self._attend(l, self.attb)
       ops.gemm(self.attb, L.o, ops.epilogue(lib.EP_RESIDUAL, residual=self.x, ssq_out=self.ssq, copy_bf16=self.xn,
                                            copy_w=nw[2 * l + 1]), out=self.x)
       ops.gemm(self.xn, L.gate_up, ops.epilogue(lib.EP_SILU_GATE, split=c.ffn, **rs), out=self.hb)
@@ -288,6 +328,7 @@ class Decoder:
     T = len(ids)
     if T < 1 or p0 < 0 or p0 + T > min(self.context, self.c.places): raise ValueError("prefill: the prompt's places past the cache or RoPE's tables")
     if not 0 <= slot < self.slots: raise ValueError(f"prefill: slot {slot} outside 0..{self.slots - 1}")
+    if self.prefix_slot not in (None, slot): raise ValueError("prefill: sequences behind a shared prefix go through prefill_batch")
     chunk = chunk or T
     for a in range(0, T, chunk):
       out = self._prefill_chunk(ids[a:a + chunk], slot, p0 + a)
@@ -322,6 +363,61 @@ class Decoder:
     ops.argmax_parts(P.parts, P.pick)
     return P.logits, P.pick
 
+  def prefill_batch(self, prompts, slots=None, p0=None, shared=None):
+    """Prompts of many sequences at once, on the matrix cores: prompt i's tokens at places p0[i], p0[i] + 1, ... of slot
+    slots[i] (slot i by default), each slot once; the first shared[i] places are the prefix's (share_prefix; by default all of them,
+    none without one) and p0 begins behind them by default. Their keys and values go into the cache; returns each prompt's
+    last token's logits ([n][vocab] fp32) and greedy picks ([n] int32). The rows of all prompts go through the matmuls
+    together, so a prompt's logits have prefill's values within the rounding of bf16 rows and fp32 sums."""
+    c, hd, dev = self.c, self.hd, self.device
+    n = len(prompts)
+    if n < 1: raise ValueError("prefill_batch: no prompt")
+    lens = np.array([len(p) for p in prompts], np.int64)
+    slots = np.arange(n) if slots is None else np.asarray(slots, np.int64)
+    sh = np.full(n, self.prefix_len, np.int64) if shared is None else np.asarray(shared, np.int64)
+    p0 = sh if p0 is None else np.asarray(p0, np.int64)
+    if not slots.shape == sh.shape == p0.shape == (n,): raise ValueError(f"prefill_batch: {n} slots, p0 and shared")
+    if (lens < 1).any(): raise ValueError("prefill_batch: an empty prompt")
+    if (slots < 0).any() or (slots >= self.slots).any() or len(set(slots.tolist())) != n: raise ValueError(f"prefill_batch: each slot once, in 0..{self.slots - 1}")
+    if (sh < 0).any() or (sh > self.prefix_len).any(): raise ValueError(f"prefill_batch: shared in 0..{self.prefix_len}")
+    if self.prefix_slot is not None and (slots == self.prefix_slot).any(): raise ValueError(f"prefill_batch: slot {self.prefix_slot} holds the shared prefix")
+    if (p0 < sh).any() or (p0 - sh + lens > self.context).any() or (p0 + lens > c.places).any():
+      raise ValueError("prefill_batch: a prompt's places inside the shared prefix, or past the cache or RoPE's tables")
+    T, starts = int(lens.sum()), np.concatenate([[0], np.cumsum(lens)])
+    P = self._prefill_buffers(T)
+    of = np.repeat(np.arange(n), lens)  # each row's prompt
+    places = np.arange(T) - starts[of] + p0[of]
+    rows = slots[of] * self.part + places - sh[of]
+    ids = np.concatenate([np.asarray(p, np.int64) for p in prompts])
+    ints = np.concatenate([ids, places, rows, starts, p0, slots * self.part, sh, starts[1:] - 1]).astype(np.int32)
+    held = torch.empty(ints.size, dtype=torch.int32, device=dev)
+    if ints.size <= PUT_MAX: ops.put_i32(ints, held)
+    else: held.copy_(torch.from_numpy(ints))
+    ids_t, places_t, rows_t, starts_t, p0_t, first_t, sh_t, last_t = held.split([T, T, T, n + 1, n, n, n, n])
+    prefix = dict(prefix_row=self.prefix_row, shared=sh_t) if sh.any() else {}
+    most = int((p0 + lens).max())
+    ws = ops.attention_packed_workspace(T, n, c.heads, c.kv, hd, most, dev)
+    x, ssq, xn, q, att, h = P.x[:T], P.ssq[:T], P.xn[:T], P.q[:T], P.att[:T], P.h[:T]
+    ops.embed_rows(self.embed, ids_t, x, ssq)
+    for l, L in enumerate(self.layers):
+      ops.rms_rows(x, L.norm1, c.eps, c.centered, out=xn)
+      ep = ops.epilogue(lib.EP_ROPE_KV, heads=c.heads, kv_heads=c.kv, head_dim=hd, cos_tab=self.cos, sin_tab=self.sin, rope_rows=self.cos.shape[0],
+                        places=places_t, cache_rows=rows_t, **self._cache(l))
+      ops.gemm(xn, L.qkv, ep, out=q)
+      ops.attention_prefill_packed(q, self.cache[l], c.heads, c.kv, hd, starts_t, p0_t, first_t, most, workspace=ws, o=att, **prefix)
+      ops.gemm(att, L.o, ops.epilogue(lib.EP_RESIDUAL, residual=x), out=x)
+      ops.rms_rows(x, L.norm2, c.eps, c.centered, out=xn)
+      ops.gemm(xn, L.gate_up, ops.epilogue(lib.EP_SILU_GATE, split=c.ffn), out=h)
+      ops.gemm(h, L.down, ops.epilogue(lib.EP_RESIDUAL, residual=x), out=x)
+    # each prompt's last row: the final norm and the output layer (bf16 rows on the matrix cores from three prompts on)
+    xl = ops.gather_rows(x, last_t)
+    few = n < 3
+    xl = ops.rms_rows(xl, self.norm, c.eps, c.centered, out_dtype=torch.float32 if few else torch.bfloat16)
+    logits = torch.empty(n, c.vocab, dtype=torch.float32, device=dev)
+    parts = torch.empty(n, c.vocab // 16, dtype=torch.int64, device=dev)
+    (ops.gemv if few else ops.gemm)(xl, self.head, ops.epilogue(lib.EP_STORE, argmax_parts=parts), out=logits)
+    return logits, ops.argmax_parts(parts)
+
   def step(self, ids=None, places=None, slots=None, replay=True):
     """One step: the logits (fp32, [batch][vocab]) and picks for tokens ids at places. With replay, the step runs as
     a HIP graph captured on the first call (every later step launches the same kernels: places are data)."""
@@ -343,18 +439,24 @@ class Decoder:
     """Each row's next place and its pick as the next token, on the GPU (no host round trip): greedy decoding. Raises
     once a row's next place would pass the cache or RoPE's tables (the host keeps the largest place: set_rows', plus
     one a call)."""
-    if self.top + 1 >= min(self.context, self.c.places): raise ValueError(f"advance: place {self.top + 1} past the cache or RoPE's tables")
+    if self.top_own + 1 >= self.context or self.top + 1 >= self.c.places: raise ValueError(f"advance: place {self.top + 1} past the cache or RoPE's tables")
     self.top += 1
+    self.top_own += 1
     self.ids.copy_(self.picks)
     self.places.add_(1)
     self.rows.add_(1)
 
-  def heads(self, k=64, inv_temp=None):
+  def heads(self, k=64, inv_temp=None, rules=None):
     """The last step's logit heads (models/serve.py:31-47): each row's k best logits and their tokens, and given each
-    row's 1/temperature, the log of the sum of exp(x t) over its row (ops.logit_heads: fh_logit_heads)."""
+    row's 1/temperature, the log of the sum of exp(x t) over its row (ops.logit_heads: fh_logit_heads). rules: ops.logit_rules'
+    arguments (each request's penalties, biases and grammar mask), whose logits the heads are then of; the step's own stay."""
+    logits = self.logits
+    if rules:
+      if getattr(self, "_ruled", None) is None: self._ruled = torch.empty_like(self.logits)
+      logits = ops.logit_rules(self.logits, out=self._ruled, **rules)
     if inv_temp is not None and not isinstance(inv_temp, torch.Tensor):
       inv_temp = torch.as_tensor(inv_temp, dtype=torch.float32, device=self.device).reshape(-1)
-    return ops.logit_heads(self.logits, k, inv_temp)
+    return ops.logit_heads(logits, k, inv_temp)
 
 
 def numpy_weights(w):

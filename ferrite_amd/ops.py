@@ -378,6 +378,12 @@ def _cache_of(what, cache, kv_heads, head_dim):
   return data, dtype, length
 
 
+def attention_heads_ok(heads, kv_heads, head_dim):
+  """Raises unless the attention of many sequences takes these heads."""
+  if head_dim not in (64, 128): raise NotImplementedError("attention of many sequences: head_dim 64 or 128")
+  if heads % kv_heads: raise ValueError("heads must be a multiple of kv_heads")
+
+
 def attention_packed_workspace(rows, sequences, heads, kv_heads, head_dim, max_context, device="cuda"):
   """fh_attention_prefill_packed's workspace, uninitialised (a workspace needs no clearing)."""
   n = lib.load().fh_attention_packed_workspace_bytes(rows, sequences, heads, kv_heads, head_dim, max_context)
@@ -445,6 +451,18 @@ def attention_decode_shared(q, cache, heads, kv_heads, head_dim, places, first_r
            _ptr(first_row), _ptr(prefix_row), _ptr(shared), max_prefix, max_own, op, odt, _ptr(workspace),
            workspace.numel() if workspace is not None else 0, _stream())
   return o
+
+
+def gather_rows(x, ids):
+  """Rows ids (int32 on the GPU) of x [rows][cols] (4-byte elements, rows contiguous), a copy (fh_gather_rows): an index
+  outside x reads its nearest row."""
+  _dev(x, ids)
+  if x.dim() != 2 or x.element_size() != 4 or x.stride(1) != 1: raise ValueError("gather_rows: rows of 4-byte elements")
+  _int_vector("gather_rows", "ids", ids, ids.numel())
+  out = torch.empty(ids.numel(), x.shape[1], dtype=x.dtype, device=x.device)
+  row = 4 * x.shape[1]
+  lib.call("fh_gather_rows", _ptr(x), x.shape[0], 4 * x.stride(0), 0, _ptr(ids), ids.numel(), row, 1, _ptr(out), row, 0, _stream())
+  return out
 
 
 def rms_rows(x, w, eps, centered=False, out=None, out_dtype=torch.bfloat16):
