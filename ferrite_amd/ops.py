@@ -349,33 +349,48 @@ def attention_prefill(q, cache, heads, kv_heads, head_dim, p0, slot_row, o=None,
   return o
 
 
+_I32, _F32 = torch.int32, torch.float32
+
+
 def _rows_operand(what, q, cols):
-  """q [rows][cols] (fp32 or bf16, rows contiguous), its device the current one: what an entry point reads rows of."""
+  """q [rows][cols] (fp32 or bf16, rows contiguous), its device the current one: what an entry point reads rows of. Returns
+  its rows."""
   _dev(q)
-  if q.dim() != 2 or q.shape[0] < 1 or q.shape[1] != cols or q.dtype not in _TORCH or q.stride(1) != 1:
-    raise ValueError(f"{what}: q [rows][{cols}] fp32 or bf16 with contiguous rows, not {tuple(q.shape)} {q.dtype}")
+  shape = q.shape
+  if len(shape) != 2 or shape[0] < 1 or shape[1] != cols or q.dtype not in _TORCH or q.stride()[1] != 1:
+    raise ValueError(f"{what}: q [rows][{cols}] fp32 or bf16 with contiguous rows, not {tuple(shape)} {q.dtype}")
+  return shape[0]
 
 
-def _here(what, device, *ts):
-  """Each tensor (or None) on `device`, and that device the current one, whose stream the call goes to."""
-  if device.type != "cuda" or _device() not in (None, device.index): raise ValueError(f"{what}: tensors must be on the current GPU")
+def _here(what, *ts):
+  """Each tensor (or None) on the current GPU, whose stream the call goes to (the first is a tensor on a GPU)."""
+  d = ts[0].get_device()
+  if _device() not in (None, d): raise ValueError(f"{what}: tensors must be on the current GPU")
   for t in ts:
-    if t is not None and t.device != device: raise ValueError(f"{what}: tensors must be on one GPU")
+    if t is not None and t.get_device() != d: raise ValueError(f"{what}: tensors must be on one GPU")
 
 
-def _int_vector(what, name, t, n):
-  if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or (n > 1 and t.stride(0) != 1):
-    raise ValueError(f"{what}: {name} is {n} contiguous int32 on the GPU")
+def _vector(what, name, t, shape, dtype=_I32):
+  if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+    raise ValueError(f"{what}: {name} is {shape[0]} contiguous {dtype} on the GPU")
 
 
 def _cache_of(what, cache, kv_heads, head_dim):
-  """cache_fields of a cache of kv_heads heads of head_dim, contiguous."""
+  """cache_fields of a contiguous cache of kv_heads heads of head_dim."""
   data, dtype, length = cache_fields(cache)
-  if tuple(cache.shape) != (2 * kv_heads, length, head_dim) or not data.is_contiguous():
+  if cache.shape != (2 * kv_heads, length, head_dim) or not data.is_contiguous():
     raise ValueError(f"{what}: a contiguous cache [{2 * kv_heads}][len][{head_dim}], not {tuple(cache.shape)}")
   if isinstance(cache, BfpCache) and data.numel() < lib.load().fh_kv_cache_bytes(dtype, kv_heads, length, head_dim):
     raise ValueError(f"{what}: the cache's buffer is smaller than its shape")
   return data, dtype, length
+
+
+@functools.lru_cache(maxsize=1024)
+def _packed_bytes(*sizes): return lib.load().fh_attention_packed_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=1024)
+def _shared_bytes(*sizes): return lib.load().fh_attention_shared_workspace_bytes(*sizes)
 
 
 def attention_heads_ok(heads, kv_heads, head_dim):
@@ -386,7 +401,7 @@ def attention_heads_ok(heads, kv_heads, head_dim):
 
 def attention_packed_workspace(rows, sequences, heads, kv_heads, head_dim, max_context, device="cuda"):
   """fh_attention_prefill_packed's workspace, uninitialised (a workspace needs no clearing)."""
-  n = lib.load().fh_attention_packed_workspace_bytes(rows, sequences, heads, kv_heads, head_dim, max_context)
+  n = _packed_bytes(rows, sequences, heads, kv_heads, head_dim, max_context)
   return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
 
 
@@ -399,29 +414,38 @@ def attention_prefill_packed(q, cache, heads, kv_heads, head_dim, starts, p0, fi
   GPU, read when the kernel runs. max_context bounds every place + 1. o (fp32 or bf16) keeps its rows that are no
   sequence's; a new o has zeros there."""
   what = "attention_prefill_packed"
-  _rows_operand(what, q, heads * head_dim)
+  cols = heads * head_dim
+  T = _rows_operand(what, q, cols)
   data, dtype, length = _cache_of(what, cache, kv_heads, head_dim)
-  T, n = q.shape[0], p0.numel()
-  _int_vector(what, "starts", starts, n + 1)
-  for name, t in (("p0", p0), ("first_row", first_row)): _int_vector(what, name, t, n)
-  if (shared is None) != (prefix_row is None): raise ValueError(f"{what}: shared and prefix_row go together")
-  if shared is not None:
-    _int_vector(what, "shared", shared, n)
-    _int_vector(what, "prefix_row", prefix_row, 1)
-  if o is None: o = torch.zeros(T, heads * head_dim, dtype=out_dtype, device=q.device)
-  if o.shape != q.shape or o.dtype not in _TORCH or o.stride(1) != 1: raise ValueError(f"{what}: o is fp32 or bf16 rows of q's shape")
-  need = lib.load().fh_attention_packed_workspace_bytes(T, n, heads, kv_heads, head_dim, max_context)
-  if need and workspace is None: workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-  _here(what, q.device, data, starts, p0, first_row, prefix_row, shared, o, workspace)
-  lib.call("fh_attention_prefill_packed", _ptr(q), _TORCH[q.dtype], q.stride(0), _ptr(data), dtype, length, T, n, heads, kv_heads,
-           head_dim, _ptr(starts), _ptr(p0), _ptr(first_row), _ptr(prefix_row), _ptr(shared), max_context, _ptr(o), _TORCH[o.dtype],
-           o.stride(0), _ptr(workspace), workspace.numel() if workspace is not None else 0, _stream())
+  n = p0.numel()
+  _vector(what, "starts", starts, (n + 1,))
+  _vector(what, "p0", p0, (n,))
+  _vector(what, "first_row", first_row, (n,))
+  if shared is None:
+    if prefix_row is not None: raise ValueError(f"{what}: shared and prefix_row go together")
+    pre, sh = None, None
+  else:
+    if prefix_row is None: raise ValueError(f"{what}: shared and prefix_row go together")
+    _vector(what, "shared", shared, (n,))
+    _vector(what, "prefix_row", prefix_row, (1,))
+    pre, sh = prefix_row.data_ptr(), shared.data_ptr()
+  if o is None: o = torch.zeros(T, cols, dtype=out_dtype, device=q.device)
+  elif o.shape != (T, cols): raise ValueError(f"{what}: o is fp32 or bf16 rows of q's shape")
+  ldo, unit = o.stride()
+  if o.dtype not in _TORCH or unit != 1: raise ValueError(f"{what}: o is fp32 or bf16 rows of q's shape")
+  ws, need = None, _packed_bytes(T, n, heads, kv_heads, head_dim, max_context)
+  if need:
+    if workspace is None: workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    ws, need = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+  _here(what, q, data, starts, p0, first_row, prefix_row, shared, o, workspace)
+  lib.call("fh_attention_prefill_packed", q.data_ptr(), _TORCH[q.dtype], q.stride()[0], data.data_ptr(), dtype, length, T, n, heads, kv_heads,
+           head_dim, starts.data_ptr(), p0.data_ptr(), first_row.data_ptr(), pre, sh, max_context, o.data_ptr(), _TORCH[o.dtype], ldo, ws, need, _stream())
   return o
 
 
 def attention_shared_workspace(batch, heads, kv_heads, head_dim, max_prefix, max_own, device="cuda"):
   """fh_attention_decode_shared's workspace, uninitialised (a workspace needs no clearing)."""
-  n = lib.load().fh_attention_shared_workspace_bytes(batch, heads, kv_heads, head_dim, max_prefix, max_own)
+  n = _shared_bytes(batch, heads, kv_heads, head_dim, max_prefix, max_own)
   return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
 
 
@@ -433,23 +457,27 @@ def attention_decode_shared(q, cache, heads, kv_heads, head_dim, places, first_r
   bounds shared, max_own the places behind it. A row at place -1 sees nothing and gives zeros. o: contiguous fp32 or bf16 of
   q's shape, or Tiles16."""
   what = "attention_decode_shared"
-  _rows_operand(what, q, heads * head_dim)
+  cols = heads * head_dim
+  batch = _rows_operand(what, q, cols)
   if not q.is_contiguous(): raise ValueError(f"{what}: q contiguous")
   data, dtype, length = _cache_of(what, cache, kv_heads, head_dim)
-  batch = q.shape[0]
-  for name, t in (("places", places), ("first_row", first_row), ("shared", shared)): _int_vector(what, name, t, batch)
-  _int_vector(what, "prefix_row", prefix_row, 1)
-  if o is None: o = torch.empty(batch, heads * head_dim, dtype=out_dtype, device=q.device)
+  _vector(what, "places", places, (batch,))
+  _vector(what, "first_row", first_row, (batch,))
+  _vector(what, "shared", shared, (batch,))
+  _vector(what, "prefix_row", prefix_row, (1,))
+  if o is None: o = torch.empty(batch, cols, dtype=out_dtype, device=q.device)
   if isinstance(o, Tiles16):
-    if (o.rows, o.cols) != tuple(q.shape): raise ValueError(f"{what}: o tiles of q's shape")
-  elif o.dtype not in _TORCH or o.shape != q.shape or not o.is_contiguous(): raise ValueError(f"{what}: o is a contiguous fp32 or bf16 tensor of q's shape")
-  need = lib.load().fh_attention_shared_workspace_bytes(batch, heads, kv_heads, head_dim, max_prefix, max_own)
-  if need and workspace is None: workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-  _here(what, q.device, data, places, first_row, prefix_row, shared, o.data if isinstance(o, Tiles16) else o, workspace)
-  op, odt, _, _ = _layout(o)
-  lib.call("fh_attention_decode_shared", _ptr(q), _TORCH[q.dtype], _ptr(data), dtype, length, batch, heads, kv_heads, head_dim, _ptr(places),
-           _ptr(first_row), _ptr(prefix_row), _ptr(shared), max_prefix, max_own, op, odt, _ptr(workspace),
-           workspace.numel() if workspace is not None else 0, _stream())
+    if (o.rows, o.cols) != (batch, cols): raise ValueError(f"{what}: o tiles of q's shape")
+    out, odt = o.data, lib.BF16_T16
+  else:
+    if o.dtype not in _TORCH or o.shape != (batch, cols) or not o.is_contiguous(): raise ValueError(f"{what}: o is a contiguous fp32 or bf16 tensor of q's shape")
+    out, odt = o, _TORCH[o.dtype]
+  if workspace is None:
+    workspace = torch.empty(_shared_bytes(batch, heads, kv_heads, head_dim, max_prefix, max_own), dtype=torch.uint8, device=q.device)
+  _here(what, q, data, places, first_row, prefix_row, shared, out, workspace)
+  lib.call("fh_attention_decode_shared", q.data_ptr(), _TORCH[q.dtype], data.data_ptr(), dtype, length, batch, heads, kv_heads, head_dim,
+           places.data_ptr(), first_row.data_ptr(), prefix_row.data_ptr(), shared.data_ptr(), max_prefix, max_own, out.data_ptr(), odt,
+           workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream())
   return o
 
 
@@ -458,7 +486,7 @@ def gather_rows(x, ids):
   outside x reads its nearest row."""
   _dev(x, ids)
   if x.dim() != 2 or x.element_size() != 4 or x.stride(1) != 1: raise ValueError("gather_rows: rows of 4-byte elements")
-  _int_vector("gather_rows", "ids", ids, ids.numel())
+  _vector("gather_rows", "ids", ids, (ids.numel(),))
   out = torch.empty(ids.numel(), x.shape[1], dtype=x.dtype, device=x.device)
   row = 4 * x.shape[1]
   lib.call("fh_gather_rows", _ptr(x), x.shape[0], 4 * x.stride(0), 0, _ptr(ids), ids.numel(), row, 1, _ptr(out), row, 0, _stream())
@@ -543,6 +571,20 @@ def logit_heads(logits, k=64, inv_temp=None, ws=None):
   return (values, ids) if lse is None else (values, ids, lse)
 
 
+def _matrix(what, name, t, rows, dtype, cols=0):
+  """(t, its pointer, rows apart, columns) of a [rows][at least cols] operand with contiguous rows, (None, None, 0, 0) for None.
+  Rows that overlap, as one row expanded to all of them, become each its own."""
+  if t is None: return None, None, 0, 0
+  shape, st = t.shape, t.stride()
+  if t.dtype is not dtype or len(shape) != 2 or shape[0] != rows or shape[1] < cols or (st[1] != 1 and shape[1] > 1):
+    raise ValueError(f"{what}: {name} is [{rows}][{cols or 'any'}] {dtype} with contiguous rows")
+  ld = st[0]
+  if ld < shape[1]:
+    if rows > 1: t = t.contiguous()
+    ld = shape[1]  # (one row's stride may be anything)
+  return t, t.data_ptr() if shape[1] else None, ld, shape[1]
+
+
 def logit_rules(logits, tokens=None, lengths=None, prompt_lengths=None, repetition=None, presence=None, frequency=None, bias_ids=None,
                 bias=None, allowed=None, out=None):
   """Each request's rules on its row of logits [rows][vocab] (fp32), into out (a new tensor by default; logits itself for
@@ -553,36 +595,30 @@ def logit_rules(logits, tokens=None, lengths=None, prompt_lengths=None, repetiti
   rounded up] int32, bit c % 32 of word c / 32 for column c. Each may be left out."""
   what = "logit_rules"
   _dev(logits)
-  if logits.dtype != torch.float32 or logits.dim() != 2 or logits.shape[0] < 1 or logits.stride(1) != 1: raise ValueError(f"{what}: fp32 rows")
-  rows, vocab = logits.shape
-
-  def vector(name, t, dtype):
-    if t is not None and (t.dtype != dtype or t.dim() != 1 or t.numel() != rows or (rows > 1 and t.stride(0) != 1)):
-      raise ValueError(f"{what}: {name} is {rows} contiguous {dtype}")
-
-  def matrix(name, t, dtype, cols=0):
-    if t is not None and (t.dtype != dtype or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < cols or (t.shape[1] > 1 and t.stride(1) != 1)):
-      raise ValueError(f"{what}: {name} is [{rows}][{cols or 'any'}] {dtype} with contiguous rows")
-    # (rows that overlap, as one row expanded to all of them: each its own)
-    return t.contiguous() if t is not None and rows > 1 and t.stride(0) < t.shape[1] else t
-
-  for name, t in (("lengths", lengths), ("prompt_lengths", prompt_lengths)): vector(name, t, torch.int32)
-  for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)): vector(name, t, torch.float32)
-  logits = matrix("logits", logits, torch.float32)
-  tokens, bias_ids, bias = matrix("tokens", tokens, torch.int32), matrix("bias_ids", bias_ids, torch.int32), matrix("bias", bias, torch.float32)
-  allowed = matrix("allowed", allowed, torch.int32, -(-vocab // 32))
-  if (bias is None) != (bias_ids is None) or (bias is not None and bias.shape != bias_ids.shape): raise ValueError(f"{what}: bias_ids and bias of one shape")
-  if bias is not None and bias.stride(0) != bias_ids.stride(0): bias, bias_ids = bias.contiguous(), bias_ids.contiguous()
+  if logits.dim() != 2 or logits.shape[0] < 1 or logits.shape[1] < 1: raise ValueError(f"{what}: fp32 rows")
+  rows, vocab = shape = logits.shape
+  one = (rows,)
+  logits, x, ldx, _ = _matrix(what, "logits", logits, rows, _F32)
+  tokens, tok, ldt, nt = _matrix(what, "tokens", tokens, rows, _I32)
+  if lengths is not None: _vector(what, "lengths", lengths, one)
+  if prompt_lengths is not None: _vector(what, "prompt_lengths", prompt_lengths, one)
+  if repetition is not None: _vector(what, "repetition", repetition, one, _F32)
+  if presence is not None: _vector(what, "presence", presence, one, _F32)
+  if frequency is not None: _vector(what, "frequency", frequency, one, _F32)
   if tokens is None and (lengths is not None or prompt_lengths is not None): raise ValueError(f"{what}: lengths without tokens")
-  if out is None: out = torch.empty(rows, vocab, dtype=torch.float32, device=logits.device)
-  if out.dtype != torch.float32 or out.shape != logits.shape or out.stride(1) != 1 or (rows > 1 and out.stride(0) < vocab):
-    raise ValueError(f"{what}: out is fp32 rows of logits' shape")
-  _here(what, logits.device, tokens, lengths, prompt_lengths, repetition, presence, frequency, bias_ids, bias, allowed, out)
-  nt, nb = (tokens.shape[1] if tokens is not None else 0), (bias.shape[1] if bias is not None else 0)
-  ld = lambda t: max(t.stride(0), t.shape[1]) if t is not None else 0  # (one row's stride may be anything)
-  lib.call("fh_logit_rules", _ptr(logits), ld(logits), rows, vocab, _ptr(tokens) if nt else None, ld(tokens), nt, _ptr(lengths) if nt else None,
-           _ptr(prompt_lengths) if nt else None, _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias_ids) if nb else None,
-           _ptr(bias) if nb else None, ld(bias), nb, _ptr(allowed), ld(allowed), _ptr(out), ld(out), _stream())
+  if (bias is None) != (bias_ids is None) or (bias is not None and bias.shape != bias_ids.shape): raise ValueError(f"{what}: bias_ids and bias of one shape")
+  bias_ids, bid, ldb, nb = _matrix(what, "bias_ids", bias_ids, rows, _I32)
+  bias, bv, ldv, _ = _matrix(what, "bias", bias, rows, _F32)
+  if ldb != ldv:
+    bias, bias_ids = bias.contiguous(), bias_ids.contiguous()
+    bid, bv, ldb = bias_ids.data_ptr(), bias.data_ptr(), nb
+  allowed, mask, ldm, _ = _matrix(what, "allowed", allowed, rows, _I32, (vocab + 31) // 32)
+  if out is None: out = torch.empty(rows, vocab, dtype=_F32, device=logits.device)
+  ldo, unit = out.stride()
+  if out.dtype is not _F32 or out.shape != shape or unit != 1 or (rows > 1 and ldo < vocab): raise ValueError(f"{what}: out is fp32 rows of logits' shape")
+  _here(what, logits, tokens, lengths, prompt_lengths, repetition, presence, frequency, bias_ids, bias, allowed, out)
+  lib.call("fh_logit_rules", x, ldx, rows, vocab, tok, ldt, nt, _ptr(lengths) if nt else None, _ptr(prompt_lengths) if nt else None, _ptr(repetition),
+           _ptr(presence), _ptr(frequency), bid, bv, ldb, nb, mask, ldm, out.data_ptr(), max(ldo, vocab), _stream())
   return out
 
 
