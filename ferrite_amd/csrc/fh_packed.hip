@@ -773,27 +773,36 @@ static int launch_seq(const char* fn, int head_dim, int cf, int pairs, int64_t b
   return check_launch(fn);
 }
 
-// Workgroups the keys of a tile are split among: enough that the grid has two a CU, each with 4 tiles of 64 keys or more, or
-// 8 of fewer keys where there are not so many, at most 32 (a wave joins the parts, a lane each)
-constexpr int SQ_CUS = 256, SQ_SPLIT_KEYS = 256, SQ_SHORT_KEYS = 64, SQ_MAX_SPLITS = 32;
-static int splits_for(int64_t groups, int64_t keys) {
-  if (groups >= SQ_CUS) return 1;
-  const int64_t s = (2 * SQ_CUS + groups - 1) / groups;
-  const int64_t most = std::max(keys / SQ_SPLIT_KEYS, std::min<int64_t>(8, keys / SQ_SHORT_KEYS));
-  return (int)std::max<int64_t>(1, std::min<int64_t>({s, most, SQ_MAX_SPLITS}));
+// Workgroups the keys of each of `groups` tiles are split among, at most 32 (a wave joins the parts, a lane each): the number
+// that takes the least time by what was measured. A workgroup alone on its CU takes a tile of 64 keys in about 1.2 us at 128
+// dimensions (8 times that in fp32), two a CU take them together in twice the time, so that more than one a CU gains nothing; a
+// second kernel costs 3 us, and each part of a pair is written and read at 4 TB/s (512 rows of 32 heads: 4 us a part). `others`:
+// workgroups beside them (a decode step's rows' own keys), of other_tiles each: free until the CUs are one each.
+constexpr int SQ_CUS = 256, SQ_MAX_SPLITS = 32;
+static int splits_for(int64_t groups, int64_t keys, int64_t pairs, int head_dim, int cf, double joined, int64_t others = 0, int64_t other_tiles = 0) {
+  const double tile = 1.2 * head_dim / 128 * (cf == FH_F32 ? 8 : 1), part = 8e-6 / 4 * pairs * (head_dim + 2);
+  const int64_t tiles = std::max<int64_t>(1, (keys + 63) / 64);
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= std::min<int64_t>(SQ_MAX_SPLITS, tiles); ++s) {
+    const double own = groups * s + others > SQ_CUS ? std::max(1.0, (double)others / SQ_CUS) * other_tiles : 0;
+    const double t = tile * (((tiles + s - 1) / s) * std::max(1.0, (double)groups * s / SQ_CUS) + own) + part * s + (s > 1 ? joined : 0);
+    if (s == 1 || t < least) { least = t; best = s; }
+  }
+  return best;
 }
 // Pairs a workgroup: 128, or 64 with two groups of waves on a tile's keys: for a decode step (one row a sequence) and prompts of
 // few rows. An fp32 cache's form has no second group.
 static int packed_pairs(int64_t rows, int n, int rep, int cf) { return cf != FH_F32 && rows * rep <= (int64_t)64 * n ? 64 : 128; }
 static int64_t packed_tiles(int64_t rows, int n, int rep, int pairs) { return rows * rep / pairs + std::min<int64_t>(n, rows); }
-static int packed_splits(int64_t rows, int n, int heads, int kv_heads, int64_t max_context) {
-  return splits_for(packed_tiles(rows, n, heads / kv_heads, 128) * kv_heads, max_context);
+static int packed_splits(int64_t rows, int n, int heads, int kv_heads, int head_dim, int cf, int64_t max_context) {
+  return splits_for(packed_tiles(rows, n, heads / kv_heads, 128) * kv_heads, max_context, rows * heads, head_dim, cf, 3);
 }
-static void shared_splits(int batch, int heads, int kv_heads, int cf, int64_t max_prefix, int64_t max_own, int& tiles, int& prefix, int& own) {
+static void shared_splits(int batch, int heads, int kv_heads, int head_dim, int cf, int64_t max_prefix, int64_t max_own, int& tiles, int& prefix, int& own) {
   const int pairs = cf == FH_F32 ? 128 : 64;
   tiles = (int)(((int64_t)batch * (heads / kv_heads) + pairs - 1) / pairs);
-  prefix = splits_for((int64_t)tiles * kv_heads, max_prefix);
-  own = splits_for((int64_t)batch * kv_heads * 2, max_own);  // (the prefix has the other half of the GPU)
+  prefix = splits_for((int64_t)tiles * kv_heads, max_prefix, (int64_t)batch * heads, head_dim, cf, 0, (int64_t)batch * kv_heads, (max_own + 127) / 128);
+  own = splits_for((int64_t)batch * kv_heads * 2, max_own, (int64_t)batch * heads, head_dim, cf, 0);  // (the prefix has the other half of the GPU)
 }
 
 // what both entry points ask of their operands (fn: the name in the message)
@@ -822,7 +831,7 @@ using namespace fh;
 extern "C" size_t fh_attention_packed_workspace_bytes(int64_t rows, int sequences, int heads, int kv_heads, int head_dim,
                                                       int64_t max_context) {
   if (rows < 1 || sequences < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || max_context < 1) return 0;
-  const int s = packed_splits(rows, sequences, heads, kv_heads, max_context);
+  const int s = std::max(packed_splits(rows, sequences, heads, kv_heads, head_dim, FH_BF16, max_context), packed_splits(rows, sequences, heads, kv_heads, head_dim, FH_F32, max_context));
   return s == 1 ? 0 : (size_t)rows * heads * s * (head_dim + 2) * sizeof(float);
 }
 
@@ -846,7 +855,7 @@ extern "C" int fh_attention_prefill_packed(const void* q, int q_dtype, int64_t l
   a.rep = heads / kv_heads;
   a.cache_exps = (const uint8_t*)cache + kv_exps_at(cache_dtype, kv_heads, cache_len, head_dim);
   a.scale = 1.0f / sqrtf((float)head_dim);
-  a.splits = a.parts = packed_splits(rows, sequences, heads, kv_heads, max_context);
+  a.splits = a.parts = packed_splits(rows, sequences, heads, kv_heads, head_dim, cache_dtype, max_context);
   a.part = (float*)workspace;
   if (a.parts > 1 && (!workspace || ws_bytes < fh_attention_packed_workspace_bytes(rows, sequences, heads, kv_heads, head_dim, max_context) || ((uintptr_t)workspace & 15)))
     return fail(FH_EINVAL, "fh_attention_prefill_packed: a 16-byte aligned workspace of fh_attention_packed_workspace_bytes");
@@ -857,9 +866,10 @@ extern "C" int fh_attention_prefill_packed(const void* q, int q_dtype, int64_t l
 extern "C" size_t fh_attention_shared_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int64_t max_prefix,
                                                       int64_t max_own) {
   if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || max_prefix < 0 || max_own < 0) return 0;
-  int tiles, prefix, own;
-  shared_splits(batch, heads, kv_heads, FH_F32, max_prefix, max_own, tiles, prefix, own);  // (the most splits of any cache)
-  return (size_t)batch * heads * (prefix + own) * (head_dim + 2) * sizeof(float);
+  int tiles, prefix, own, tiles32, prefix32, own32;  // (the most of any cache)
+  shared_splits(batch, heads, kv_heads, head_dim, FH_BF16, max_prefix, max_own, tiles, prefix, own);
+  shared_splits(batch, heads, kv_heads, head_dim, FH_F32, max_prefix, max_own, tiles32, prefix32, own32);
+  return (size_t)batch * heads * std::max(prefix + own, prefix32 + own32) * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int fh_attention_decode_shared(const void* q, int q_dtype, const void* cache, int cache_dtype, int64_t cache_len,
@@ -883,7 +893,7 @@ extern "C" int fh_attention_decode_shared(const void* q, int q_dtype, const void
   a.rep = heads / kv_heads;
   a.cache_exps = (const uint8_t*)cache + kv_exps_at(cache_dtype, kv_heads, cache_len, head_dim);
   a.scale = 1.0f / sqrtf((float)head_dim);
-  shared_splits(batch, heads, kv_heads, cache_dtype, max_prefix, max_own, a.tiles, a.splits, a.own_splits);
+  shared_splits(batch, heads, kv_heads, head_dim, cache_dtype, max_prefix, max_own, a.tiles, a.splits, a.own_splits);
   a.parts = a.splits + a.own_splits;
   a.part = (float*)workspace;
   if (!workspace || ws_bytes < fh_attention_shared_workspace_bytes(batch, heads, kv_heads, head_dim, max_prefix, max_own) || ((uintptr_t)workspace & 15))
