@@ -95,12 +95,14 @@ __device__ inline bool seq_item(const SeqArgs& a, SeqItem& it) {
       it.place0 = 0; it.step = -1;
       return true;
     }
-    blk -= a.tiles * a.splits;       // a row's own keys
-    const int64_t b = blk / a.own_splits;
+    blk -= a.tiles * a.splits;       // a row's own keys: the tiles of its pairs (one, but for more heads a key head than pairs a tile)
     it.split = blk % a.own_splits; it.splits = a.own_splits; it.part = a.splits + it.split;
+    const int row_tiles = (a.rep + BQ - 1) / BQ;
+    const int64_t b = blk / a.own_splits / row_tiles;
+    it.pair0 = blk / a.own_splits % row_tiles * BQ;
     int sh, pre, own;
     row_counts(a, b, sh, pre, own);
-    it.row0 = b; it.pair0 = 0; it.pairs = a.rep;
+    it.row0 = b; it.pairs = a.rep;
     it.prefix = 0; it.own = a.first_row[b]; it.shared = 0;
     it.place0 = own - 1; it.step = 0;
     return true;
@@ -781,7 +783,7 @@ static int launch_seq(const char* fn, int head_dim, int cf, int pairs, int64_t b
 constexpr int SQ_CUS = 256, SQ_MAX_SPLITS = 32;
 static int splits_for(int64_t groups, int64_t keys, int64_t pairs, int head_dim, int cf, double joined, int64_t others = 0, int64_t other_tiles = 0) {
   const double tile = 1.2 * head_dim / 128 * (cf == FH_F32 ? 8 : 1), part = 8e-6 / 4 * pairs * (head_dim + 2);
-  const int64_t tiles = std::max<int64_t>(1, (keys + 63) / 64);
+  const int64_t tiles = std::max<int64_t>(1, (std::min<int64_t>(keys, 1LL << 40) + 63) / 64);
   int best = 1;
   double least = 0;
   for (int s = 1; s <= std::min<int64_t>(SQ_MAX_SPLITS, tiles); ++s) {
@@ -798,8 +800,9 @@ static int64_t packed_tiles(int64_t rows, int n, int rep, int pairs) { return ro
 static int packed_splits(int64_t rows, int n, int heads, int kv_heads, int head_dim, int cf, int64_t max_context) {
   return splits_for(packed_tiles(rows, n, heads / kv_heads, 128) * kv_heads, max_context, rows * heads, head_dim, cf, 3);
 }
+static int shared_pairs(int cf) { return cf == FH_F32 ? 128 : 64; }
 static void shared_splits(int batch, int heads, int kv_heads, int head_dim, int cf, int64_t max_prefix, int64_t max_own, int& tiles, int& prefix, int& own) {
-  const int pairs = cf == FH_F32 ? 128 : 64;
+  const int pairs = shared_pairs(cf);
   tiles = (int)(((int64_t)batch * (heads / kv_heads) + pairs - 1) / pairs);
   prefix = splits_for((int64_t)tiles * kv_heads, max_prefix, (int64_t)batch * heads, head_dim, cf, 0, (int64_t)batch * kv_heads, (max_own + 127) / 128);
   own = splits_for((int64_t)batch * kv_heads * 2, max_own, (int64_t)batch * heads, head_dim, cf, 0);  // (the prefix has the other half of the GPU)
@@ -815,7 +818,7 @@ static int seq_check(const char* fn, const SeqArgs& a, int q_dtype, int cache_dt
   if (q_dtype != FH_F32 && q_dtype != FH_BF16) return no(FH_EINVAL, "q is FH_F32 or FH_BF16");
   if (cache_dtype < FH_F32 || cache_dtype > FH_BFP4) return no(FH_EUNSUP, "cache is FH_F32, FH_BF16, FH_BFP8 or FH_BFP4");
   if (a.cache_len < 1) return no(FH_EINVAL, "cache_len at least 1");
-  if (a.rows * (a.heads / a.kv_heads) >= (1LL << 31) || a.cache_len >= (1LL << 31)) return no(FH_EUNSUP, "fewer than 2^31 cache rows and pairs of a row and a key head's heads");
+  if (a.rows * (a.heads / a.kv_heads) >= (1LL << 30) || a.cache_len >= (1LL << 30)) return no(FH_EUNSUP, "fewer than 2^30 cache rows and pairs of a row and a key head's heads");
   if ((a.shared == nullptr) != (a.prefix_row == nullptr)) return no(FH_EINVAL, "prefix_row and shared go together");
   const int64_t cols = (int64_t)a.heads * head_dim;
   if (a.ldq < cols || a.ldo < cols || a.ldq % (q_dtype == FH_F32 ? 4 : 8) || (o_dtype != FH_BF16_T16 && a.ldo % 4) ||
@@ -846,7 +849,8 @@ extern "C" int fh_attention_prefill_packed(const void* q, int q_dtype, int64_t l
   a.q = q; a.q_bf16 = q_dtype == FH_BF16; a.ldq = ldq; a.cache = cache; a.cache_len = cache_len;
   a.heads = heads; a.kv_heads = kv_heads; a.rows = rows; a.n = sequences;
   a.starts = starts; a.places = p0; a.first_row = first_row; a.prefix_row = prefix_row; a.shared = shared;
-  a.max_prefix = max_context; a.max_own = max_context; a.o = o; a.o_bf16 = o_dtype == FH_BF16; a.ldo = ldo;
+  a.max_prefix = cache_len; a.max_own = std::min(max_context, 2 * cache_len);  // (no more than a prefix and a slot hold)
+  a.o = o; a.o_bf16 = o_dtype == FH_BF16; a.ldo = ldo;
   if (!starts) return fail(FH_EINVAL, "fh_attention_prefill_packed: null pointer");
   if (rows < 1 || rows >= (1LL << 31) || sequences < 1 || max_context < 1)
     return fail(FH_EINVAL, "fh_attention_prefill_packed: need 1 <= rows < 2^31, sequences >= 1 and max_context >= 1");
@@ -882,7 +886,7 @@ extern "C" int fh_attention_decode_shared(const void* q, int q_dtype, const void
   a.q = q; a.q_bf16 = q_dtype == FH_BF16; a.ldq = (int64_t)heads * head_dim; a.cache = cache; a.cache_len = cache_len;
   a.heads = heads; a.kv_heads = kv_heads; a.rows = batch; a.n = batch;
   a.places = places; a.first_row = first_row; a.prefix_row = prefix_row; a.shared = shared;
-  a.max_prefix = max_prefix; a.max_own = max_own;
+  a.max_prefix = std::min(max_prefix, cache_len); a.max_own = std::min(max_own, cache_len);
   a.o = o; a.o_bf16 = o_dtype != FH_F32; a.o_tiles = o_dtype == FH_BF16_T16; a.ldo = a.ldq;
   if (!prefix_row || !shared) return fail(FH_EINVAL, "fh_attention_decode_shared: null pointer");
   if (batch < 1 || max_prefix < 0 || max_own < 0)
@@ -898,5 +902,6 @@ extern "C" int fh_attention_decode_shared(const void* q, int q_dtype, const void
   a.part = (float*)workspace;
   if (!workspace || ws_bytes < fh_attention_shared_workspace_bytes(batch, heads, kv_heads, head_dim, max_prefix, max_own) || ((uintptr_t)workspace & 15))
     return fail(FH_EINVAL, "fh_attention_decode_shared: a 16-byte aligned workspace of fh_attention_shared_workspace_bytes");
-  return launch_seq(fn, head_dim, cache_dtype, 64, ((int64_t)a.tiles * a.splits + (int64_t)batch * a.own_splits) * kv_heads, as_stream(stream), a);
+  const int pairs = shared_pairs(cache_dtype), row_tiles = (a.rep + pairs - 1) / pairs;
+  return launch_seq(fn, head_dim, cache_dtype, 64, ((int64_t)a.tiles * a.splits + (int64_t)batch * row_tiles * a.own_splits) * kv_heads, as_stream(stream), a);
 }

@@ -191,8 +191,8 @@ __global__ __launch_bounds__(512) void rules_kernel(RuleArgs a) {
 
 template <int CB, bool VEC>
 static void launch_rules(dim3 g, int threads, size_t lds, hipStream_t s, const RuleArgs& a) {
-  static const hipError_t allowed = hipFuncSetAttribute((const void*)rules_kernel<CB, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
-  (void)allowed;  // (a refusal shows as the launch's error)
+  if (lds > 65536)  // (on the current device, whichever it is; a refusal shows as the launch's error)
+    (void)hipFuncSetAttribute((const void*)rules_kernel<CB, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
   hipLaunchKernelGGL((rules_kernel<CB, VEC>), g, dim3(threads), lds, s, a);
 }
 
@@ -209,7 +209,8 @@ extern "C" int fh_logit_rules(const float* logits, int64_t ldl, int64_t rows, in
   if (rows < 1 || vocab < 1 || ldl < vocab || ldo < vocab) return fail(FH_EINVAL, "fh_logit_rules: need rows, vocab >= 1, ldl and ldo >= vocab");
   if (rows > 65535 || vocab > (1LL << 31) - 1) return fail(FH_EUNSUP, "fh_logit_rules: at most 65535 rows and 2^31 - 1 columns");
   if (out == logits && ldo != ldl) return fail(FH_EINVAL, "fh_logit_rules: in place, ldo is ldl");
-  if (tokens ? max_tokens < 0 || ldt < max_tokens || max_tokens > (1LL << 31) - 1 : lengths || prompt_lengths)
+  if (tokens && max_tokens >= (1LL << 30)) return fail(FH_EUNSUP, "fh_logit_rules: fewer than 2^30 tokens a row");
+  if (tokens ? max_tokens < 0 || ldt < max_tokens : lengths || prompt_lengths)
     return fail(FH_EINVAL, "fh_logit_rules: tokens' rows at least max_tokens apart, lengths only with tokens");
   if ((bias_ids == nullptr) != (bias == nullptr) || (bias_ids && (biases < 0 || ldb < biases)))
     return fail(FH_EINVAL, "fh_logit_rules: bias_ids and bias go together, rows at least biases apart");
@@ -220,12 +221,13 @@ extern "C" int fh_logit_rules(const float* logits, int64_t ldl, int64_t rows, in
   a.lengths = lengths; a.prompts = prompt_lengths; a.repetition = repetition; a.presence = presence; a.frequency = frequency;
   a.bias_ids = bias_ids; a.bias = bias; a.ldb = ldb; a.nbias = bias_ids ? (int)biases : 0;
   a.allowed = (const uint32_t*)allowed; a.ldm = ldm; a.out = out; a.ldo = ldo;
-  // parts: two workgroups a CU of 256, at least 1024 columns, at most 64 KB of cells. Threads by the part: 64 columns each, 256 to
-  // 512 (128 rows of 128256 with tokens, 300 biases and a mask: 41 us; 256 threads 47, 1024 46, parts of 16384 42 to 50)
+  // Parts: two workgroups a CU of 256 share the columns in whole 1024s, at most 64 KB of cells (with the biases more than a
+  // launch may have unasked: launch_rules asks). Threads by the part: 64 columns each, 256 to 512 (128 rows of 128256 with
+  // tokens, 300 biases and a mask, in parts of 32768: 40 us; 256 threads 47, 1024 46; parts of 16384 42 to 50, of 26624 50).
   const bool wide = a.tokens && max_tokens >= 16384;
   const int64_t most = wide ? 16384 : 32768, even = (vocab * rows / 512 + 1023) / 1024 * 1024;
   a.part = (int)std::min(most, std::max<int64_t>(1024, even));
-  const int threads = std::min(512, std::max(256, a.part / 64));
+  const int threads = std::min(512, std::max(256, (a.part / 64 + 63) / 64 * 64));
   const size_t lds = (a.tokens || a.nbias ? (size_t)a.part * (wide ? 4 : 2) : 0) + (a.nbias ? (size_t)(a.nbias + 3) / 4 * 48 + RHASH * 4 : 0);
   const bool vec = vocab % 4 == 0 && ldl % 4 == 0 && ldo % 4 == 0 && !((uintptr_t)logits & 15) && !((uintptr_t)out & 15);
   const dim3 g((unsigned)((vocab + a.part - 1) / a.part), (unsigned)rows);

@@ -134,6 +134,51 @@ def test_packed_ignores_rows_outside_the_cache(cuda):
   assert torch.isfinite(o).all()
 
 
+def test_packed_many_sequences(cuda):
+  # more sequences than a wave's lanes look through at once, some of them empty, the last round of them not full
+  rng = np.random.default_rng(21)
+  for n in (64, 65, 150):
+    lens = [int(i) for i in rng.integers(0, 9, n)]
+    lens[-1], lens[63] = 5, 0
+    got, want, tol = packed(22 + n, 2, 1, 64, lens, [int(i) for i in rng.integers(0, 70, n)], 33, pad=3)
+    S.check(got, want, tol, n)
+
+
+def test_many_heads_of_a_key_head(cuda):
+  # more query heads a key head than a wave has pairs, and than a workgroup
+  for heads in (40, 200):
+    got, want, tol = packed(23, heads, 1, 64, [3, 1], [5, 66], 20)
+    S.check(got, want, tol, heads)
+    got, want, tol = shared(24, heads, 1, 64, 3, 150, 70)
+    S.check(got, want, tol, heads)
+
+
+def test_bounds_past_the_cache(cuda):
+  # places and bounds far past the cache: no more keys are read than a prefix and a slot could hold
+  rng = np.random.default_rng(25)
+  cache, _ = S.cache(rng, 2, 40, 64, "bf16")
+  q = torch.from_numpy(rng.normal(0, 1, (6, 128)).astype(np.float32)).cuda()
+  o = ops().attention_prefill_packed(q, cache, 2, 1, 64, ints([0, 6]), ints([1 << 30]), ints([0]), 1 << 40)
+  assert torch.isfinite(o).all()
+  o = ops().attention_decode_shared(q, cache, 2, 1, 64, ints([1 << 30] * 6), ints([3] * 6), ints([0]), ints([1 << 30] * 6), 1 << 40, 1 << 40)
+  assert torch.isfinite(o).all()
+
+
+def test_two_calls_at_once(cuda):
+  # the same call on two streams at a time, each with a workspace of its own
+  rng = np.random.default_rng(26)
+  cache, _ = S.cache(rng, 4, 3000, 64, "bf16")
+  q = torch.from_numpy(rng.normal(0, 1, (8, 256)).astype(np.float32)).cuda()
+  args = (q, cache, 4, 2, 64, ints([2500] * 8), ints([2600 + 20 * i for i in range(8)]), ints([0]), ints([2490] * 8), 2490, 20)
+  want = ops().attention_decode_shared(*args)
+  torch.cuda.synchronize()
+  streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+  for i in range(10):
+    with torch.cuda.stream(streams[i % 2]): outs.append(ops().attention_decode_shared(*args))
+  torch.cuda.synchronize()
+  assert all(torch.equal(o, want) for o in outs)
+
+
 def shared(seed, heads, kv, hd, batch, prefix, own, fmt="bf16", q="fp32", o="bf16", some=False, tiles=False, max_more=0):
   """A decode call behind a prefix and its oracle: (o, want, tol)."""
   rng = np.random.default_rng(seed)

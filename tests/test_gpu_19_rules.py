@@ -150,3 +150,23 @@ def test_repeats_and_graph(cuda):
     assert torch.equal(out, eager[i]), i
     run(*cases[(i + 1) % 3])
     torch.cuda.synchronize()
+
+
+def test_large_batch_captured(cuda):
+  # the widest parts (more LDS than a launch has unasked), from a graph, against the eager call
+  x, c = case(10, 128, 128256, 40, 1024, False)
+  dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()
+  X, held = dev(x), {k: dev(v) for k, v in c.items() if v is not None}
+  args = dict(tokens=held["tokens"], lengths=held["lengths"], prompt_lengths=held["prompts"], repetition=held["rep"], presence=held["pre"],
+              frequency=held["fre"], bias_ids=held["ids"], bias=held["bias"])
+  eager = ops().logit_rules(X, **args)
+  rows = [0, 1, 77, 127]
+  check(eager[rows], *oracle(x[rows], **{k: v[rows] for k, v in c.items() if v is not None}))
+  out = torch.zeros_like(X)
+  torch.cuda.synchronize()
+  g = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(g): ops().logit_rules(X, out=out, **args)
+  for _ in range(2):
+    out.zero_()
+    g.replay()
+    assert torch.equal(out, eager)

@@ -34,7 +34,7 @@ def rules(**kw):
   (dict(heads=7), ValueError), (dict(hd=96), NotImplementedError), (dict(hd=256, ldq=2048, ldo=2048), NotImplementedError), (dict(qd=lib.BFP8), ValueError), (dict(cd=lib.I32), NotImplementedError),
   (dict(od=lib.BF16_T16), ValueError), (dict(ldq=510), ValueError), (dict(ldq=256), ValueError), (dict(ldo=500), ValueError), (dict(q=P + 4), ValueError),
   (dict(cache=P + 8), ValueError), (dict(o=P + 4), ValueError), (dict(ctx=0), ValueError), (dict(shared=P), ValueError), (dict(prefix=P), ValueError),
-  (dict(len=0), ValueError), (dict(rows=1 << 31), ValueError)])
+  (dict(len=0), ValueError), (dict(rows=1 << 31), ValueError), (dict(len=1 << 30), NotImplementedError), (dict(rows=1 << 29), NotImplementedError)])
 def test_packed_refuses(kw, err):
   lib.load()
   with pytest.raises(err, match="fh_attention_prefill_packed"): packed(**kw)
@@ -55,7 +55,7 @@ def test_shared_refuses(kw, err):
   (dict(x=None), ValueError), (dict(out=None), ValueError), (dict(rows=0), ValueError), (dict(ldl=63), ValueError), (dict(ldo=63), ValueError),
   (dict(out=P, ldo=65), ValueError), (dict(lengths=P), ValueError), (dict(tokens=P, ldt=3, most=4), ValueError), (dict(ids=P), ValueError),
   (dict(ids=P, bias=P, ldb=4, nb=5), ValueError), (dict(ids=P, bias=P, ldb=2000, nb=1025), NotImplementedError), (dict(allowed=P, ldm=1), ValueError),
-  (dict(rows=65536), NotImplementedError)])
+  (dict(rows=65536), NotImplementedError), (dict(tokens=P, ldt=1 << 30, most=1 << 30), NotImplementedError)])
 def test_rules_refuse(kw, err):
   lib.load()
   with pytest.raises(err, match="fh_logit_rules"): rules(**kw)
