@@ -3,24 +3,33 @@
 // prefix_row + p where p < shared (rows that other sequences read too) and at first_row + p - shared behind them, and a
 // query at place p sees places 0 .. p: o = sum_k softmax_k(q k / sqrt(hd)) v. A query that sees no place gives zeros.
 //
-// The query heads of a key head read the same keys, so a workgroup takes rows of pairs (query row, head of the group): 32 a
-// wave, 4 waves, one key head; a prompt of 20 rows of 4 heads a key head is one tile of 80 pairs, and a decode step's rows
-// behind one prefix are 32 pairs to 8 rows. It walks the keys its pairs see in tiles staged in LDS, the next tile's loads in
-// flight meanwhile. Scores transposed, S^T = K Q^T, keys down and pairs across: a lane holds one pair's scores, so the
-// softmax's statistics need one exchange between the wave's halves; and P^T is the next product's operand as it lies, O^T +=
-// V^T P^T. The running max of a softmax moves only when a tile's lies more than 2^8 above it: exponents up to 256 lose
-// nothing in fp32 sums or bf16 products, and the output is rescaled a few times a row rather than every tile.
+// The query heads of a key head read the same keys, so a workgroup of 4 waves takes pairs (query row, head of the group) of one
+// key head, 32 a wave: a prompt of 20 rows of 4 heads a key head is one tile of 80 pairs, and 8 rows of a decode step behind one
+// prefix are 32. 128 pairs a workgroup, or 64 with the tile's keys shared by two groups of waves (a decode step, prompts of few
+// rows: what those wait for is a wave's chain of products). It walks the keys its pairs see in tiles of 64 staged in LDS, the
+// next tile's loads in flight meanwhile. Scores transposed, S^T = K Q^T, keys down and pairs across: a lane holds one pair's
+// scores, so the softmax's statistics need one exchange between the wave's halves; and P^T is the next product's operand as it
+// lies, O^T += V^T P^T. The running max moves only when a tile's lies more than 2^8 above it: weights up to 256 lose nothing in
+// fp32 sums or bf16 products, and the output is rescaled a few times a row rather than every tile.
 //
-// Two forms. A bf16 or block-float cache (whose values are bf16) and bf16 output: v_mfma_f32_32x32x16_bf16, an fp32 q as two bf16 terms (off by
-// 2^-16 of itself at most; a bf16 q is exact in one), the softmax's weights rounded to bf16 (2^-8 at most, what the output's
-// own rounding adds; their sum is taken before it). With fp32 output q and the weights go in as three terms, off by 2^-24 at
-// most. An fp32 cache takes v_mfma_f32_32x32x2_f32, nothing rounded.
+// The arithmetic goes by the types. A bf16 or block-float cache (whose values are bf16) takes v_mfma_f32_32x32x16_bf16: for bf16
+// output an fp32 q goes in as two bf16 terms (off by 2^-16 of itself at most; a bf16 q is exact in one) and the softmax's
+// weights rounded to bf16 (2^-8 at most, what the output's own rounding adds; their sum is taken before it); for fp32 output q
+// and the weights as three terms, off by 2^-24 at most. An fp32 cache takes v_mfma_f32_32x32x2_f32, nothing rounded.
 //
-// Where tiles are few, the keys are split among workgroups, each leaving its weighted sum, max and sum of weights in the
-// workspace, and a second kernel joins them; a shared prefix is always one of two parts or more, the rows' own keys others.
+// Where tiles are few, the keys are split among workgroups (splits_for), each leaving its weighted sum, max and sum of weights
+// in the workspace, and a second kernel joins them; a shared prefix's keys and a row's own are always parts of their own. Joining
+// in the last workgroup instead would need a release at device scope, which costs more here than the second launch.
 //
 // A key that a pair does not see has the weight 0, but 0 times an infinite or NaN value is NaN: a wave whose result is not
 // finite takes its pairs again one at a time over the keys each sees alone (attend_again).
+//
+// What bounds it (32 heads of 128, 8 key heads, on one MI355X): four prompts of up to 4096 tokens, bf16 q, 331-347 us, 870-920
+// TFLOP/s of the products its rows need (the library's 8192^3 product reaches 1200): the matrix cores are busy 43% of the cycles
+// at the 1.8 GHz the chip holds under this load, the softmax's exponentials and conversions about as long, and moving reads
+// ahead, wave priorities or addresses out of the loop changed nothing. 16 prompts of up to 400 tokens, fp32 q (twice the scores'
+// products): 50 us for 122 MB; a workgroup's few tiles do not hide its start and end. 64 rows behind a prefix of 16384, each
+// with up to 700 rows of its own: 54 us and 5 for the join; 16 rows behind 4096: 14 and 5, a chain of launches and latencies.
 #include <math.h>
 #include <algorithm>
 #include <type_traits>
@@ -691,7 +700,8 @@ __global__ __launch_bounds__(64 * SQ_NW, 2) void seq_f32_kernel(SeqArgs a) {
   seq_finish<HD, CF>(a, it, wpair, limit, t0 * BK, min(t1 * BK, keys), acc, m, l);
 }
 
-// A pair's parts joined, a wave a pair: lane p holds part p's statistics, then a lane HD / 64 dimensions of each part's sum,
+// A pair's parts joined, a wave a pair (2048 pairs of 9 parts: 5 us; the parts stored as the products leave them in registers,
+// whole lines a store, and joined 8 dimensions a wave: 7 to 10 us, fewer waves each with a longer chain): lane p holds part p's statistics, then a lane HD / 64 dimensions of each part's sum,
 // times 2^(its max - the largest). A part that saw no key (its max -inf) has no weight; a pair with none gives zeros. Parts
 // of rows that are no sequence's were never written and are not read.
 template <int HD>

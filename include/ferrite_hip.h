@@ -272,13 +272,17 @@ int fh_attention_prefill(const float* q, int64_t ldq, const void* cache, int cac
  * FH_F32 or FH_BF16, the cache any of fh_kv_cache_bytes' formats, head_dim 64 or 128; query head h reads kv head
  * h / (heads / kv_heads). q's rows and the cache are 16-byte aligned, o's rows aligned to 4 values. Rows and cache values
  * that a query does not see have no part in its result, NaN and infinities included. A workspace (16-byte aligned) as
- * everywhere: no clearing, no state, not shared by calls that overlap. No counterpart in the reference, whose prompts are
- * prefilled one at a time (models/llama.py:498-504) and whose rows each read their own slot (models/llama.py:429-452). */
+ * everywhere: no clearing, no state, not shared by calls that overlap. Scores, softmax and sums are fp32. Products of a
+ * bf16 or block-float cache run on the matrix cores in bf16 terms: for bf16 output an fp32 q in two (2^-16 of itself), the
+ * softmax weights in one (2^-8, the output's own rounding); for fp32 output both in three (2^-24). An fp32 cache's run in
+ * fp32. A call repeats its bits; a call of other sizes may add a row's keys in other parts. No counterpart in the
+ * reference, whose prompts are prefilled one at a time (models/llama.py:498-504) and whose rows each read their own slot
+ * (models/llama.py:429-452). */
 
 /* The causal attention of packed prompts: rows starts[s] .. starts[s + 1] - 1 of q [rows][ldq] are sequence s's, at places
  * p0[s], p0[s] + 1, ..., their keys and values already in the cache; starts [sequences + 1] does not decrease (a sequence
- * may have no rows), and rows of o before starts[0] or from starts[sequences] on are left as they were. max_context: a bound of every
- * place + 1 (keys past it are not read). */
+ * may have no rows), and rows of o before starts[0] or from starts[sequences] on are left as they were. max_context: a
+ * bound of every place + 1 (keys past it are not read). */
 size_t fh_attention_packed_workspace_bytes(int64_t rows, int sequences, int heads, int kv_heads, int head_dim,
                                            int64_t max_context);
 int fh_attention_prefill_packed(const void* q, int q_dtype, int64_t ldq, const void* cache, int cache_dtype, int64_t cache_len,
