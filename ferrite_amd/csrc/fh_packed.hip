@@ -477,10 +477,9 @@ __global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf
 
   constexpr int NP = BK * HD / 8 / (64 * SQ_NW);  // pieces of 8 a thread
   SeqRaw kraw[ASYNC ? 1 : NP], vraw[ASYNC ? 1 : NP];
-  // a thread's pieces of a tile: rows pr + PR j, unit pu of each; where they lie from the tile's first row on
-  constexpr int PR = 64 * SQ_NW / (HD / 8);
+  // a thread's pieces of a tile: rows pr + PSTEP j, unit pu of each (a wave's loads into LDS in order: its rows lie together)
+  constexpr int PSTEP = (ASYNC ? 64 : 64 * SQ_NW) / (HD / 8);
   const int pr = ASYNC ? (64 * NP * wave + lane) / (HD / 8) : tid / (HD / 8), pu = lane % (HD / 8);
-  constexpr int PSTEP = ASYNC ? 64 / (HD / 8) : PR;  // (a wave's instructions in order: its rows lie together)
   auto load = [&](int t, int b) {  // tile t's loads: into buffer b, or into registers
     const int k0 = t * BK;
     // the tile's rows run on from its first, as they are, unless the keys end or the prefix ends in it, or it leaves the cache
@@ -550,13 +549,13 @@ __global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf
       for (int r = 0; r < 16; ++r) s[0][r] += s[1][r];
     } else {
 #pragma unroll
-    for (int st = 0; st < HD / 16; ++st)
+      for (int st = 0; st < HD / 16; ++st)
 #pragma unroll
-      for (int kb = 0; kb < NB; ++kb) {
-        const bf16x8 kf = *(const bf16x8*)(K + (32 * kb + ql) * KLD + 8 * ((2 * st + hh) ^ Tile::kswap(ql)));
+        for (int kb = 0; kb < NB; ++kb) {
+          const bf16x8 kf = *(const bf16x8*)(K + (32 * kb + ql) * KLD + 8 * ((2 * st + hh) ^ Tile::kswap(ql)));
 #pragma unroll
-        for (int u = 0; u < QT; ++u) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st][u], s[kb], 0, 0, 0);
-      }
+          for (int u = 0; u < QT; ++u) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st][u], s[kb], 0, 0, 0);
+        }
     }
     seq_softmax<HD, NB>(s, k0 + 32 * kb0, limit, wave_min, hh, scale2, m, l, acc);
     // O^T += V^T P^T, 16 keys a step: the lane's weights 8 j .. 8 j + 7 of block kb are keys 32 kb + 16 j + {4 hh .. 4 hh + 3,
@@ -700,10 +699,11 @@ __global__ __launch_bounds__(64 * SQ_NW, 2) void seq_f32_kernel(SeqArgs a) {
   seq_finish<HD, CF>(a, it, wpair, limit, t0 * BK, min(t1 * BK, keys), acc, m, l);
 }
 
-// A pair's parts joined, a wave a pair (2048 pairs of 9 parts: 5 us; the parts stored as the products leave them in registers,
-// whole lines a store, and joined 8 dimensions a wave: 7 to 10 us, fewer waves each with a longer chain): lane p holds part p's statistics, then a lane HD / 64 dimensions of each part's sum,
+// A pair's parts joined, a wave a pair: lane p holds part p's statistics, then a lane HD / 64 dimensions of each part's sum,
 // times 2^(its max - the largest). A part that saw no key (its max -inf) has no weight; a pair with none gives zeros. Parts
-// of rows that are no sequence's were never written and are not read.
+// of rows that are no sequence's were never written and are not read. 2048 pairs of 9 parts: 5 us; with the parts stored as
+// the products leave them in registers, whole lines a store, and joined 8 dimensions of 32 pairs a wave, 7 to 10: fewer waves,
+// each with a longer chain.
 template <int HD>
 __global__ __launch_bounds__(256) void seq_join(SeqArgs a) {
   const int lane = threadIdx.x & 63;

@@ -177,6 +177,7 @@ class Decoder:
     self.prefix_row, self.shared = (torch.zeros(n, dtype=torch.int32, device=self.device) for n in (1, B))
     self.top = 0  # the largest place of the rows set (set_rows), which advance raises,
     self.top_own = 0  # and the largest behind the prefix: the row of its slot
+    self.placed = True  # (False from a change of the sharing until the rows are set again)
 
   def weight_bytes(self):
     """Bytes of the weights one decode step reads: every matrix, a row of the embedding, the norms."""
@@ -206,6 +207,7 @@ class Decoder:
     ops.put_i32([(slot or 0) * self.part], self.prefix_row)
     self.ws_shared = ops.attention_shared_workspace(self.batch, self.c.heads, self.c.kv, self.hd, length, self.context, self.device) if slot is not None else None
     self.graph = None  # (the step is captured again)
+    self.placed = False
 
   def _attend(self, l, out):
     """A step's attention over block l's cache."""
@@ -237,6 +239,7 @@ class Decoder:
     if (s < 0).any() or (s >= self.slots).any(): raise ValueError(f"a slot outside 0..{self.slots - 1}")
     if self.prefix_slot is not None and (s == self.prefix_slot).any(): raise ValueError(f"slot {self.prefix_slot} holds the shared prefix")
     self.top, self.top_own = int(p.max()), int((p - sh).max())  # (kept on the host for advance's check)
+    self.placed = True
     if host:
       first = s * np.int32(self.part)
       v = [p, first, first + p - sh]
@@ -422,6 +425,7 @@ class Decoder:
     """One step: the logits (fp32, [batch][vocab]) and picks for tokens ids at places. With replay, the step runs as
     a HIP graph captured on the first call (every later step launches the same kernels: places are data)."""
     if ids is not None or places is not None: self._put(ids, places, slots)
+    if not self.placed: raise ValueError("step: the rows' places are to be set again after share_prefix")
     if not replay:
       self._step()
     else:

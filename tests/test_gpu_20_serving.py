@@ -142,6 +142,7 @@ def test_refusals(cuda):
   with pytest.raises(ValueError): dec.prefill_batch([[1]], shared=[3])
   dec.prefill([1, 2, 3], slot=2)
   dec.share_prefix(2, 3)
+  with pytest.raises(ValueError): dec.step()                       # (the rows' places are those of before)
   with pytest.raises(ValueError): dec.prefill([1], slot=0)
   with pytest.raises(ValueError): dec.prefill_batch([[1]], slots=[2])
   with pytest.raises(ValueError): dec.prefill_batch([[1]], p0=[2])
