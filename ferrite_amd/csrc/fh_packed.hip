@@ -24,9 +24,9 @@
 // A key that a pair does not see has the weight 0, but 0 times an infinite or NaN value is NaN: a wave whose result is not
 // finite takes its pairs again one at a time over the keys each sees alone (attend_again).
 //
-// What bounds it (32 heads of 128, 8 key heads, on one MI355X): four prompts of up to 4096 tokens, bf16 q, 331-347 us, 870-920
-// TFLOP/s of the products its rows need (the library's 8192^3 product reaches 1200): the matrix cores are busy 43% of the cycles
-// at the 1.8 GHz the chip holds under this load, the softmax's exponentials and conversions about as long, and moving reads
+// What bounds it (32 heads of 128, 8 key heads, on one MI355X): four prompts of up to 4096 tokens, bf16 q, 331-362 us (394 on
+// another), 840-920 (770) TFLOP/s of the products its rows need (the library's 8192^3 product reaches 1200): the matrix
+// cores are busy 43% of the cycles at the 1.8 GHz the chip holds under this load, the softmax's exponentials and conversions about as long, and moving reads
 // ahead, wave priorities or addresses out of the loop changed nothing. 16 prompts of up to 400 tokens, fp32 q (twice the scores'
 // products): 50 us for 122 MB; a workgroup's few tiles do not hide its start and end. 64 rows behind a prefix of 16384, each
 // with up to 700 rows of its own: 54 us and 5 for the join; 16 rows behind 4096: 14 and 5, a chain of launches and latencies.
@@ -222,16 +222,10 @@ __device__ inline uint4 seq_bf16x8(const SeqRaw& r) {
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
-template <int CF>
+// (an fp32 cache's)
 __device__ inline void seq_f32x8(const SeqRaw& r, float4& x, float4& y) {
-  if constexpr (CF == FH_F32) {
-    x = make_float4(__uint_as_float(r.a.x), __uint_as_float(r.a.y), __uint_as_float(r.a.z), __uint_as_float(r.a.w));
-    y = make_float4(__uint_as_float(r.b.x), __uint_as_float(r.b.y), __uint_as_float(r.b.z), __uint_as_float(r.b.w));
-  } else {
-    const uint4 w = seq_bf16x8<CF>(r);
-    x = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
-    y = make_float4(__uint_as_float(w.z << 16), __uint_as_float(w.z & 0xFFFF0000u), __uint_as_float(w.w << 16), __uint_as_float(w.w & 0xFFFF0000u));
-  }
+  x = make_float4(__uint_as_float(r.a.x), __uint_as_float(r.a.y), __uint_as_float(r.a.z), __uint_as_float(r.a.w));
+  y = make_float4(__uint_as_float(r.b.x), __uint_as_float(r.b.y), __uint_as_float(r.b.z), __uint_as_float(r.b.w));
 }
 
 __device__ inline float q_value(const SeqArgs& a, int64_t at) {
@@ -662,8 +656,8 @@ __global__ __launch_bounds__(64 * SQ_NW, 2) void seq_f32_kernel(SeqArgs a) {
       const int i = tid + 64 * SQ_NW * j, r = i / (HD / 8), c = (i % (HD / 8)) * 8;
       float4* k = (float4*)(Ks[b] + r * LD + c);
       float4* v = (float4*)(Vs[b] + r * LD + c);
-      seq_f32x8<CF>(kraw[j], k[0], k[1]);
-      seq_f32x8<CF>(vraw[j], v[0], v[1]);
+      seq_f32x8(kraw[j], k[0], k[1]);
+      seq_f32x8(vraw[j], v[0], v[1]);
     }
   };
   if (t0 < t1) { load(t0); store(0); }
