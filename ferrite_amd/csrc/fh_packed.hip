@@ -13,9 +13,11 @@
 // fp32 sums or bf16 products, and the output is rescaled a few times a row rather than every tile.
 //
 // The arithmetic goes by the types. A bf16 or block-float cache (whose values are bf16) takes v_mfma_f32_32x32x16_bf16: for bf16
-// output an fp32 q goes in as two bf16 terms (off by 2^-16 of itself at most; a bf16 q is exact in one) and the softmax's
-// weights rounded to bf16 (2^-8 at most, what the output's own rounding adds; their sum is taken before it); for fp32 output q
-// and the weights as three terms, off by 2^-24 at most. An fp32 cache takes v_mfma_f32_32x32x2_f32, nothing rounded.
+// output an fp32 q and the softmax's weights go in as two bf16 terms each, off by 2^-16 of themselves at most, as the decode
+// attention over whole slots keeps them (a bf16 q is exact in one; the weights' sum is taken before their rounding). Weights in
+// one term, 2^-8, are 1-24% faster (4 prompts of up to 4096 334 us, two terms 441; 16 of up to 400 46 and 51; 64 rows behind
+// 16384 54 and 62), but take the output's error from its own rounding's 1.6e-3 to 2.3e-3. For fp32 output q and the weights go
+// in as three terms, off by 2^-24 at most. An fp32 cache takes v_mfma_f32_32x32x2_f32, nothing rounded.
 //
 // Where tiles are few, the keys are split among workgroups (splits_for), each leaving its weighted sum, max and sum of weights
 // in the workspace, and a second kernel joins them; a shared prefix's keys and a row's own are always parts of their own. Joining
@@ -24,12 +26,11 @@
 // A key that a pair does not see has the weight 0, but 0 times an infinite or NaN value is NaN: a wave whose result is not
 // finite takes its pairs again one at a time over the keys each sees alone (attend_again).
 //
-// What bounds it (32 heads of 128, 8 key heads, on one MI355X): four prompts of up to 4096 tokens, bf16 q, 331-362 us (394 on
-// another), 840-920 (770) TFLOP/s of the products its rows need (the library's 8192^3 product reaches 1200): the matrix
-// cores are busy 43% of the cycles at the 1.8 GHz the chip holds under this load, the softmax's exponentials and conversions about as long, and moving reads
-// ahead, wave priorities or addresses out of the loop changed nothing. 16 prompts of up to 400 tokens, fp32 q (twice the scores'
-// products): 50 us for 122 MB; a workgroup's few tiles do not hide its start and end. 64 rows behind a prefix of 16384, each
-// with up to 700 rows of its own: 54 us and 5 for the join; 16 rows behind 4096: 14 and 5, a chain of launches and latencies.
+// What bounds it (32 heads of 128, 8 key heads, on one MI355X): four prompts of up to 4096 tokens 441 us with a bf16 q, 537 with
+// an fp32 one: the products, counted with their terms, at 1030 and 1130 TFLOP/s of the 1200
+// that the library's 8192^3 product reaches. 16 prompts of up to 400 tokens, fp32 q: 51 us for 122 MB; a workgroup's few tiles
+// do not hide its start and end. 64 rows behind a prefix of 16384, each with up to 700 rows of its own: 62 us, 5 of them the
+// join; 16 rows behind 4096: 18, a chain of two launches and their latencies.
 #include <math.h>
 #include <algorithm>
 #include <type_traits>
@@ -746,8 +747,8 @@ static void launch_seq(unsigned blocks, hipStream_t s, const SeqArgs& a) {
   const dim3 g(blocks), b(64 * SQ_NW);
   if constexpr (CF == FH_F32) hipLaunchKernelGGL((seq_f32_kernel<HD, PACKED>), g, b, 0, s, a);
   else if (a.o_bf16) {
-    if (a.q_bf16) hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 1, 1, KG, PACKED>), g, b, 0, s, a);
-    else hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 2, 1, KG, PACKED>), g, b, 0, s, a);
+    if (a.q_bf16) hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 1, 2, KG, PACKED>), g, b, 0, s, a);
+    else hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 2, 2, KG, PACKED>), g, b, 0, s, a);
   } else {
     if (a.q_bf16) hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 1, 3, KG, PACKED>), g, b, 0, s, a);
     else hipLaunchKernelGGL((seq_bf16_kernel<HD, CF, 3, 3, KG, PACKED>), g, b, 0, s, a);

@@ -273,8 +273,8 @@ int fh_attention_prefill(const float* q, int64_t ldq, const void* cache, int cac
  * h / (heads / kv_heads). q's rows and the cache are 16-byte aligned, o's rows aligned to 4 values. Rows and cache values
  * that a query does not see have no part in its result, NaN and infinities included. A workspace (16-byte aligned) as
  * everywhere: no clearing, no state, not shared by calls that overlap. Scores, softmax and sums are fp32. Products of a
- * bf16 or block-float cache run on the matrix cores in bf16 terms: for bf16 output an fp32 q in two (2^-16 of itself), the
- * softmax weights in one (2^-8, the output's own rounding); for fp32 output both in three (2^-24). An fp32 cache's run in
+ * bf16 or block-float cache run on the matrix cores in bf16 terms: for bf16 output an fp32 q and the softmax weights in two
+ * each (2^-16 of themselves, as fh_attention_decode), for fp32 output in three (2^-24). An fp32 cache's run in
  * fp32. A call repeats its bits; a call of other sizes may add a row's keys in other parts. No counterpart in the
  * reference, whose prompts are prefilled one at a time (models/llama.py:498-504) and whose rows each read their own slot
  * (models/llama.py:429-452). */

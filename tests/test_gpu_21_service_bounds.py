@@ -1,0 +1,85 @@
+"""What a batch's calls keep to where they could go wrong unseen: attention's bf16 output within its own rounding and the 2^-16
+that its weights and q are held to."""
+import math
+import numpy as np
+import pytest
+import torch
+import seq_cases as S
+
+pytestmark = pytest.mark.gpu
+
+
+def ops():
+  from ferrite_amd import ops as m
+  return m
+
+
+def ints(v):
+  return torch.tensor(list(v), dtype=torch.int32, device="cuda")
+
+
+def attend(q, values, where, limit, kv, hd):
+  """softmax(q k / sqrt(hd)) v in 64 bits for q [L][heads hd], row t over the first limit[t] of cache rows `where`, and a bound
+  of a kernel's error before its output's own rounding: scores in 32 bits (a sum of hd products: (hd + 2) 2^-24 of the sum of
+  their sizes, and 2^-16 of it for q in two bf16 terms; the exponent's scale and exp 8 2^-24 (1 + |s|)), twice that for
+  each weight (its own and the sum's), the weights in two bf16 terms 2^-16, sums of n terms n 2^-24."""
+  L, heads = q.shape[0], q.shape[1] // hd
+  rep = heads // kv
+  q = q.double().view(L, kv, rep, hd).transpose(0, 1)                                   # [kv][L][rep][hd]
+  k, v = values[:kv][:, where], values[kv:][:, where]                                   # [kv][n][hd]
+  s = torch.einsum("glrd,gnd->glrn", q, k) / math.sqrt(hd)
+  size = torch.einsum("glrd,gnd->glrn", q.abs(), k.abs()) / math.sqrt(hd)
+  seen = (torch.arange(len(where))[None] < torch.as_tensor(limit)[:, None])[None, :, None]
+  p = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+  out, big = torch.einsum("glrn,gnd->glrd", p, v), torch.einsum("glrn,gnd->glrd", p, v.abs())
+  ds = ((hd + 2) * 2.0 ** -24 * size + 2.0 ** -16 * size + 8 * 2.0 ** -24 * (1 + s.abs())).masked_fill(~seen, 0).amax(-1, keepdim=True)
+  tol = (2 * ds + (len(where) + 16) * 2.0 ** -24 + 2.0 ** -16) * big
+  return (t.transpose(0, 1).reshape(L, heads * hd) for t in (out, tol))
+
+
+def check(got, want, tol, what):
+  # (bf16: half a step of what the kernel holds, 2^-8 of it)
+  err = (got.double().cpu() - want).abs()
+  most = tol + 2.0 ** -8 * (want.abs() + tol) + 1e-30
+  assert (err <= most).all(), (what, int((err > most).sum()), float((err / most).max()))
+
+
+HEADS = [(9, 3, 64, "bf16", "fp32"), (8, 2, 128, "bfp8", "fp32"), (8, 2, 128, "bf16", "bf16"), (4, 4, 64, "bfp4", "bf16"), (32, 8, 128, "bf16", "fp32")]
+
+
+@pytest.mark.parametrize("heads,kv,hd,fmt,q", HEADS)
+@pytest.mark.parametrize("lens,cached", [([20, 1, 33], [0, 40, 7]), ([300, 150], [0, 90]), ([2, 3], [700, 900])])
+def test_packed_bf16_output(cuda, heads, kv, hd, fmt, q, lens, cached):
+  # (scores near 0, so that the bound is of the weights' rounding and not the scores')
+  print(f"packed bf16 {lens} {cached} {heads}/{kv} {hd} {fmt} {q}", flush=True)
+  rng = np.random.default_rng(71)
+  first = np.concatenate([[2], 2 + np.cumsum([a + c + 1 for a, c in zip(lens, cached)])])
+  cache, values = S.cache(rng, 2 * kv, int(first[-1]) + 3, hd, fmt)
+  qb = torch.from_numpy(rng.normal(0, 0.1, (sum(lens), heads * hd)).astype(np.float32)).to(S.DTYPE[q])
+  starts = np.concatenate([[0], np.cumsum(lens)])
+  got = ops().attention_prefill_packed(qb.cuda(), cache, heads, kv, hd, ints(starts), ints(cached), ints(first[:-1]), max(a + c for a, c in zip(lens, cached)),
+                                       out_dtype=torch.bfloat16)
+  for s, (a, c) in enumerate(zip(lens, cached)):
+    lo = int(starts[s])
+    want, tol = attend(qb[lo:lo + a], values, torch.arange(a + c) + int(first[s]), c + 1 + np.arange(a), kv, hd)
+    check(got[lo:lo + a], want, tol, s)
+
+
+@pytest.mark.parametrize("heads,kv,hd,fmt,q", HEADS)
+@pytest.mark.parametrize("batch,prefix,own", [(3, 20, 5), (17, 300, 90), (4, 2000, 700)])
+@pytest.mark.parametrize("tiles", [False, True])
+def test_shared_bf16_output(cuda, heads, kv, hd, fmt, q, batch, prefix, own, tiles):
+  # (what attention_decode keeps its weights to, so that a step behind a shared prefix loses nothing)
+  print(f"shared bf16 {batch} {prefix} {own} {heads}/{kv} {hd} {fmt} {q} {tiles}", flush=True)
+  rng = np.random.default_rng(72)
+  mine = rng.integers(1, own + 1, batch)
+  first = prefix + 4 + np.concatenate([[0], np.cumsum(mine)])
+  cache, values = S.cache(rng, 2 * kv, int(first[-1]) + 3, hd, fmt)
+  qb = torch.from_numpy(rng.normal(0, 0.1, (batch, heads * hd)).astype(np.float32)).to(S.DTYPE[q])
+  got = ops().attention_decode_shared(qb.cuda(), cache, heads, kv, hd, ints(prefix + mine - 1), ints(first[:-1]), ints([2]), ints([prefix] * batch), prefix, own,
+                                      o=ops().tiles16(batch, heads * hd) if tiles else None, out_dtype=torch.bfloat16)
+  if tiles: got = got.to_rows()
+  for b in range(batch):
+    where = S.rows_of(2, prefix, int(first[b]), prefix + int(mine[b]))
+    want, tol = attend(qb[b:b + 1], values, where, [len(where)], kv, hd)
+    check(got[b:b + 1], want, tol, b)
