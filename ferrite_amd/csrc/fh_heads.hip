@@ -190,9 +190,10 @@ __global__ __launch_bounds__(HT) void heads_part(HeadArgs a) {
   if (a.inv_temp) {
     const float t = a.inv_temp[row];
     m = block_max(m, sm);
+    const float top = m == -INFINITY ? 0.f : m;  // (a mask may leave nothing of a part: a sum of 0)
     float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < HE; ++j) s += c0 + j < a.vocab ? expf((v[j] - m) * t) : 0.f;
+    for (int j = 0; j < HE; ++j) s += c0 + j < a.vocab ? expf((v[j] - top) * t) : 0.f;
     s = block_sum(s, sm);
     if (tid == 0) {
       if (one) a.lse[row] = fmaf(m, t, logf(s));
@@ -228,8 +229,9 @@ __global__ __launch_bounds__(HT) void heads_merge(HeadArgs a) {
     float m = -INFINITY;
     for (int p = tid; p < a.parts; p += HT) m = fmaxf(m, st[p].x);
     m = block_max(m, sm);
+    const float top = m == -INFINITY ? 0.f : m;
     float s = 0.f;
-    for (int p = tid; p < a.parts; p += HT) s += st[p].y * expf((st[p].x - m) * t);
+    for (int p = tid; p < a.parts; p += HT) s += st[p].y * expf((st[p].x - top) * t);
     s = block_sum(s, sm);
     if (tid == 0) a.lse[row] = fmaf(m, t, logf(s));
   }

@@ -375,9 +375,9 @@ int fh_argmax_parts(const void* parts, int64_t rows, int64_t nparts, int32_t* id
  * largest first, the first column of equal values first (numpy's stable argsort of -x; Tensor.topk's topk_kernel,
  * ferrite/compiler.py:1716-1838), into values [rows][k] and their columns into ids [rows][k]; and, given inv_temp
  * (each row's 1/temperature, [rows]), lse [rows] = log of the sum over the row of exp(x t), as max t + log sum
- * exp((x - max) t) in fp32. Selection is exact (no rounding of the values compared). A row is cut into parts of 4096
- * columns, a workgroup each, whose k best (and sums) a second kernel merges; at most 4096 / k parts (a vocabulary of
- * 262144 at k = 64). NaNs are not ordered as numpy orders them. Workspace: fh_heads_workspace_bytes (0 for one part),
+ * exp((x - max) t) in fp32 (columns at -inf add nothing; -inf for a row of them alone). Selection is exact (no rounding of
+ * the values compared). A row is cut into parts of 4096 columns, a workgroup each, whose k best (and sums) a second kernel
+ * merges; at most 4096 / k parts (a vocabulary of 262144 at k = 64). NaNs are not ordered as numpy orders them. Workspace: fh_heads_workspace_bytes (0 for one part),
  * no state kept between calls. */
 size_t fh_heads_workspace_bytes(int rows, int64_t vocab, int k);
 int fh_logit_heads(const float* logits, int64_t ldl, int rows, int64_t vocab, int k, const float* inv_temp,

@@ -1,10 +1,11 @@
 """What a batch's calls keep to where they could go wrong unseen: attention's bf16 output within its own rounding and the 2^-16
-that its weights and q are held to."""
+that its weights and q are held to; heads under grammars that leave whole parts of a row empty."""
 import math
 import numpy as np
 import pytest
 import torch
 import seq_cases as S
+from oracle.serve import head_of
 
 pytestmark = pytest.mark.gpu
 
@@ -16,6 +17,29 @@ def ops():
 
 def ints(v):
   return torch.tensor(list(v), dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("V", [49152, 4100, 128256])
+def test_heads_under_a_mask_that_leaves_parts_of_a_row_empty(cuda, V):
+  # a grammar that allows a few columns of one part of 4096, one that allows columns of the last part alone, none at all, all
+  rng = np.random.default_rng(V)
+  x = rng.normal(0, 3, (4, V)).astype(np.float32)
+  bits = np.zeros((4, V), bool)
+  bits[0, 11:60], bits[1, V - 3:], bits[3] = True, True, True
+  words = np.zeros((4, -(-V // 32) * 32), np.uint32)
+  words[:, :V] = bits
+  words = (words.reshape(4, -1, 32) << np.arange(32, dtype=np.uint32)).sum(2, dtype=np.uint32).view(np.int32)
+  y = ops().logit_rules(torch.from_numpy(x).cuda(), allowed=torch.from_numpy(words).cuda())
+  t = [1.0, 0.5, 2.0, 1 / 0.7]
+  values, ids, lse = ops().logit_heads(y, 40, torch.tensor(t, dtype=torch.float32, device="cuda"))
+  z = np.where(bits, x, -np.inf).astype(np.float32)
+  for r in (0, 1, 3):
+    wv, wi, wl = head_of(z[r], float(np.float32(t[r])), 40)
+    assert np.array_equal(ids[r].cpu().numpy(), wi) and np.array_equal(values[r].cpu().numpy(), wv), r
+    # (fp32: the maximum's product, each exp and its argument, a sum of at most V terms pairwise, the log: test_heads' bound)
+    assert abs(float(lse[r]) - wl) <= 2e-6 * abs(wl) + 2e-6, (r, float(lse[r]), wl)
+  # (nothing left: no sum, the first columns, -inf each)
+  assert float(lse[2]) == -math.inf and (values[2] == -math.inf).all() and ids[2].tolist() == list(range(40))
 
 
 def attend(q, values, where, limit, kv, hd):
