@@ -199,7 +199,7 @@ class Decoder:
     else:
       if not 0 <= slot < self.slots: raise ValueError(f"share_prefix: slot {slot} outside 0..{self.slots - 1}")
       if not 1 <= length <= min(self.context, self.c.places): raise ValueError(f"share_prefix: {length} places of a slot of {self.context}")
-      rows = np.full(self.batch, length, np.int32) if rows is None else np.asarray(rows, np.int32)
+      rows = np.full(self.batch, length, np.int32) if rows is None else np.array(rows, np.int32)  # (a copy: the caller may write to its own)
       if rows.shape != (self.batch,) or (rows < 0).any() or (rows > length).any(): raise ValueError(f"share_prefix: {self.batch} rows' counts in 0..{length}")
       ops.attention_heads_ok(self.c.heads, self.c.kv, self.hd)
     self.prefix_slot, self.prefix_len, self.shared_host = slot, int(length), rows
