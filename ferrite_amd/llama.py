@@ -178,6 +178,8 @@ class Decoder:
     self.top = 0  # the largest place of the rows set (set_rows), which advance raises,
     self.top_own = 0  # and the largest behind the prefix: the row of its slot
     self.placed = True  # (False from a change of the sharing until the rows are set again)
+    self.behind = np.full(self.slots, -1, np.int64)  # the prefix's places before each slot's rows, where known (_follow)
+    self.sharing = False  # (a prefix was shared at some time)
 
   def weight_bytes(self):
     """Bytes of the weights one decode step reads: every matrix, a row of the embedding, the norms."""
@@ -189,11 +191,20 @@ class Decoder:
     first place behind the prefix on where the row shares one (share_prefix)."""
     self._put(places=places, slots=slots)
 
+  def _follow(self, what, slots, shared, own):
+    """Slots whose rows follow the first shared[i] places of the prefix, written from row own[i] on: noted where a slot begins anew
+    (row 0), and refused where it holds rows known to follow another number of places, which would be read as what they are not."""
+    for s, n, o in zip(slots, shared, own):
+      if o > 0 and self.behind[s] not in (-1, n): raise ValueError(f"{what}: slot {s} holds what follows {self.behind[s]} places of a prefix, not {n}")
+    for s, n, o in zip(slots, shared, own):
+      if o == 0: self.behind[s] = n
+
   def share_prefix(self, slot=None, length=0, rows=None):
     """The first `length` places of slot `slot` (a prompt prefilled there) become the prefix of the batch's sequences: row b
     shares the first rows[b] of them (all of them by default), kept once and read once a step, and its own slot holds its
     places from rows[b] on. A sequence may then have rows[b] + context places. The prefix's slot is not a row's while one
-    shares it. share_prefix() ends it. The rows are set again afterwards (set_rows, step's places)."""
+    shares it, and a slot filled behind one number of places is refused to a row that shares another. share_prefix() ends it. The
+    rows are set again afterwards (set_rows, step's places)."""
     if slot is None:
       slot, length, rows = None, 0, np.zeros(self.batch, np.int32)
     else:
@@ -201,7 +212,9 @@ class Decoder:
       if not 1 <= length <= min(self.context, self.c.places): raise ValueError(f"share_prefix: {length} places of a slot of {self.context}")
       rows = np.full(self.batch, length, np.int32) if rows is None else np.array(rows, np.int32)  # (a copy: the caller may write to its own)
       if rows.shape != (self.batch,) or (rows < 0).any() or (rows > length).any(): raise ValueError(f"share_prefix: {self.batch} rows' counts in 0..{length}")
+      if self.behind[slot] > 0: raise ValueError(f"share_prefix: slot {slot} holds what follows {self.behind[slot]} places of a prefix, not a prompt from its first place on")
       ops.attention_heads_ok(self.c.heads, self.c.kv, self.hd)
+      self.sharing = True
     self.prefix_slot, self.prefix_len, self.shared_host = slot, int(length), rows
     ops.put_i32(rows, self.shared)
     ops.put_i32([(slot or 0) * self.part], self.prefix_row)
@@ -238,6 +251,9 @@ class Decoder:
     if (p < sh).any() or (p - sh >= self.context).any() or (p >= self.c.places).any(): raise ValueError("a place inside the shared prefix, or past the cache or RoPE's tables")
     if (s < 0).any() or (s >= self.slots).any(): raise ValueError(f"a slot outside 0..{self.slots - 1}")
     if self.prefix_slot is not None and (s == self.prefix_slot).any(): raise ValueError(f"slot {self.prefix_slot} holds the shared prefix")
+    if self.sharing:
+      host_of = (lambda t: t) if host else (lambda t: t.cpu().numpy())
+      self._follow("set_rows", host_of(s), self.shared_host, host_of(p - sh))
     self.top, self.top_own = int(p.max()), int((p - sh).max())  # (kept on the host for advance's check)
     self.placed = True
     if host:
@@ -332,6 +348,7 @@ class Decoder:
     if T < 1 or p0 < 0 or p0 + T > min(self.context, self.c.places): raise ValueError("prefill: the prompt's places past the cache or RoPE's tables")
     if not 0 <= slot < self.slots: raise ValueError(f"prefill: slot {slot} outside 0..{self.slots - 1}")
     if self.prefix_slot not in (None, slot): raise ValueError("prefill: sequences behind a shared prefix go through prefill_batch")
+    self._follow("prefill", [slot], [0], [p0])
     chunk = chunk or T
     for a in range(0, T, chunk):
       out = self._prefill_chunk(ids[a:a + chunk], slot, p0 + a)
@@ -369,9 +386,10 @@ class Decoder:
   def prefill_batch(self, prompts, slots=None, p0=None, shared=None):
     """Prompts of many sequences at once, on the matrix cores: prompt i's tokens at places p0[i], p0[i] + 1, ... of slot
     slots[i] (slot i by default), each slot once; the first shared[i] places are the prefix's (share_prefix; by default all of them,
-    none without one) and p0 begins behind them by default. Their keys and values go into the cache; returns each prompt's
-    last token's logits ([n][vocab] fp32) and greedy picks ([n] int32). The rows of all prompts go through the matmuls
-    together, so a prompt's logits have prefill's values within the rounding of bf16 rows and fp32 sums."""
+    none without one) and p0 begins behind them by default. The row that steps a slot later shares as many (share_prefix's rows;
+    set_rows refuses another count). Their keys and values go into the cache; returns each prompt's last token's logits
+    ([n][vocab] fp32) and greedy picks ([n] int32). The rows of all prompts go through the matmuls together, so a prompt's
+    logits have prefill's values within the rounding of bf16 rows and fp32 sums."""
     c, hd, dev = self.c, self.hd, self.device
     n = len(prompts)
     if n < 1: raise ValueError("prefill_batch: no prompt")
@@ -386,6 +404,7 @@ class Decoder:
     if self.prefix_slot is not None and (slots == self.prefix_slot).any(): raise ValueError(f"prefill_batch: slot {self.prefix_slot} holds the shared prefix")
     if (p0 < sh).any() or (p0 - sh + lens > self.context).any() or (p0 + lens > c.places).any():
       raise ValueError("prefill_batch: a prompt's places inside the shared prefix, or past the cache or RoPE's tables")
+    self._follow("prefill_batch", slots, sh, p0 - sh)
     T, starts = int(lens.sum()), np.concatenate([[0], np.cumsum(lens)])
     P = self._prefill_buffers(T)
     of = np.repeat(np.arange(n), lens)  # each row's prompt

@@ -31,3 +31,42 @@ def test_the_callers_counts_are_copied(decoder):
   decoder.set_rows([70, 40, 9], [0, 1, 2])
   assert decoder.shared.tolist() == [70, 35, 0] and decoder.rows.tolist() == [0, 100 + 5, 200 + 9]
   with pytest.raises(ValueError): decoder.set_rows([70, 20, 9], [0, 1, 2])  # (place 20 is the prefix's)
+
+
+def test_a_slot_is_read_behind_the_places_it_was_filled_behind(decoder, monkeypatch):
+  # prefill_batch fills slots behind the whole prefix by default: a row that shares less of it would read them from another row
+  def launched(T): raise RuntimeError("the checks passed")
+  monkeypatch.setattr(decoder, "_prefill_buffers", launched)
+  def fill(*a, **kw):  # prefill_batch up to where it would launch
+    with pytest.raises(RuntimeError, match="the checks passed"): decoder.prefill_batch(*a, **kw)
+  decoder.share_prefix(3, 70, rows=[70, 35, 0])
+  fill([[1, 2], [3, 4], [5, 6]])
+  with pytest.raises(ValueError, match="slot 1 holds what follows 70 places of a prefix, not 35"): decoder.set_rows([72, 40, 2], [0, 1, 2])
+  for where in (torch.tensor, list):
+    with pytest.raises(ValueError, match="not 35"): decoder.set_rows(where([72, 37, 0]), where([0, 1, 2]))
+  decoder.set_rows([72, 35, 0], [0, 1, 2])           # (a row that begins its slot anew reads nothing of it)
+  fill([[1, 2], [3, 4], [5, 6]], shared=[70, 35, 0])
+  decoder.set_rows([72, 37, 2], [0, 1, 2])
+  with pytest.raises(ValueError, match="slot 1"): decoder.prefill_batch([[7]], slots=[1], p0=[72])          # (a second turn by the default)
+  fill([[7]], slots=[1], p0=[37], shared=[35])
+  with pytest.raises(ValueError, match="slot 0"): decoder.share_prefix(0, 20)               # (no whole prompt)
+  decoder.share_prefix()
+  with pytest.raises(ValueError, match="slot 0"): decoder.set_rows([2, 0, 2], [0, 1, 2])
+  decoder.set_rows([0, 0, 2], [0, 1, 2])
+
+
+def test_a_whole_sequence_is_not_read_behind_a_prefix(decoder, monkeypatch):
+  monkeypatch.setattr(decoder, "_prefill_chunk", lambda ids, slot, p0: None)
+  decoder.prefill([1] * 80, slot=0)
+  decoder.prefill([1] * 70, slot=3)
+  decoder.share_prefix(3, 70)
+  with pytest.raises(ValueError, match="slot 0 holds what follows 0 places of a prefix, not 70"): decoder.set_rows([80, 70, 70], [0, 1, 2])
+  decoder.set_rows([75, 75, 75], [1, 1, 2])           # (slots filled by nobody here: what they hold is the program's)
+  decoder.share_prefix()
+  decoder.set_rows([80, 5, 5], [0, 1, 2])
+  decoder.share_prefix(3, 70)
+  decoder.set_rows([70, 75, 75], [0, 1, 2])           # (slot 0 anew, behind the prefix)
+  decoder.share_prefix()
+  with pytest.raises(ValueError, match="slot 0"): decoder.prefill([1], slot=0, p0=6)
+  decoder.prefill([1], slot=0)
+  decoder.prefill([1], slot=0, p0=1)

@@ -107,3 +107,19 @@ def test_shared_bf16_output(cuda, heads, kv, hd, fmt, q, batch, prefix, own, til
     where = S.rows_of(2, prefix, int(first[b]), prefix + int(mine[b]))
     want, tol = attend(qb[b:b + 1], values, where, [len(where)], kv, hd)
     check(got[b:b + 1], want, tol, b)
+
+
+def test_rows_given_on_the_gpu_behind_the_places_their_slots_were_filled_behind(cuda):
+  # places and slots as tensors on the GPU: the same cache rows, steps and refusals as the host's
+  from test_gpu_20_serving import decoder
+  rng = np.random.default_rng(73)
+  prompt = lambda n: [int(i) for i in rng.integers(0, 2048, n)]
+  dec = decoder(74, "bf16", 3, 100, 4)
+  dec.prefill(prompt(70), slot=3)
+  dec.share_prefix(3, 70, rows=[70, 35, 0])
+  prompts = [prompt(n) for n in (5, 9, 20)]
+  dec.prefill_batch(prompts)
+  with pytest.raises(ValueError, match="slot 1 holds"): dec.step([1, 2, 3], ints([75, 44, 20]), ints([0, 1, 2]))
+  dec.prefill_batch(prompts, shared=[70, 35, 0])
+  got = dec.step([1, 2, 3], ints([75, 44, 20]), ints([0, 1, 2]))[0].clone()
+  assert torch.equal(got, dec.step([1, 2, 3], [75, 44, 20], [0, 1, 2])[0]) and dec.rows.tolist() == [5, 109, 220]
