@@ -785,13 +785,20 @@ static int launch_seq(const char* fn, int head_dim, int cf, int pairs, int64_t b
 // dimensions (8 times that in fp32), two a CU take them together in twice the time, so that more than one a CU gains nothing; a
 // second kernel costs 3 us, and each part of a pair is written and read at 4 TB/s (512 rows of 32 heads: 4 us a part). `others`:
 // workgroups beside them (a decode step's rows' own keys), of other_tiles each: free until the CUs are one each.
+//
+// A workspace holds the parts of any call of no more rows, keys and heads (callers take one for their largest), so its size is a
+// bound that grows with each of them: a part a split for the pairs there are, up to the most that any sizes choose (below 3 parts
+// of 128 pairs a CU for packed prompts, 4 for a decode step, whose own keys are a part more); at most `most` splits keep to it.
 constexpr int SQ_CUS = 256, SQ_MAX_SPLITS = 32;
-static int splits_for(int64_t groups, int64_t keys, int64_t pairs, int head_dim, int cf, double joined, int64_t others = 0, int64_t other_tiles = 0) {
+constexpr int64_t SQ_PACKED_PARTS = 3 * 128 * SQ_CUS, SQ_SHARED_PARTS = 4 * 128 * SQ_CUS;
+static int64_t key_tiles(int64_t keys) { return std::max<int64_t>(1, (std::min<int64_t>(keys, 1LL << 40) + 63) / 64); }
+static int most_splits(int64_t keys) { return (int)std::min<int64_t>(SQ_MAX_SPLITS, key_tiles(keys)); }
+static int splits_for(int64_t groups, int64_t keys, int64_t pairs, int head_dim, int cf, double joined, int64_t most, int64_t others = 0, int64_t other_tiles = 0) {
   const double tile = 1.2 * head_dim / 128 * (cf == FH_F32 ? 8 : 1), part = 8e-6 / 4 * pairs * (head_dim + 2);
-  const int64_t tiles = std::max<int64_t>(1, (std::min<int64_t>(keys, 1LL << 40) + 63) / 64);
+  const int64_t tiles = key_tiles(keys);
   int best = 1;
   double least = 0;
-  for (int s = 1; s <= std::min<int64_t>(SQ_MAX_SPLITS, tiles); ++s) {
+  for (int s = 1; s <= std::min<int64_t>(most_splits(keys), std::max<int64_t>(1, most)); ++s) {
     const double own = groups * s + others > SQ_CUS ? std::max(1.0, (double)others / SQ_CUS) * other_tiles : 0;
     const double t = tile * (((tiles + s - 1) / s) * std::max(1.0, (double)groups * s / SQ_CUS) + own) + part * s + (s > 1 ? joined : 0);
     if (s == 1 || t < least) { least = t; best = s; }
@@ -803,15 +810,18 @@ static int splits_for(int64_t groups, int64_t keys, int64_t pairs, int head_dim,
 static int packed_pairs(int64_t rows, int n, int rep, int cf) { return cf != FH_F32 && rows * rep <= (int64_t)64 * n ? 64 : 128; }
 static int64_t packed_tiles(int64_t rows, int n, int rep, int pairs) { return rows * rep / pairs + std::min<int64_t>(n, rows); }
 static int packed_splits(int64_t rows, int n, int heads, int kv_heads, int head_dim, int cf, int64_t max_context) {
-  return splits_for(packed_tiles(rows, n, heads / kv_heads, 128) * kv_heads, max_context, rows * heads, head_dim, cf, 3);
+  return splits_for(packed_tiles(rows, n, heads / kv_heads, 128) * kv_heads, max_context, rows * heads, head_dim, cf, 3, SQ_PACKED_PARTS / (rows * heads));
 }
 static int shared_pairs(int cf) { return cf == FH_F32 ? 128 : 64; }
 static void shared_splits(int batch, int heads, int kv_heads, int head_dim, int cf, int64_t max_prefix, int64_t max_own, int& tiles, int& prefix, int& own) {
   const int pairs = shared_pairs(cf);
   tiles = (int)(((int64_t)batch * (heads / kv_heads) + pairs - 1) / pairs);
-  prefix = splits_for((int64_t)tiles * kv_heads, max_prefix, (int64_t)batch * heads, head_dim, cf, 0, (int64_t)batch * kv_heads, (max_own + 127) / 128);
-  own = splits_for((int64_t)batch * kv_heads * 2, max_own, (int64_t)batch * heads, head_dim, cf, 0);  // (the prefix has the other half of the GPU)
+  const int64_t rows = (int64_t)batch * heads, most = SQ_SHARED_PARTS / rows;
+  own = splits_for((int64_t)batch * kv_heads * 2, max_own, rows, head_dim, cf, 0, most - 1);  // (the prefix has the other half of the GPU)
+  prefix = splits_for((int64_t)tiles * kv_heads, max_prefix, rows, head_dim, cf, 0, most - own, (int64_t)batch * kv_heads, (max_own + 127) / 128);
 }
+
+static size_t parts_bytes(int64_t parts, int head_dim) { return (size_t)parts * (head_dim + 2) * sizeof(float); }
 
 // what both entry points ask of their operands (fn: the name in the message)
 static int seq_check(const char* fn, const SeqArgs& a, int q_dtype, int cache_dtype, int head_dim, int o_dtype) {
@@ -839,8 +849,8 @@ using namespace fh;
 extern "C" size_t fh_attention_packed_workspace_bytes(int64_t rows, int sequences, int heads, int kv_heads, int head_dim,
                                                       int64_t max_context) {
   if (rows < 1 || sequences < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || max_context < 1) return 0;
-  const int s = std::max(packed_splits(rows, sequences, heads, kv_heads, head_dim, FH_BF16, max_context), packed_splits(rows, sequences, heads, kv_heads, head_dim, FH_F32, max_context));
-  return s == 1 ? 0 : (size_t)rows * heads * s * (head_dim + 2) * sizeof(float);
+  const int s = most_splits(max_context);
+  return s == 1 ? 0 : parts_bytes(std::min(rows * heads * s, SQ_PACKED_PARTS), head_dim);
 }
 
 extern "C" int fh_attention_prefill_packed(const void* q, int q_dtype, int64_t ldq, const void* cache, int cache_dtype,
@@ -866,7 +876,7 @@ extern "C" int fh_attention_prefill_packed(const void* q, int q_dtype, int64_t l
   a.scale = 1.0f / sqrtf((float)head_dim);
   a.splits = a.parts = packed_splits(rows, sequences, heads, kv_heads, head_dim, cache_dtype, max_context);
   a.part = (float*)workspace;
-  if (a.parts > 1 && (!workspace || ws_bytes < fh_attention_packed_workspace_bytes(rows, sequences, heads, kv_heads, head_dim, max_context) || ((uintptr_t)workspace & 15)))
+  if (a.parts > 1 && (!workspace || ws_bytes < parts_bytes(rows * heads * a.parts, head_dim) || ((uintptr_t)workspace & 15)))
     return fail(FH_EINVAL, "fh_attention_prefill_packed: a 16-byte aligned workspace of fh_attention_packed_workspace_bytes");
   const int pairs = packed_pairs(rows, sequences, a.rep, cache_dtype);
   return launch_seq(fn, head_dim, cache_dtype, pairs, packed_tiles(rows, sequences, a.rep, pairs) * a.splits * kv_heads, as_stream(stream), a);
@@ -875,10 +885,8 @@ extern "C" int fh_attention_prefill_packed(const void* q, int q_dtype, int64_t l
 extern "C" size_t fh_attention_shared_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int64_t max_prefix,
                                                       int64_t max_own) {
   if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || max_prefix < 0 || max_own < 0) return 0;
-  int tiles, prefix, own, tiles32, prefix32, own32;  // (the most of any cache)
-  shared_splits(batch, heads, kv_heads, head_dim, FH_BF16, max_prefix, max_own, tiles, prefix, own);
-  shared_splits(batch, heads, kv_heads, head_dim, FH_F32, max_prefix, max_own, tiles32, prefix32, own32);
-  return (size_t)batch * heads * std::max(prefix + own, prefix32 + own32) * (head_dim + 2) * sizeof(float);
+  const int64_t pairs = (int64_t)batch * heads;
+  return parts_bytes(std::max(2 * pairs, std::min(pairs * (most_splits(max_prefix) + most_splits(max_own)), SQ_SHARED_PARTS)), head_dim);
 }
 
 extern "C" int fh_attention_decode_shared(const void* q, int q_dtype, const void* cache, int cache_dtype, int64_t cache_len,
@@ -905,7 +913,7 @@ extern "C" int fh_attention_decode_shared(const void* q, int q_dtype, const void
   shared_splits(batch, heads, kv_heads, head_dim, cache_dtype, max_prefix, max_own, a.tiles, a.splits, a.own_splits);
   a.parts = a.splits + a.own_splits;
   a.part = (float*)workspace;
-  if (!workspace || ws_bytes < fh_attention_shared_workspace_bytes(batch, heads, kv_heads, head_dim, max_prefix, max_own) || ((uintptr_t)workspace & 15))
+  if (!workspace || ws_bytes < parts_bytes((int64_t)batch * heads * a.parts, head_dim) || ((uintptr_t)workspace & 15))
     return fail(FH_EINVAL, "fh_attention_decode_shared: a 16-byte aligned workspace of fh_attention_shared_workspace_bytes");
   const int pairs = shared_pairs(cache_dtype), row_tiles = (a.rep + pairs - 1) / pairs;
   return launch_seq(fn, head_dim, cache_dtype, 64, ((int64_t)a.tiles * a.splits + (int64_t)batch * row_tiles * a.own_splits) * kv_heads, as_stream(stream), a);

@@ -400,7 +400,8 @@ def attention_heads_ok(heads, kv_heads, head_dim):
 
 
 def attention_packed_workspace(rows, sequences, heads, kv_heads, head_dim, max_context, device="cuda"):
-  """fh_attention_prefill_packed's workspace, uninitialised (a workspace needs no clearing)."""
+  """fh_attention_prefill_packed's workspace for calls of no more rows, heads and context, uninitialised (a workspace needs no
+  clearing)."""
   n = _packed_bytes(rows, sequences, heads, kv_heads, head_dim, max_context)
   return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
 
@@ -444,7 +445,8 @@ def attention_prefill_packed(q, cache, heads, kv_heads, head_dim, starts, p0, fi
 
 
 def attention_shared_workspace(batch, heads, kv_heads, head_dim, max_prefix, max_own, device="cuda"):
-  """fh_attention_decode_shared's workspace, uninitialised (a workspace needs no clearing)."""
+  """fh_attention_decode_shared's workspace for calls of no more rows, heads and places, uninitialised (a workspace needs no
+  clearing)."""
   n = _shared_bytes(batch, heads, kv_heads, head_dim, max_prefix, max_own)
   return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
 

@@ -272,7 +272,8 @@ int fh_attention_prefill(const float* q, int64_t ldq, const void* cache, int cac
  * FH_F32 or FH_BF16, the cache any of fh_kv_cache_bytes' formats, head_dim 64 or 128; query head h reads kv head
  * h / (heads / kv_heads). q's rows and the cache are 16-byte aligned, o's rows aligned to 4 values. Rows and cache values
  * that a query does not see have no part in its result, NaN and infinities included. A workspace (16-byte aligned) as
- * everywhere: no clearing, no state, not shared by calls that overlap. Scores, softmax and sums are fp32. Products of a
+ * everywhere: no clearing, no state, not shared by calls that overlap; one sized for some rows (or batch), heads and bounds
+ * serves every call of no more of each. Scores, softmax and sums are fp32. Products of a
  * bf16 or block-float cache run on the matrix cores in bf16 terms: for bf16 output an fp32 q and the softmax weights in two
  * each (2^-16 of themselves, as fh_attention_decode), for fp32 output in three (2^-24). An fp32 cache's run in
  * fp32. A call repeats its bits; a call of other sizes may add a row's keys in other parts. No counterpart in the

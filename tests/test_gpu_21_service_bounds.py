@@ -1,5 +1,6 @@
 """What a batch's calls keep to where they could go wrong unseen: attention's bf16 output within its own rounding and the 2^-16
-that its weights and q are held to; heads under grammars that leave whole parts of a row empty."""
+that its weights and q are held to; heads under grammars that leave whole parts of a row empty; rows given on the GPU; one
+workspace for a service's largest calls."""
 import math
 import numpy as np
 import pytest
@@ -123,3 +124,33 @@ def test_rows_given_on_the_gpu_behind_the_places_their_slots_were_filled_behind(
   dec.prefill_batch(prompts, shared=[70, 35, 0])
   got = dec.step([1, 2, 3], ints([75, 44, 20]), ints([0, 1, 2]))[0].clone()
   assert torch.equal(got, dec.step([1, 2, 3], [75, 44, 20], [0, 1, 2])[0]) and dec.rows.tolist() == [5, 109, 220]
+
+
+def test_one_workspace_for_a_services_largest_calls(cuda):
+  # taken once for the largest batch and bounds, it serves smaller ones, whose keys are split where the largest's are not
+  rng = np.random.default_rng(75)
+  heads, kv, hd = 32, 8, 128
+  cache, values = S.cache(rng, 2 * kv, 5000, hd, "bf16")
+  ws = ops().attention_packed_workspace(8192, 16, heads, kv, hd, 4096)
+  ws.fill_(255)
+  for lens, cached in (([200], [3000]), ([3], [4090]), ([40, 30], [500, 9])):
+    first = np.concatenate([[0], np.cumsum([a + c for a, c in zip(lens, cached)])])
+    starts = np.concatenate([[0], np.cumsum(lens)])
+    q = torch.from_numpy(rng.normal(0, 0.1, (sum(lens), heads * hd)).astype(np.float32))
+    got = ops().attention_prefill_packed(q.cuda(), cache, heads, kv, hd, ints(starts), ints(cached), ints(first[:-1]), 4096, workspace=ws, out_dtype=torch.bfloat16)
+    for s, (a, c) in enumerate(zip(lens, cached)):
+      lo, some = int(starts[s]), slice(max(0, a - 7), a)  # (the last rows of each, in 64 bits)
+      want, tol = attend(q[lo:lo + a][some], values, torch.arange(a + c) + int(first[s]), (c + 1 + np.arange(a))[some], kv, hd)
+      check(got[lo:lo + a][some], want, tol, (lens, s))
+  ws = ops().attention_shared_workspace(16, heads, kv, hd, 4096, 4096)
+  ws.fill_(255)
+  for batch, prefix, own in ((16, 4096, 40), (3, 4000, 300), (1, 10, 900)):
+    first = prefix + np.arange(batch) * 50
+    mine = rng.integers(1, own + 1, batch)
+    q = torch.from_numpy(rng.normal(0, 0.1, (batch, heads * hd)).astype(np.float32))
+    got = ops().attention_decode_shared(q.cuda(), cache, heads, kv, hd, ints(prefix + mine - 1), ints(first), ints([0]), ints([prefix] * batch), prefix, own,
+                                        workspace=ws, out_dtype=torch.bfloat16)
+    for b in range(batch):
+      where = S.rows_of(0, prefix, int(first[b]), prefix + int(mine[b]))
+      want, tol = attend(q[b:b + 1], values, where, [len(where)], kv, hd)
+      check(got[b:b + 1], want, tol, (batch, b))
