@@ -392,6 +392,7 @@ class Decoder:
     logits have prefill's values within the rounding of bf16 rows and fp32 sums."""
     c, hd, dev = self.c, self.hd, self.device
     n = len(prompts)
+    ops.attention_heads_ok(c.heads, c.kv, hd)  # (before any block's keys are put)
     if n < 1: raise ValueError("prefill_batch: no prompt")
     lens = np.array([len(p) for p in prompts], np.int64)
     slots = np.arange(n) if slots is None else np.asarray(slots, np.int64)

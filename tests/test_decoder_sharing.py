@@ -70,3 +70,12 @@ def test_a_whole_sequence_is_not_read_behind_a_prefix(decoder, monkeypatch):
   with pytest.raises(ValueError, match="slot 0"): decoder.prefill([1], slot=0, p0=6)
   decoder.prefill([1], slot=0)
   decoder.prefill([1], slot=0, p0=1)
+
+
+def test_heads_that_packed_attention_does_not_take_are_refused_before_any_key_is_put(decoder, monkeypatch):
+  def launched(T): raise AssertionError("past the checks")
+  monkeypatch.setattr(decoder, "_prefill_buffers", launched)
+  decoder.hd = 32
+  with pytest.raises(NotImplementedError, match="head_dim"): decoder.prefill_batch([[1, 2]])
+  with pytest.raises(NotImplementedError, match="head_dim"): decoder.share_prefix(3, 70)
+  assert (decoder.behind == -1).all() and decoder.prefix_slot is None
