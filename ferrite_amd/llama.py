@@ -204,9 +204,9 @@ class Decoder:
     shares the first rows[b] of them (all of them by default), kept once and read once a step, and its own slot holds its
     places from rows[b] on. A sequence may then have rows[b] + context places. The prefix's slot is not a row's while one
     shares it, and a slot filled behind one number of places is refused to a row that shares another. share_prefix() ends it. The
-    rows are set again afterwards (set_rows, step's places)."""
+    rows are set again afterwards (set_rows, step's places); a step captured before is captured again where the length changes."""
     if slot is None:
-      slot, length, rows = None, 0, np.zeros(self.batch, np.int32)
+      length, rows = 0, np.zeros(self.batch, np.int32)
     else:
       if not 0 <= slot < self.slots: raise ValueError(f"share_prefix: slot {slot} outside 0..{self.slots - 1}")
       if not 1 <= length <= min(self.context, self.c.places): raise ValueError(f"share_prefix: {length} places of a slot of {self.context}")
@@ -215,11 +215,14 @@ class Decoder:
       if self.behind[slot] > 0: raise ValueError(f"share_prefix: slot {slot} holds what follows {self.behind[slot]} places of a prefix, not a prompt from its first place on")
       ops.attention_heads_ok(self.c.heads, self.c.kv, self.hd)
       self.sharing = True
+    # (the captured step reads the slot's first row and the counts when it runs; another length is another launch)
+    if (slot is None) != (self.prefix_slot is None) or int(length) != self.prefix_len:
+      if self.graph is not None: torch.cuda.synchronize(self.device)  # (a replay may be running)
+      self.ws_shared = ops.attention_shared_workspace(self.batch, self.c.heads, self.c.kv, self.hd, length, self.context, self.device) if slot is not None else None
+      self.graph = None  # (the step is captured again)
     self.prefix_slot, self.prefix_len, self.shared_host = slot, int(length), rows
     ops.put_i32(rows, self.shared)
     ops.put_i32([(slot or 0) * self.part], self.prefix_row)
-    self.ws_shared = ops.attention_shared_workspace(self.batch, self.c.heads, self.c.kv, self.hd, length, self.context, self.device) if slot is not None else None
-    self.graph = None  # (the step is captured again)
     self.placed = False
 
   def _attend(self, l, out):

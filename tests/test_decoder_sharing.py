@@ -79,3 +79,16 @@ def test_heads_that_packed_attention_does_not_take_are_refused_before_any_key_is
   with pytest.raises(NotImplementedError, match="head_dim"): decoder.prefill_batch([[1, 2]])
   with pytest.raises(NotImplementedError, match="head_dim"): decoder.share_prefix(3, 70)
   assert (decoder.behind == -1).all() and decoder.prefix_slot is None
+
+
+def test_the_captured_step_stays_where_only_the_counts_change(decoder, monkeypatch):
+  # a request with another count: the step's kernels read it when they run; another length, or an end, is another capture, which
+  # waits for a replay that may be running
+  waited = []
+  monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: waited.append(device))
+  for share, kept in (((3, 70), False), ((3, 70, [70, 0, 35]), True), ((2, 70), True), ((2, 64), False), ((), False), ((), True)):
+    decoder.graph = graph = object()
+    waited.clear()
+    decoder.share_prefix(*share)
+    assert (decoder.graph is graph) == kept and (decoder.graph is None) == (not kept) and len(waited) == (not kept), share
+    assert not decoder.placed and decoder.prefix_row.item() == (share[0] if share else 0) * 100

@@ -154,3 +154,21 @@ def test_one_workspace_for_a_services_largest_calls(cuda):
       where = S.rows_of(0, prefix, int(first[b]), prefix + int(mine[b]))
       want, tol = attend(q[b:b + 1], values, where, [len(where)], kv, hd)
       check(got[b:b + 1], want, tol, (batch, b))
+
+
+def test_the_captured_step_after_other_counts_and_another_slot(cuda):
+  # the same graph, replayed after share_prefix gave other counts and another slot of the same length, against eager steps
+  from test_gpu_20_serving import decoder
+  rng = np.random.default_rng(76)
+  prompt = lambda n: [int(i) for i in rng.integers(0, 2048, n)]
+  dec = decoder(77, "bf16", 3, 100, 5)
+  for slot in (3, 4): dec.prefill(prompt(70), slot=slot)
+  prompts, graph = [prompt(n) for n in (5, 9, 20)], None
+  for slot, counts in ((3, [70, 70, 70]), (3, [70, 35, 0]), (4, [70, 35, 0]), (4, [0, 70, 12])):
+    dec.share_prefix(slot, 70, rows=counts)
+    dec.prefill_batch(prompts, shared=counts)
+    places = [n + len(p) for n, p in zip(counts, prompts)]
+    want = dec.step([1, 2, 3], places, [0, 1, 2], replay=False)[0].clone()
+    for _ in range(2): assert torch.equal(dec.step([1, 2, 3], places, [0, 1, 2])[0], want), (slot, counts)
+    assert graph is None or dec.graph is graph
+    graph = dec.graph
