@@ -2,6 +2,7 @@
 (a service takes one for its largest batch), and what the sizes are."""
 import random
 import pytest
+import torch
 from ferrite_amd import lib
 
 pytestmark = pytest.mark.skipif(not lib.PATH.exists(), reason="libferrite_hip.so not built")
@@ -53,3 +54,12 @@ def test_a_workspace_too_small_is_refused():
   with pytest.raises(ValueError, match="fh_attention_packed_workspace_bytes"): R.packed(ctx=100000, len=100000, ws=R.P, wb=10 * 8 * 2 * 66 * 4 - 1)
   with pytest.raises(ValueError, match="fh_attention_shared_workspace_bytes"): R.shared(ws=R.P, wb=4 * 8 * 2 * 66 * 4 - 1)
   with pytest.raises(ValueError, match="fh_attention_shared_workspace_bytes"): R.shared(ws=R.P + 8, wb=1 << 30)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="(a call that is not refused would launch on the host's pointers)")
+@pytest.mark.parametrize("batch,prefix,own,parts", [(16, 200, 4096, 4 + 2), (16, 4096, 8192, 16 + 2)])
+def test_many_own_keys_behind_a_short_prefix_are_split(batch, prefix, own, parts):
+  # (what the smallest accepted workspace says of the parts: one part less than these is refused)
+  import test_sequences_refusals as R
+  with pytest.raises(ValueError, match="fh_attention_shared_workspace_bytes"):
+    R.shared(batch=batch, heads=32, kv=8, hd=128, len=100000, mp=prefix, mo=own, ws=R.P, wb=batch * 32 * parts * 4 * 130 - 1)
