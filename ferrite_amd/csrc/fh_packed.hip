@@ -26,11 +26,12 @@
 // A key that a pair does not see has the weight 0, but 0 times an infinite or NaN value is NaN: a wave whose result is not
 // finite takes its pairs again one at a time over the keys each sees alone (attend_again).
 //
-// What bounds it (32 heads of 128, 8 key heads, on one MI355X): four prompts of up to 4096 tokens 441 us with a bf16 q, 537 with
-// an fp32 one: the products, counted with their terms, at 1030 and 1130 TFLOP/s of the 1200
-// that the library's 8192^3 product reaches. 16 prompts of up to 400 tokens, fp32 q: 51 us for 122 MB; a workgroup's few tiles
-// do not hide its start and end. 64 rows behind a prefix of 16384, each with up to 700 rows of its own: 62 us, 5 of them the
-// join; 16 rows behind 4096: 18, a chain of two launches and their latencies.
+// What bounds it (32 heads of 128, 8 key heads, MI355X; ranges over cards and runs): four prompts of up to 4096 tokens 441-481 us
+// with a bf16 q, 537-567 with an fp32 one: the products, counted with their terms, at 950-1030 and 1070-1130 TFLOP/s where the
+// library's 8192^3 product reaches 1200; the matrix cores are busy 52% of the cycles at the 1.76 GHz the chip holds under this
+// load. 16 prompts of up to 400 tokens, fp32 q: 51-56 us for 122 MB; a workgroup's few tiles do not hide its start and end. 64 rows
+// behind a prefix of 16384, each with up to 700 rows of its own: 62-73 us, 5 of them the join; 16 rows behind 4096: 18-19, a
+// chain of two launches and their latencies.
 #include <math.h>
 #include <algorithm>
 #include <type_traits>
@@ -782,8 +783,9 @@ static int launch_seq(const char* fn, int head_dim, int cf, int pairs, int64_t b
 
 // Workgroups the keys of each of `groups` tiles are split among, at most 32 (a wave joins the parts, a lane each): the number
 // that takes the least time by what was measured. A workgroup alone on its CU takes a tile of 64 keys in about 1.2 us at 128
-// dimensions (8 times that in fp32), two a CU take them together in twice the time, so that more than one a CU gains nothing; a
-// second kernel costs 3 us, and each part of a pair is written and read at 4 TB/s (512 rows of 32 heads: 4 us a part). `others`:
+// dimensions (8 times that in fp32; one figure for every other cache, number of terms and tile of pairs), two a CU take them together in twice the time, so that more than one a CU gains nothing. It
+// weighs splits against each other and is no forecast: a call's start, its end and its second launch are not in it (16 rows
+// behind 4096: 7 us by the sum, 18 measured). A second kernel costs 3 us, and each part of a pair is written and read at 4 TB/s (512 rows of 32 heads: 4 us a part). `others`:
 // workgroups beside them (a decode step's rows' own keys), of other_tiles each: free until the CUs are one each.
 //
 // A workspace holds the parts of any call of no more rows, keys and heads (callers take one for their largest), so its size is a

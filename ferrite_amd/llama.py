@@ -201,8 +201,8 @@ class Decoder:
 
   def share_prefix(self, slot=None, length=0, rows=None):
     """The first `length` places of slot `slot` (a prompt prefilled there) become the prefix of the batch's sequences: row b
-    shares the first rows[b] of them (all of them by default), kept once and read once a step, and its own slot holds its
-    places from rows[b] on. A sequence may then have rows[b] + context places. The prefix's slot is not a row's while one
+    shares the first rows[b] of them (all of them by default), kept once and read for many rows at a time, and its own slot holds
+    its places from rows[b] on. A sequence may then have rows[b] + context places. The prefix's slot is not a row's while one
     shares it, and a slot filled behind one number of places is refused to a row that shares another. share_prefix() ends it. The
     rows are set again afterwards (set_rows, step's places); a step captured before is captured again where the length changes."""
     if slot is None:
@@ -445,7 +445,8 @@ class Decoder:
     return logits, ops.argmax_parts(parts)
 
   def step(self, ids=None, places=None, slots=None, replay=True):
-    """One step: the logits (fp32, [batch][vocab]) and picks for tokens ids at places. With replay, the step runs as
+    """One step: the logits (fp32, [batch][vocab]) and greedy picks for tokens ids at places: the model's own, before any rules
+    (a row under rules takes its token from heads). With replay, the step runs as
     a HIP graph captured on the first call (every later step launches the same kernels: places are data)."""
     if ids is not None or places is not None: self._put(ids, places, slots)
     if not self.placed: raise ValueError("step: the rows' places are to be set again after share_prefix")
@@ -463,7 +464,8 @@ class Decoder:
     return self.logits, self.picks
 
   def advance(self):
-    """Each row's next place and its pick as the next token, on the GPU (no host round trip): greedy decoding. Raises
+    """Each row's next place and its pick as the next token, on the GPU (no host round trip): greedy decoding by the model's own
+    logits. Rows under rules are stepped with the tokens drawn from heads(rules=) instead, step(tokens, places). Raises
     once a row's next place would pass the cache or RoPE's tables (the host keeps the largest place: set_rows', plus
     one a call)."""
     if self.top_own + 1 >= self.context or self.top + 1 >= self.c.places: raise ValueError(f"advance: place {self.top + 1} past the cache or RoPE's tables")
@@ -476,7 +478,8 @@ class Decoder:
   def heads(self, k=64, inv_temp=None, rules=None):
     """The last step's logit heads (models/serve.py:31-47): each row's k best logits and their tokens, and given each
     row's 1/temperature, the log of the sum of exp(x t) over its row (ops.logit_heads: fh_logit_heads). rules: ops.logit_rules'
-    arguments (each request's penalties, biases and grammar mask), whose logits the heads are then of; the step's own stay."""
+    arguments (each request's penalties, biases and grammar mask), whose logits the heads are then of; the step's own logits and
+    picks stay. A row whose mask leaves nothing has -inf for its values and its sum."""
     logits = self.logits
     if rules:
       if getattr(self, "_ruled", None) is None: self._ruled = torch.empty_like(self.logits)

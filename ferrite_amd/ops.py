@@ -455,7 +455,7 @@ def attention_decode_shared(q, cache, heads, kv_heads, head_dim, places, first_r
                             workspace=None, o=None, out_dtype=torch.float32):
   """The decode attention of a batch that shares a prefix (fh_attention_decode_shared): row b of q [batch][heads*hd] (fp32
   or bf16) is at places[b] of its sequence, whose places below shared[b] lie at cache rows prefix_row + place (read once for
-  the batch) and the rest at first_row[b] + place - shared[b]. All int32 on the GPU, read when the kernels run; max_prefix
+  64 pairs of a row and a head of a key head) and the rest at first_row[b] + place - shared[b]. All int32 on the GPU, read when the kernels run; max_prefix
   bounds shared, max_own the places behind it. A row at place -1 sees nothing and gives zeros. o: contiguous fp32 or bf16 of
   q's shape, or Tiles16."""
   what = "attention_decode_shared"

@@ -294,7 +294,8 @@ int fh_attention_prefill_packed(const void* q, int q_dtype, int64_t ldq, const v
 
 /* The decode attention of a batch that shares a prefix: row b of q [batch][heads*head_dim] is at places[b] of its sequence,
  * whose first shared[b] places are the prefix's (each row its own count, 0 for none). The prefix's rows are read once for
- * the whole batch. max_prefix bounds shared, max_own the places behind it (keys past either are not read). o: FH_F32,
+ * 64 pairs of a row and a query head of each key head (128 pairs of an fp32 cache): 16 rows of 4 heads a key head read them
+ * once, 64 rows four times, from the L2 where it holds them. max_prefix bounds shared, max_own the places behind it (keys past either are not read). o: FH_F32,
  * FH_BF16 or FH_BF16_T16, rows of heads * head_dim. */
 size_t fh_attention_shared_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int64_t max_prefix, int64_t max_own);
 int fh_attention_decode_shared(const void* q, int q_dtype, const void* cache, int cache_dtype, int64_t cache_len, int batch,
