@@ -194,10 +194,14 @@ class Decoder:
   def _follow(self, what, slots, shared, own):
     """Slots whose rows follow the first shared[i] places of the prefix, written from row own[i] on: noted where a slot begins anew
     (row 0), and refused where it holds rows known to follow another number of places, which would be read as what they are not."""
-    for s, n, o in zip(slots, shared, own):
-      if o > 0 and self.behind[s] not in (-1, n): raise ValueError(f"{what}: slot {s} holds what follows {self.behind[s]} places of a prefix, not {n}")
-    for s, n, o in zip(slots, shared, own):
-      if o == 0: self.behind[s] = n
+    slots, shared, own = np.asarray(slots), np.asarray(shared), np.asarray(own)
+    held = self.behind[slots]
+    bad = (own > 0) & (held != -1) & (held != shared)
+    if bad.any():
+      i = int(bad.argmax())
+      raise ValueError(f"{what}: slot {slots[i]} holds what follows {held[i]} places of a prefix, not {shared[i]}")
+    anew = own == 0
+    self.behind[slots[anew]] = shared[anew]
 
   def share_prefix(self, slot=None, length=0, rows=None):
     """The first `length` places of slot `slot` (a prompt prefilled there) become the prefix of the batch's sequences: row b
