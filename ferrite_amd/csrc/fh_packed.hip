@@ -820,13 +820,14 @@ static void shared_splits(int batch, int heads, int kv_heads, int head_dim, int 
   tiles = (int)(((int64_t)batch * (heads / kv_heads) + pairs - 1) / pairs);
   const int64_t rows = (int64_t)batch * heads, most = SQ_SHARED_PARTS / rows, groups = (int64_t)tiles * kv_heads, mine = (int64_t)batch * kv_heads;
   // (a row's own keys taken to be half of max_own, on the mean)
-  const int64_t other = (std::min<int64_t>(max_own, 1LL << 40) + 127) / 128, prefix_work = groups * key_tiles(max_prefix), own_work = mine * std::max<int64_t>(1, other);
+  const int64_t other = (std::min<int64_t>(max_own, 1LL << 40) + 127) / 128;
+  const double prefix_work = (double)groups * key_tiles(max_prefix), own_work = (double)mine * std::max<int64_t>(1, other);
   // A row's own keys have half of the GPU beside the prefix, and where that leaves a chain of 8 tiles or more too many, the CUs
   // that their share of all the tiles is worth: 16 rows of 32 heads of 128 after 200 places with 4096 of their own 87 -> 52 us,
   // after 4096 with as many 89 -> 57, after 2048 with 2000 of at most 4096 51 -> 37, with 300 of them 18.1 -> 20.2. For shorter
   // chains that share costs more than it gives (4 rows after 180 with 40 of at most 512 10.2 -> 12.6).
   own = splits_for(mine * 2, max_own, rows, head_dim, cf, 0, most - 1);
-  const int more = splits_for(std::min<int64_t>(mine + mine * prefix_work / own_work, 1LL << 30), max_own, rows, head_dim, cf, 0, most - 1);
+  const int more = splits_for((int64_t)std::min(mine * (1 + prefix_work / own_work), 1e9), max_own, rows, head_dim, cf, 0, most - 1);
   if (key_tiles(max_own) / own - key_tiles(max_own) / more >= 8) own = more;
   prefix = splits_for(groups, max_prefix, rows, head_dim, cf, 0, most - own, mine, other);
 }

@@ -172,3 +172,22 @@ def test_the_captured_step_after_other_counts_and_another_slot(cuda):
     for _ in range(2): assert torch.equal(dec.step([1, 2, 3], places, [0, 1, 2])[0], want), (slot, counts)
     assert graph is None or dec.graph is graph
     graph = dec.graph
+
+
+@pytest.mark.parametrize("batch,prefix,own,bound", [(16, 200, 2500, 4096), (2, 65, 4000, 8192), (16, 300, 90, 1 << 30)])
+def test_many_own_keys_behind_a_short_prefix(cuda, batch, prefix, own, bound):
+  # the rows' own keys split over most of the GPU; a bound far above what is there
+  print(f"own keys {batch} {prefix} {own} {bound}", flush=True)
+  rng = np.random.default_rng(78)
+  heads, kv, hd = 32, 8, 128
+  mine = rng.integers(1, own + 1, batch)
+  mine[0] = own
+  first = prefix + 4 + np.concatenate([[0], np.cumsum(mine)])
+  cache, values = S.cache(rng, 2 * kv, int(first[-1]) + 3, hd, "bf16")
+  q = torch.from_numpy(rng.normal(0, 0.1, (batch, heads * hd)).astype(np.float32))
+  got = ops().attention_decode_shared(q.cuda(), cache, heads, kv, hd, ints(prefix + mine - 1), ints(first[:-1]), ints([2]), ints([prefix] * batch), prefix, bound,
+                                      out_dtype=torch.bfloat16)
+  for b in range(batch):
+    where = S.rows_of(2, prefix, int(first[b]), prefix + int(mine[b]))
+    want, tol = attend(q[b:b + 1], values, where, [len(where)], kv, hd)
+    check(got[b:b + 1], want, tol, b)
