@@ -1,0 +1,184 @@
+// The heads of a projection's rows made ready for attention over a cache in pages, in one pass: q's and k's heads through their
+// RMSNorm (each head its own mean of squares) and the rotation of their row's place, q out, k and v into the page that the
+// sequence's table names for the place, rounded once into whatever the cache holds.
+//   n = x rsqrt(mean x^2 + eps) w        (w + 1 centered; q's and k's heads, where weights are given)
+//   y = n cos + (-n2, n1) sin            (their halves n1, n2)
+//
+// A workgroup a row, HD / 8 lanes a head: a lane holds columns 4 l .. 4 l + 3 of each half, so that a pair turns in the lane, a
+// head's squares meet over 8 or 16 lanes, and a block float's run of 16 columns over 4.
+#include <algorithm>
+#include "fh_common.h"
+
+namespace fh {
+
+struct AppendArgs {
+  const void* x; int64_t ldx;
+  int64_t rows; int n, heads, kv_heads;
+  const float* q_norm; const float* k_norm; float eps; int centered;
+  const float* cos_tab; const float* sin_tab; int64_t rope_rows;
+  const int32_t* starts; const int32_t* p0; const int32_t* tables; int64_t ldt; int table_cols, pages, page_shift;
+  void* q; int q_bf16; int64_t ldq;
+  void* cache; uint8_t* exps; int64_t cache_len;
+};
+
+template <bool BF>
+__device__ inline float4 load4(const void* p, int64_t at) {
+  if constexpr (!BF) return *(const float4*)((const float*)p + at);
+  else {
+    const uint2 w = *(const uint2*)((const uint16_t*)p + at);
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
+  }
+}
+__device__ inline uint32_t two_bf16(float lo, float hi) { return bf16_rne_f(lo) | (bf16_rne_f(hi) << 16); }
+__device__ inline void store4(void* p, bool bf, int64_t at, float4 v) {
+  if (bf) *(uint2*)((uint16_t*)p + at) = make_uint2(two_bf16(v.x, v.y), two_bf16(v.z, v.w));
+  else *(float4*)((float*)p + at) = v;
+}
+
+// 4 columns of a run of 16 of a block float, the run's other columns in the quad's other lanes: their bytes, and the exponent
+template <bool FOUR>
+__device__ inline uint32_t run4(float4 v, uint32_t& top) {
+  const uint32_t b[4] = {bf16_rne_f(v.x), bf16_rne_f(v.y), bf16_rne_f(v.z), bf16_rne_f(v.w)};
+  top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = max(top, (b[i] >> 7) & 255u);
+  top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
+  top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t m = bfp_magnitude(b[i], top, FOUR), s = b[i] >> 15 ? 0u - m : m;
+    w |= FOUR ? (s & 15u) << (4 * i) : (s & 255u) << (8 * i);
+  }
+  return w;
+}
+
+template <int HD, int CF, bool BF>
+__global__ __launch_bounds__(1024) void append_kernel(AppendArgs a) {
+  constexpr int G = HD / 8;  // lanes a head
+  const int64_t t = blockIdx.x;
+  const int lane = threadIdx.x & 63, l = threadIdx.x % G, total = a.heads + 2 * a.kv_heads;
+  // the row's sequence: as many as end at or before it
+  int s = 0;
+  const int begin = a.starts[0];
+  for (int s0 = 0; s0 < a.n; s0 += 64) s += __builtin_popcountll(__ballot(s0 + lane < a.n && a.starts[min(s0 + lane, a.n - 1) + 1] <= t));
+  if (t < begin || s >= a.n) return;
+  const int64_t place = (int64_t)a.p0[s] + t - a.starts[s];
+  const int64_t turn = place < 0 ? 0 : place >= a.rope_rows ? a.rope_rows - 1 : place;
+  int64_t row = -1;  // (a place or a page outside: k and v are not written)
+  if (place >= 0 && place >> a.page_shift < a.table_cols) {
+    const int page = a.tables[s * a.ldt + (place >> a.page_shift)];
+    if (page >= 0 && page < a.pages) row = ((int64_t)page << a.page_shift) + (place & ((1 << a.page_shift) - 1));
+  }
+  for (int h = threadIdx.x / G; h < total; h += blockDim.x / G) {
+    const int64_t at = t * a.ldx + (int64_t)h * HD + 4 * l;
+    float4 u = load4<BF>(a.x, at), v = load4<BF>(a.x, at + HD / 2);
+    if (h < a.heads + a.kv_heads) {
+      const float* w = h < a.heads ? a.q_norm : a.k_norm;
+      if (w) {
+        float ss = u.x * u.x + u.y * u.y + u.z * u.z + u.w * u.w + (v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w);
+#pragma unroll
+        for (int m = 1; m < G; m <<= 1) ss += __shfl_xor(ss, m, 64);
+        const float r = 1.f / sqrtf(ss * (1.f / HD) + a.eps), c = a.centered ? 1.f : 0.f;
+        const float4 wu = *(const float4*)(w + 4 * l), wv = *(const float4*)(w + HD / 2 + 4 * l);
+        u.x *= r * (wu.x + c); u.y *= r * (wu.y + c); u.z *= r * (wu.z + c); u.w *= r * (wu.w + c);
+        v.x *= r * (wv.x + c); v.y *= r * (wv.y + c); v.z *= r * (wv.z + c); v.w *= r * (wv.w + c);
+      }
+      if (a.cos_tab) {
+        const float* cs = a.cos_tab + turn * HD + 4 * l;
+        const float* sn = a.sin_tab + turn * HD + 4 * l;
+        const float4 c0 = *(const float4*)cs, c1 = *(const float4*)(cs + HD / 2), s0 = *(const float4*)sn, s1 = *(const float4*)(sn + HD / 2);
+        const float4 y = make_float4(u.x * c0.x - v.x * s0.x, u.y * c0.y - v.y * s0.y, u.z * c0.z - v.z * s0.z, u.w * c0.w - v.w * s0.w);
+        v = make_float4(v.x * c1.x + u.x * s1.x, v.y * c1.y + u.y * s1.y, v.z * c1.z + u.z * s1.z, v.w * c1.w + u.w * s1.w);
+        u = y;
+      }
+    }
+    if (h < a.heads) {
+      const int64_t to = t * a.ldq + (int64_t)h * HD + 4 * l;
+      store4(a.q, a.q_bf16, to, u);
+      store4(a.q, a.q_bf16, to + HD / 2, v);
+      continue;
+    }
+    if (row < 0) continue;
+    const int64_t to = (int64_t)(h - a.heads) * a.cache_len + row;
+    if constexpr (CF == FH_F32 || CF == FH_BF16) {
+      store4(a.cache, CF == FH_BF16, to * HD + 4 * l, u);
+      store4(a.cache, CF == FH_BF16, to * HD + HD / 2 + 4 * l, v);
+    } else {
+      uint32_t tu, tv;
+      const uint32_t mu = run4<CF == FH_BFP4>(u, tu), mv = run4<CF == FH_BFP4>(v, tv);
+      if constexpr (CF == FH_BFP8) {
+        uint8_t* m = (uint8_t*)a.cache + to * HD + 4 * l;
+        *(uint32_t*)m = mu;
+        *(uint32_t*)(m + HD / 2) = mv;
+      } else {
+        uint8_t* m = (uint8_t*)a.cache + to * (HD / 2) + 2 * l;
+        *(uint16_t*)m = (uint16_t)mu;
+        *(uint16_t*)(m + HD / 4) = (uint16_t)mv;
+      }
+      if ((l & 3) == 0) {
+        a.exps[to * (HD / 16) + l / 4] = (uint8_t)tu;
+        a.exps[to * (HD / 16) + HD / 32 + l / 4] = (uint8_t)tv;
+      }
+    }
+  }
+}
+
+template <int HD, int CF>
+static void launch_append(bool bf, hipStream_t s, const AppendArgs& a) {
+  const int lanes = (a.heads + 2 * a.kv_heads) * (HD / 8);
+  const dim3 g((unsigned)a.rows), b(std::min(1024, (lanes + 63) / 64 * 64));
+  if (bf) hipLaunchKernelGGL((append_kernel<HD, CF, true>), g, b, 0, s, a);
+  else hipLaunchKernelGGL((append_kernel<HD, CF, false>), g, b, 0, s, a);
+}
+
+template <int HD>
+static void launch_append(int cf, bool bf, hipStream_t s, const AppendArgs& a) {
+  switch (cf) {
+    case FH_F32: launch_append<HD, FH_F32>(bf, s, a); break;
+    case FH_BF16: launch_append<HD, FH_BF16>(bf, s, a); break;
+    case FH_BFP8: launch_append<HD, FH_BFP8>(bf, s, a); break;
+    default: launch_append<HD, FH_BFP4>(bf, s, a); break;
+  }
+}
+
+}  // namespace fh
+
+using namespace fh;
+
+extern "C" int fh_rope_append_paged(const void* qkv, int x_dtype, int64_t ldx, int64_t rows, int sequences, int heads, int kv_heads,
+                                    int head_dim, const float* q_norm, const float* k_norm, float eps, int centered,
+                                    const float* cos_tab, const float* sin_tab, int64_t rope_rows, const int32_t* starts,
+                                    const int32_t* p0, const int32_t* tables, int64_t ldt, int64_t table_cols, int page, void* q,
+                                    int q_dtype, int64_t ldq, void* cache, int cache_dtype, int64_t cache_len, void* stream) {
+  auto no = [](int code, const char* what) { set_error("fh_rope_append_paged: %s", what); return code; };
+  if (!qkv || !q || !cache || !starts || !p0 || !tables) return no(FH_EINVAL, "null pointer");
+  if (rows < 1 || rows >= (1LL << 31) || sequences < 1) return no(FH_EINVAL, "need 1 <= rows < 2^31 and sequences >= 1");
+  if (heads < 1 || kv_heads < 1) return no(FH_EINVAL, "need heads and kv_heads of at least 1");
+  if (heads > 65535 || kv_heads > 65535) return no(FH_EUNSUP, "at most 65535 heads");
+  if (head_dim != 64 && head_dim != 128) return no(FH_EUNSUP, "head_dim 64 or 128");
+  if (x_dtype != FH_F32 && x_dtype != FH_BF16) return no(FH_EINVAL, "qkv is FH_F32 or FH_BF16");
+  if (q_dtype != FH_F32 && q_dtype != FH_BF16) return no(FH_EINVAL, "q is FH_F32 or FH_BF16");
+  if (cache_dtype < FH_F32 || cache_dtype > FH_BFP4) return no(FH_EUNSUP, "cache is FH_F32, FH_BF16, FH_BFP8 or FH_BFP4");
+  if ((cos_tab == nullptr) != (sin_tab == nullptr) || (cos_tab && rope_rows < 1)) return no(FH_EINVAL, "cos_tab and sin_tab go together, with rope_rows, their rows");
+  if (page < 16 || (page & (page - 1))) return no(FH_EUNSUP, "pages of 16, 32, 64, ... rows (a power of 2)");
+  if (cache_len < page || cache_len % page) return no(FH_EINVAL, "cache_len is whole pages");
+  if (cache_len >= (1LL << 30)) return no(FH_EUNSUP, "fewer than 2^30 cache rows");
+  if (table_cols < 1 || ldt < table_cols) return no(FH_EINVAL, "tables of at least one page a sequence, rows at least as far apart");
+  if (ldx < (int64_t)(heads + 2 * kv_heads) * head_dim || ldq < (int64_t)heads * head_dim || ldx % 4 || ldq % 4 ||
+      ((uintptr_t)qkv & (x_dtype == FH_F32 ? 15 : 7)) || ((uintptr_t)q & (q_dtype == FH_F32 ? 15 : 7)) || ((uintptr_t)cache & 15))
+    return no(FH_EINVAL, "rows at least their heads, qkv's and q's aligned to 4 values, the cache to 16 bytes");
+  if (((uintptr_t)q_norm & 15) || ((uintptr_t)k_norm & 15) || ((uintptr_t)cos_tab & 15) || ((uintptr_t)sin_tab & 15))
+    return no(FH_EINVAL, "norms and tables 16-byte aligned");
+  AppendArgs a = {};
+  a.x = qkv; a.ldx = ldx; a.rows = rows; a.n = sequences; a.heads = heads; a.kv_heads = kv_heads;
+  a.q_norm = q_norm; a.k_norm = k_norm; a.eps = eps; a.centered = centered;
+  a.cos_tab = cos_tab; a.sin_tab = sin_tab; a.rope_rows = rope_rows;
+  a.starts = starts; a.p0 = p0; a.tables = tables; a.ldt = ldt; a.table_cols = (int)std::min<int64_t>(table_cols, 1 << 30);
+  a.page_shift = __builtin_ctz((unsigned)page); a.pages = (int)(cache_len >> a.page_shift);
+  a.q = q; a.q_bf16 = q_dtype == FH_BF16; a.ldq = ldq;
+  a.cache = cache; a.exps = (uint8_t*)cache + kv_exps_at(cache_dtype, kv_heads, cache_len, head_dim); a.cache_len = cache_len;
+  if (head_dim == 128) launch_append<128>(cache_dtype, x_dtype == FH_BF16, as_stream(stream), a);
+  else launch_append<64>(cache_dtype, x_dtype == FH_BF16, as_stream(stream), a);
+  return check_launch("fh_rope_append_paged");
+}

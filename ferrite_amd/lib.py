@@ -64,6 +64,11 @@ SIGNATURES = {
   "fh_attention_prefill_packed": ([P, I, L, P, I, L, L, I, I, I, I, P, P, P, P, P, L, P, I, L, P, S, P], I),
   "fh_attention_shared_workspace_bytes": ([I, I, I, I, L, L], S),
   "fh_attention_decode_shared": ([P, I, P, I, L, I, I, I, I, P, P, P, P, L, L, P, I, P, S, P], I),
+  "fh_rope_append_paged": ([P, I, L, L, I, I, I, I, P, P, ctypes.c_float, I, P, P, L, P, P, P, L, L, I, P, I, L, P, I, L, P], I),
+  "fh_attention_paged_workspace_bytes": ([L, I, I, I, I, L], S),
+  "fh_attention_paged": ([P, I, L, P, I, L, L, I, I, I, I, P, P, P, L, L, I, L, P, I, L, P, S, P], I),
+  "fh_lora_workspace_bytes": ([L, L, I, I], S),
+  "fh_lora": ([P, I, L, L, L, P, P, I, I, I, I, ctypes.POINTER(L), P, P, P, L, P, I, L, P, S, P], I),
   "fh_rms_rows": ([P, L, L, L, P, ctypes.c_float, I, P, I, L, P], I),
   "fh_moe_route": ([P, L, I, L, P, ctypes.c_float, I, P, I, I, I, I, P, P, P, P], I),
   "fh_moe_workspace_bytes": ([I, I, L, L], S),

@@ -483,6 +483,160 @@ def attention_decode_shared(q, cache, heads, kv_heads, head_dim, places, first_r
   return o
 
 
+def _paged_operands(what, starts, p0, tables, page, length):
+  """The arguments that say where packed rows' sequences lie in a cache of `length` rows in pages: tables' rows and columns."""
+  n = p0.numel()
+  _vector(what, "starts", starts, (n + 1,))
+  _vector(what, "p0", p0, (n,))
+  shape, st = tables.shape, tables.stride()
+  if tables.dtype is not _I32 or len(shape) != 2 or shape[0] != n or shape[1] < 1 or (shape[1] > 1 and st[1] != 1) or (n > 1 and st[0] < shape[1]):
+    raise ValueError(f"{what}: tables is [{n}][pages a sequence] {_I32} with contiguous rows")
+  if length % page if page > 0 else True: raise ValueError(f"{what}: a cache of {length} rows is not whole pages of {page}")
+  return n, max(st[0], shape[1]), shape[1]
+
+
+def rope_append_paged(qkv, cache, heads, kv_heads, head_dim, cos, sin, starts, p0, tables, page, q_norm=None, k_norm=None, eps=1e-5, centered=False,
+                      q=None, out_dtype=torch.float32):
+  """A projection's rows qkv [T][(heads + 2 kv_heads) hd] (fp32 or bf16) made ready for attention_paged (fh_rope_append_paged): q's and
+  k's heads through their RMSNorm (q_norm, k_norm [hd] fp32, each where given) and turned by their place's row of cos and sin
+  [places][hd] (fp32; None, None: not turned), q returned (fp32 or bf16), k and v put into the cache's pages. Rows starts[s] .. starts[s + 1] - 1
+  are sequence s's, at places p0[s], p0[s] + 1, ...; place p lies at cache row tables[s][p // page] page + p % page. starts
+  [sequences + 1], p0 and tables [sequences][pages] are int32 on the GPU, read when the kernel runs. page is 16, 32, 64, ... q keeps its
+  rows that are no sequence's; a new q has zeros there. A place or page outside writes no key or value."""
+  what = "rope_append_paged"
+  T = _rows_operand(what, qkv, (heads + 2 * kv_heads) * head_dim)
+  data, dtype, length = _cache_of(what, cache, kv_heads, head_dim)
+  n, ldt, cols = _paged_operands(what, starts, p0, tables, page, length)
+  if q_norm is not None: _vector(what, "q_norm", q_norm, (head_dim,), _F32)
+  if k_norm is not None: _vector(what, "k_norm", k_norm, (head_dim,), _F32)
+  if (cos is None) != (sin is None): raise ValueError(f"{what}: cos and sin go together")
+  turns = 0
+  if cos is not None:
+    if cos.dim() != 2 or cos.shape[1] != head_dim or cos.shape != sin.shape: raise ValueError(f"{what}: cos and sin are [places][{head_dim}] fp32")
+    turns = cos.shape[0]
+    _vector(what, "cos", cos, cos.shape, _F32)
+    _vector(what, "sin", sin, cos.shape, _F32)
+  if q is None: q = torch.zeros(T, heads * head_dim, dtype=out_dtype, device=qkv.device)
+  if q.dtype not in _TORCH or q.shape != (T, heads * head_dim) or q.stride()[1] != 1: raise ValueError(f"{what}: q is [{T}][{heads * head_dim}] fp32 or bf16 with contiguous rows")
+  _here(what, qkv, data, starts, p0, tables, q_norm, k_norm, cos, sin, q)
+  lib.call("fh_rope_append_paged", qkv.data_ptr(), _TORCH[qkv.dtype], _rows_apart(qkv), T, n, heads, kv_heads, head_dim, _ptr(q_norm), _ptr(k_norm), eps, int(centered),
+           _ptr(cos), _ptr(sin), turns, starts.data_ptr(), p0.data_ptr(), tables.data_ptr(), ldt, cols, page, q.data_ptr(), _TORCH[q.dtype],
+           _rows_apart(q), data.data_ptr(), dtype, length, _stream())
+  return q
+
+
+def _rows_apart(t):
+  """A [rows][cols] operand's row stride (one row's may be anything)."""
+  return t.stride()[0] if t.shape[0] > 1 else t.shape[1]
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_bytes(*sizes): return lib.load().fh_attention_paged_workspace_bytes(*sizes)
+
+
+def attention_paged_workspace(rows, sequences, heads, kv_heads, head_dim, max_context, device="cuda"):
+  """fh_attention_paged's workspace for calls of no more rows, sequences, heads and context, uninitialised (a workspace needs no
+  clearing)."""
+  n = _paged_bytes(rows, sequences, heads, kv_heads, head_dim, max_context)
+  return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
+
+
+def attention_paged(q, cache, heads, kv_heads, head_dim, starts, p0, tables, page, max_context, workspace=None, o=None, out_dtype=torch.float32):
+  """The causal attention of packed rows over a cache in pages (fh_attention_paged): prompts, chunks of them and single tokens in one
+  call. q [T][heads hd] (fp32 or bf16); starts, p0, tables and page as rope_append_paged's, which put the rows' own keys. max_context
+  bounds every place + 1. o (fp32 or bf16) keeps its rows that are no sequence's; a new o has zeros there. A row at a place
+  below 0 sees nothing and gives zeros."""
+  what = "attention_paged"
+  cols = heads * head_dim
+  T = _rows_operand(what, q, cols)
+  data, dtype, length = _cache_of(what, cache, kv_heads, head_dim)
+  n, ldt, pages = _paged_operands(what, starts, p0, tables, page, length)
+  if o is None: o = torch.zeros(T, cols, dtype=out_dtype, device=q.device)
+  if o.dtype not in _TORCH or o.shape != (T, cols) or o.stride()[1] != 1: raise ValueError(f"{what}: o is fp32 or bf16 rows of q's shape")
+  ws, need = None, _paged_bytes(T, n, heads, kv_heads, head_dim, max_context)
+  if need:
+    if workspace is None: workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    ws, need = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+  _here(what, q, data, starts, p0, tables, o, workspace)
+  lib.call("fh_attention_paged", q.data_ptr(), _TORCH[q.dtype], _rows_apart(q), data.data_ptr(), dtype, length, T, n, heads, kv_heads, head_dim,
+           starts.data_ptr(), p0.data_ptr(), tables.data_ptr(), ldt, pages, page, max_context, o.data_ptr(), _TORCH[o.dtype], _rows_apart(o), ws, need, _stream())
+  return o
+
+
+@dataclass
+class Adapters:
+  """Low-rank adapters of a projection [K] -> [N] whose columns are `parts` runs (q, k and v; gate and up; or one): a [adapters][parts
+  rank][K], each part's `rank` rows after the last one's, and b [adapters][N][rank], contiguous fp32 or bf16 alike, rank and K
+  multiples of 8; scale [adapters] fp32, or None for 1. pack_adapters makes one from a checkpoint's matrices."""
+  a: torch.Tensor
+  b: torch.Tensor
+  scale: torch.Tensor | None
+  parts: tuple
+
+  @property
+  def rank(self): return self.b.shape[2]
+
+
+def pack_adapters(matrices, parts, scales=None, dtype=torch.bfloat16, device="cuda"):
+  """Adapters of a projection whose columns are runs of `parts`. matrices: for each adapter a list with, for each part, (A [r][K], B
+  [columns][r]) as a checkpoint holds lora_A and lora_B, or None where the adapter leaves the part alone; ranks may differ
+  (zeros fill them to the largest, in eights). scales: each adapter's factor (alpha / r)."""
+  given = [m for ad in matrices for m in ad if m is not None]
+  if not given or any(len(ad) != len(parts) for ad in matrices): raise ValueError(f"pack_adapters: for each adapter {len(parts)} parts' (A, B) or None")
+  K, r = given[0][0].shape[1], -(-max(A.shape[0] for A, _ in given) // 8) * 8
+  a = torch.zeros(len(matrices), len(parts), r, K, dtype=dtype, device=device)
+  b = torch.zeros(len(matrices), sum(parts), r, dtype=dtype, device=device)
+  for i, ad in enumerate(matrices):
+    n0 = 0
+    for p, (cols, m) in enumerate(zip(parts, ad)):
+      if m is not None:
+        A, B = m
+        if A.shape[1] != K or B.shape != (cols, A.shape[0]): raise ValueError(f"pack_adapters: A {tuple(A.shape)} and B {tuple(B.shape)} of a part [{K}] -> [{cols}]")
+        a[i, p, :A.shape[0]], b[i, n0:n0 + cols, :A.shape[0]] = A.to(device), B.to(device)
+      n0 += cols
+  s = None if scales is None else torch.as_tensor(scales, dtype=_F32).to(device)
+  return Adapters(a.view(len(matrices), len(parts) * r, K), b, s, tuple(parts))
+
+
+def lora_workspace(rows, adapters, device="cuda"):
+  """fh_lora's workspace for calls of no more rows with these adapters, uninitialised (a workspace needs no clearing)."""
+  n = lib.load().fh_lora_workspace_bytes(rows, adapters.a.shape[2], adapters.rank, len(adapters.parts))
+  return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
+
+
+@functools.lru_cache(maxsize=256)
+def _columns(parts): return (ctypes.c_int64 * len(parts))(*parts)
+
+
+@functools.lru_cache(maxsize=1024)
+def _lora_bytes(*sizes): return lib.load().fh_lora_workspace_bytes(*sizes)
+
+
+def lora(x, adapters, ids, residual=None, out=None, workspace=None, out_dtype=torch.float32):
+  """Each row's low-rank adapter beside a shared projection (fh_lora): out = residual + scale_i (x A_i^T) B_i^T for row t of x [T][K] (fp32 or
+  bf16) with i = ids[t] (int32 on the GPU, read when the kernels run); a row whose id is none of the adapters' keeps its residual.
+  residual [T][N] (fp32 or bf16, out's type) may be out itself; None: zeros."""
+  what = "lora"
+  a, b = adapters.a, adapters.b
+  parts = tuple(adapters.parts)
+  if a.dim() != 3 or b.dim() != 3 or a.dtype not in _TORCH or b.dtype != a.dtype or not a.is_contiguous() or not b.is_contiguous():
+    raise ValueError(f"{what}: adapters a [n][parts rank][K] and b [n][N][rank], contiguous, fp32 or bf16 alike")
+  (n, C, K), N, r = a.shape, b.shape[1], b.shape[2]
+  if n < 1 or b.shape[0] != n or C != r * len(parts) or N != sum(parts): raise ValueError(f"{what}: adapters a {tuple(a.shape)} and b {tuple(b.shape)} for parts of {parts} columns")
+  T = _rows_operand(what, x, K)
+  _vector(what, "ids", ids, (T,))
+  if adapters.scale is not None: _vector(what, "scale", adapters.scale, (n,), _F32)
+  if out is None: out = torch.empty(T, N, dtype=out_dtype if residual is None else residual.dtype, device=x.device)
+  for t in (out,) if residual is None else (out, residual):
+    if t.dtype not in _TORCH or t.dtype != out.dtype or t.shape != (T, N) or t.stride()[1] != 1: raise ValueError(f"{what}: residual and out are [{T}][{N}] fp32 or bf16 alike with contiguous rows")
+  if workspace is None: workspace = torch.empty(_lora_bytes(T, K, r, len(parts)), dtype=torch.uint8, device=x.device)
+  _here(what, x, a, b, adapters.scale, ids, residual, out, workspace)
+  lib.call("fh_lora", x.data_ptr(), _TORCH[x.dtype], _rows_apart(x), T, K, a.data_ptr(), b.data_ptr(), _TORCH[a.dtype], n, r, len(parts), _columns(parts),
+           _ptr(adapters.scale), ids.data_ptr(), _ptr(residual), 0 if residual is None else _rows_apart(residual), out.data_ptr(), _TORCH[out.dtype], _rows_apart(out),
+           workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream())
+  return out
+
+
 def gather_rows(x, ids):
   """Rows ids (int32 on the GPU) of x [rows][cols] (4-byte elements, rows contiguous), a copy (fh_gather_rows): an index
   outside x reads its nearest row."""

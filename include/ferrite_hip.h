@@ -303,6 +303,54 @@ int fh_attention_decode_shared(const void* q, int q_dtype, const void* cache, in
                                const int32_t* prefix_row, const int32_t* shared, int64_t max_prefix, int64_t max_own, void* o,
                                int o_dtype, void* workspace, size_t ws_bytes, void* stream);
 
+/* ---- a cache in pages -----------------------------------------------------------------------------------------------
+ * A KV cache of fh_kv_cache_bytes' layout whose rows are cut into pages of `page` consecutive ones (16, 32, 64, ... rows, a
+ * power of 2; cache_len whole pages), so that sequences of any lengths share it: place p of sequence s lies at cache row
+ * tables[s][p / page] page + p % page, tables [sequences][table_cols] rows ldt apart. Rows starts[s] .. starts[s + 1] - 1 of a call's
+ * packed rows are sequence s's, at places p0[s], p0[s] + 1, ...: prompts, chunks of them and single tokens as they come; starts
+ * [sequences + 1] does not decrease (a sequence may have no rows), and rows before starts[0] or from starts[sequences] on are no
+ * sequence's: what is written for rows is left as it was there. All of it is device data, read when the kernels run (a captured
+ * call replays with what the arrays hold then). head_dim 64 or 128. No counterpart in the reference, whose cache is one run of
+ * rows a sequence (models/llama.py:429-452, 506-514). */
+
+/* A projection's rows made ready for attention: qkv [rows][ldx] (FH_F32 or FH_BF16: heads of q, then k, then v); q's and k's heads
+ * through their RMSNorm x rsqrt(mean(x^2) + eps) w (w + 1 when centered), each head its own mean (q_norm, k_norm [head_dim]; each
+ * NULL for none), and turned as FH_EP_ROPE_KV turns them by their place's row of cos_tab and sin_tab ([rope_rows][head_dim], a place
+ * outside reads the nearest row; both NULL: not turned); q out (FH_F32 or FH_BF16), k and v into the cache at their place's row,
+ * rounded as FH_EP_ROPE_KV's put. A place past the table or a page outside the cache writes no key or value. For projections
+ * whose q, k and v are not final in the product (an adapter's part is added first), and for models with normed heads. qkv's
+ * and q's rows are aligned to 4 values; norms, tables of angles and the cache to 16 bytes. */
+int fh_rope_append_paged(const void* qkv, int x_dtype, int64_t ldx, int64_t rows, int sequences, int heads, int kv_heads,
+                         int head_dim, const float* q_norm, const float* k_norm, float eps, int centered,
+                         const float* cos_tab, const float* sin_tab, int64_t rope_rows, const int32_t* starts,
+                         const int32_t* p0, const int32_t* tables, int64_t ldt, int64_t table_cols, int page, void* q,
+                         int q_dtype, int64_t ldq, void* cache, int cache_dtype, int64_t cache_len, void* stream);
+
+/* The causal attention of packed rows over a cache in pages: a row at place p sees places 0 .. p of its sequence (none below 0:
+ * zeros), max_context a bound of every place + 1 (keys past it are not read). Types, alignment, arithmetic and what unseen
+ * keys may hold as fh_attention_prefill_packed's; a page outside the cache is read as its nearest one. */
+size_t fh_attention_paged_workspace_bytes(int64_t rows, int sequences, int heads, int kv_heads, int head_dim, int64_t max_context);
+int fh_attention_paged(const void* q, int q_dtype, int64_t ldq, const void* cache, int cache_dtype, int64_t cache_len,
+                       int64_t rows, int sequences, int heads, int kv_heads, int head_dim, const int32_t* starts,
+                       const int32_t* p0, const int32_t* tables, int64_t ldt, int64_t table_cols, int page, int64_t max_context,
+                       void* o, int o_dtype, int64_t ldo, void* workspace, size_t ws_bytes, void* stream);
+
+/* ---- low-rank adapters ----------------------------------------------------------------------------------------------
+ * Beside a projection that all rows share, each row's own adapter: y = residual + scale_i (x A_i^T) B_i^T with i = ids[row]; a row
+ * whose id is outside 0 .. adapters - 1 keeps its residual. x [rows][ldx] FH_F32 or FH_BF16; a [adapters][parts rank][K] and
+ * b [adapters][N][rank] in w_dtype (FH_F32 or FH_BF16), the layout of a checkpoint's lora_A and lora_B; the projection's N columns are
+ * `parts` runs (1 to 4) of part_cols[p] columns (host memory), part p's rows of b products of rows p rank .. of a. rank a
+ * multiple of 8 up to 128, K and part_cols multiples of 8 (zeros behind what an adapter has of them). scale [adapters] (NULL: 1).
+ * residual [rows][ldr] and y [rows][ldy] in y_dtype (FH_F32 or FH_BF16); residual may be y itself (then ldr = ldy), otherwise
+ * they do not overlap; NULL: zeros. x A^T, sums and the addition are fp32; products are bf16's, fp32 values in two terms for a bf16 y
+ * (2^-16 of themselves) and three for an fp32 one (2^-24); a row with values that are not finite gives values that are not.
+ * Everything 16-byte aligned, rows too. A call repeats its bits; one of other sizes may add K in other parts. Workspace: no
+ * clearing, no state; one for some rows serves fewer. No counterpart in the reference. */
+size_t fh_lora_workspace_bytes(int64_t rows, int64_t K, int rank, int parts);
+int fh_lora(const void* x, int x_dtype, int64_t ldx, int64_t rows, int64_t K, const void* a, const void* b, int w_dtype, int adapters,
+            int rank, int parts, const int64_t* part_cols, const float* scale, const int32_t* ids, const void* residual, int64_t ldr,
+            void* y, int y_dtype, int64_t ldy, void* workspace, size_t ws_bytes, void* stream);
+
 /* out[rows][dim] = x * rsqrt(mean(x^2) + eps) * w (w + 1 when centered), fp32 or bf16 out: the RMSNorm before a
  * prefill GEMM (models/llama.py:82-85), which then takes bf16 rows. */
 int fh_rms_rows(const float* x, int64_t ldx, int64_t rows, int64_t dim, const float* norm_w, float eps, int centered,
