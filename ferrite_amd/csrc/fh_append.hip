@@ -53,6 +53,39 @@ __device__ inline uint32_t run4(float4 v, uint32_t& top) {
   return w;
 }
 
+// A head's norm and rotation, in F's arithmetic: u and v are the lane's columns of its halves. A block float's keys take 64 bits: it
+// rounds twice, and a value that 32 bits leave on the other side of a border ends a whole step of its run away.
+template <typename F, int HD>
+__device__ inline void norm_turn(const AppendArgs& a, const float* w, int64_t turn, int l, float4& u, float4& v) {
+  F x[4] = {u.x, u.y, u.z, u.w}, y[4] = {v.x, v.y, v.z, v.w};
+  if (w) {
+    F ss = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss += x[i] * x[i] + y[i] * y[i];
+#pragma unroll
+    for (int m = 1; m < HD / 8; m <<= 1) ss += __shfl_xor(ss, m, 64);
+    const F r = F(1) / sqrt(ss * F(1.0 / HD) + F(a.eps)), c = a.centered ? F(1) : F(0);
+    const float4 wu = *(const float4*)(w + 4 * l), wv = *(const float4*)(w + HD / 2 + 4 * l);
+    const float wx[4] = {wu.x, wu.y, wu.z, wu.w}, wy[4] = {wv.x, wv.y, wv.z, wv.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[i] *= r * (wx[i] + c); y[i] *= r * (wy[i] + c); }
+  }
+  if (a.cos_tab) {
+    const float* cs = a.cos_tab + turn * HD + 4 * l;
+    const float* sn = a.sin_tab + turn * HD + 4 * l;
+    const float4 c0 = *(const float4*)cs, c1 = *(const float4*)(cs + HD / 2), s0 = *(const float4*)sn, s1 = *(const float4*)(sn + HD / 2);
+    const float cx[4] = {c0.x, c0.y, c0.z, c0.w}, cy[4] = {c1.x, c1.y, c1.z, c1.w}, sx[4] = {s0.x, s0.y, s0.z, s0.w}, sy[4] = {s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const F t = x[i] * cx[i] - y[i] * sx[i];
+      y[i] = y[i] * cy[i] + x[i] * sy[i];
+      x[i] = t;
+    }
+  }
+  u = make_float4((float)x[0], (float)x[1], (float)x[2], (float)x[3]);
+  v = make_float4((float)y[0], (float)y[1], (float)y[2], (float)y[3]);
+}
+
 template <int HD, int CF, bool BF>
 __global__ __launch_bounds__(1024) void append_kernel(AppendArgs a) {
   constexpr int G = HD / 8;  // lanes a head
@@ -75,23 +108,8 @@ __global__ __launch_bounds__(1024) void append_kernel(AppendArgs a) {
     float4 u = load4<BF>(a.x, at), v = load4<BF>(a.x, at + HD / 2);
     if (h < a.heads + a.kv_heads) {
       const float* w = h < a.heads ? a.q_norm : a.k_norm;
-      if (w) {
-        float ss = u.x * u.x + u.y * u.y + u.z * u.z + u.w * u.w + (v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w);
-#pragma unroll
-        for (int m = 1; m < G; m <<= 1) ss += __shfl_xor(ss, m, 64);
-        const float r = 1.f / sqrtf(ss * (1.f / HD) + a.eps), c = a.centered ? 1.f : 0.f;
-        const float4 wu = *(const float4*)(w + 4 * l), wv = *(const float4*)(w + HD / 2 + 4 * l);
-        u.x *= r * (wu.x + c); u.y *= r * (wu.y + c); u.z *= r * (wu.z + c); u.w *= r * (wu.w + c);
-        v.x *= r * (wv.x + c); v.y *= r * (wv.y + c); v.z *= r * (wv.z + c); v.w *= r * (wv.w + c);
-      }
-      if (a.cos_tab) {
-        const float* cs = a.cos_tab + turn * HD + 4 * l;
-        const float* sn = a.sin_tab + turn * HD + 4 * l;
-        const float4 c0 = *(const float4*)cs, c1 = *(const float4*)(cs + HD / 2), s0 = *(const float4*)sn, s1 = *(const float4*)(sn + HD / 2);
-        const float4 y = make_float4(u.x * c0.x - v.x * s0.x, u.y * c0.y - v.y * s0.y, u.z * c0.z - v.z * s0.z, u.w * c0.w - v.w * s0.w);
-        v = make_float4(v.x * c1.x + u.x * s1.x, v.y * c1.y + u.y * s1.y, v.z * c1.z + u.z * s1.z, v.w * c1.w + u.w * s1.w);
-        u = y;
-      }
+      if (CF == FH_F32 || CF == FH_BF16 || h < a.heads) norm_turn<float, HD>(a, w, turn, l, u, v);
+      else norm_turn<double, HD>(a, w, turn, l, u, v);
     }
     if (h < a.heads) {
       const int64_t to = t * a.ldq + (int64_t)h * HD + 4 * l;
