@@ -5,11 +5,19 @@
 
 using namespace fh;
 
+// Workgroups that the GPU holds at a time: two a CU, three of the smaller dimensions' where their registers leave room. They share
+// the keys (SeqWalk); a call of no more rows than sequences with at most PG_WHOLE places takes a workgroup a sequence and key head instead
+// and needs no second launch. The rest is what was measured best:
+// the least share of a workgroup, and the cost from which a tile of 128 pairs of 128 dimensions is cut (its parts are 66 KB each, written and read).
+constexpr int PG_WHOLE = 448, PG_LEAST_TOKENS = 128, PG_LEAST = 256, PG_UNCUT = 512;
+static int paged_slots(int head_dim) { return SQ_CUS * (head_dim == 64 ? 3 : 2); }
+
 extern "C" size_t fh_attention_paged_workspace_bytes(int64_t rows, int sequences, int heads, int kv_heads, int head_dim,
                                                      int64_t max_context) {
   if (rows < 1 || sequences < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || max_context < 1) return 0;
-  const int s = most_splits(max_context);
-  return s == 1 ? 0 : parts_bytes(std::min(rows * heads * s, SQ_PACKED_PARTS), head_dim);
+  // (two parts a workgroup, at most 128 pairs each and no more than there are: the bound of any call of no more)
+  const int64_t pairs = std::min<int64_t>(128, rows * (heads / kv_heads));
+  return parts_bytes(2 * std::max<int64_t>(paged_slots(head_dim), (int64_t)kv_heads * ((heads / kv_heads + 63) / 64)) * pairs, head_dim);
 }
 
 extern "C" int fh_attention_paged(const void* q, int q_dtype, int64_t ldq, const void* cache, int cache_dtype, int64_t cache_len,
@@ -39,10 +47,23 @@ extern "C" int fh_attention_paged(const void* q, int q_dtype, int64_t ldq, const
   a.rep = heads / kv_heads;
   a.cache_exps = (const uint8_t*)cache + kv_exps_at(cache_dtype, kv_heads, cache_len, head_dim);
   a.scale = 1.0f / sqrtf((float)head_dim);
-  a.splits = a.parts = packed_splits(rows, sequences, heads, kv_heads, head_dim, cache_dtype, max_context);
-  a.part = (float*)workspace;
-  if (a.parts > 1 && (!workspace || ws_bytes < parts_bytes(rows * heads * a.parts, head_dim) || ((uintptr_t)workspace & 15)))
-    return fail(FH_EINVAL, "fh_attention_paged: a 16-byte aligned workspace of fh_attention_paged_workspace_bytes");
   const int pairs = packed_pairs(rows, sequences, a.rep, cache_dtype);
-  return launch_seq<true>(fn, head_dim, cache_dtype, pairs, packed_tiles(rows, sequences, a.rep, pairs) * a.splits * kv_heads, as_stream(stream), a);
+  const bool tokens = pairs == 64, small = tokens || cache_dtype == FH_F32;
+  a.tile_rows = std::max(1, pairs / a.rep);
+  a.head_tiles = (a.rep + pairs - 1) / pairs;
+  a.slot_pairs = (int)std::min<int64_t>(pairs, rows * a.rep);
+  a.whole = tokens && rows <= sequences && max_context <= PG_WHOLE;
+  a.walkers = a.whole ? sequences : std::max(1, paged_slots(head_dim) / (kv_heads * a.head_tiles));
+  // (the costs' unit: their sum stays below 2^30)
+  const int64_t tiles = rows / a.tile_rows + std::min<int64_t>(sequences, rows), cost = max_context + SEQ_START + a.tile_rows;
+  while ((double)tiles * (double)((cost + rows) >> a.unit) >= (double)(1 << 30) && a.unit < 30) ++a.unit;
+  a.least = std::max(1, (small ? PG_LEAST_TOKENS : PG_LEAST) >> a.unit);
+  a.uncut = small ? 0 : PG_UNCUT * head_dim / 128 >> a.unit;
+  a.parts = a.walkers > 1 && !a.whole && cost >> a.unit >= a.uncut ? 2 : 1;
+  if (a.parts == 1) a.uncut = 0x7FFFFFFF;
+  a.part = (float*)workspace;
+  const int64_t blocks = (int64_t)a.walkers * kv_heads * a.head_tiles;
+  if (a.parts > 1 && (!workspace || ws_bytes < parts_bytes(2 * blocks * a.slot_pairs, head_dim) || ((uintptr_t)workspace & 15)))
+    return fail(FH_EINVAL, "fh_attention_paged: a 16-byte aligned workspace of fh_attention_paged_workspace_bytes");
+  return launch_seq<true>(fn, head_dim, cache_dtype, pairs, blocks, as_stream(stream), a);
 }

@@ -22,6 +22,12 @@ __device__ __forceinline__ void load_to_lds(const void* from, uint16_t* to) {
   const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uintptr_t)(SEQ_LDS uint16_t*)to);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(at) : "memory", "m0");
 }
+// the same from a wave-uniform base and a lane's own offset
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint16_t* to) {
+  const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uintptr_t)to);  // (an LDS address' low half is its offset)
+  const uint64_t b = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)((uint64_t)base >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint64_t)base);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2" :: "v"(offset), "s"(at), "s"(b) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 constexpr int SQ_NW = 4;               // waves a workgroup
@@ -39,7 +45,10 @@ struct SeqArgs {
   const int32_t* places;        // [n] the place of a sequence's first row
   const int32_t* first_row; const int32_t* prefix_row; const int32_t* shared;
   int64_t max_prefix, max_own;  // bounds of shared, and of the places behind it
-  const int32_t* tables; int64_t ldt; int table_cols, pages, page_shift;  // (pages) each sequence's pages, 2^page_shift rows each
+  // (pages) each sequence's pages, 2^page_shift rows each; rows a tile, tiles of a row's heads, workgroups a tile of heads shares its
+  // keys among, pairs a part holds, the least share of a workgroup (SeqWalk)
+  const int32_t* tables; int64_t ldt; int table_cols, pages, page_shift;
+  int tile_rows, head_tiles, walkers, slot_pairs, least, unit, uncut, whole;
   int splits, own_splits;       // workgroups the keys are split among (a decode step's prefix; each row's own keys)
   int tiles;                    // tiles of pairs (a decode step's prefix)
   int parts;                    // parts a pair (1: the kernel writes o)
@@ -53,6 +62,7 @@ struct SeqItem {
   int kvh, split, splits, part;
   int64_t prefix, own; int shared;  // key k's cache row: prefix + k below shared, own + k from there on
   const int32_t* table;             // (pages) the sequence's
+  int t0, t1, slot;                 // (pages) the tiles of keys from t0 to t1 alone, into this part (-1: all there are, into o)
   int place0, step;                 // pair p sees keys 0 .. place0 + step (p / rep) of them; step -1: each row's own count
 };
 
@@ -94,11 +104,11 @@ __device__ inline bool seq_item(const SeqArgs& a, SeqItem& it) {
   } else {
     it.split = it.part = blk % a.splits; it.splits = a.splits;
     const int tile = blk / a.splits, lane = threadIdx.x & 63;
-    const int prefix = FORM != SEQ_PAGED && a.shared ? a.prefix_row[0] : 0;
+    const int prefix = a.shared ? a.prefix_row[0] : 0;
     int before = 0;
     for (int s0 = 0; s0 < a.n; s0 += 64) {  // 64 sequences a round: the one whose tiles hold this one
       const int s = min(s0 + lane, a.n - 1);
-      const int st = a.starts[s], en = a.starts[s + 1], place = a.places[s], first = FORM == SEQ_PAGED ? 0 : a.first_row[s], shd = FORM != SEQ_PAGED && a.shared ? a.shared[s] : 0;
+      const int st = a.starts[s], en = a.starts[s + 1], place = a.places[s], first = a.first_row[s], shd = a.shared ? a.shared[s] : 0;
       const int lo = clampi(st, 0, a.rows), len = s0 + lane < a.n ? clampi(en, lo, a.rows) - lo : 0;
       const int tiles = (int)(((int64_t)len * a.rep + BQ - 1) / BQ);
       int incl = tiles;
@@ -113,8 +123,7 @@ __device__ inline bool seq_item(const SeqArgs& a, SeqItem& it) {
         const int nt = __builtin_amdgcn_readlane(tiles, at), in = __builtin_amdgcn_readlane(incl, at);
         const int t = nt - 1 - (tile - (before + in - nt));  // (a sequence's longest tile first)
         it.row0 = __builtin_amdgcn_readlane(lo, at); it.pair0 = t * BQ; it.pairs = __builtin_amdgcn_readlane(len, at) * a.rep;
-        if constexpr (FORM == SEQ_PAGED) it.table = a.tables + (int64_t)(s0 + at) * a.ldt;
-        it.shared = FORM != SEQ_PAGED && a.shared ? clampi(__builtin_amdgcn_readlane(shd, at), 0, a.max_prefix) : 0;
+        it.shared = a.shared ? clampi(__builtin_amdgcn_readlane(shd, at), 0, a.max_prefix) : 0;
         it.prefix = prefix;
         it.own = (int64_t)__builtin_amdgcn_readlane(first, at) - it.shared;
         it.place0 = __builtin_amdgcn_readlane(place, at); it.step = 1;
@@ -142,6 +151,92 @@ __device__ inline int wave_most(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
+// Rows over pages: how the work is shared. A sequence's rows go in tiles of `tile_rows`, each a number of tiles of 64 keys, and a
+// tile's cost is its keys and SEQ_START more (what it takes before its first key and behind its last, in keys; both in units
+// of 2^unit, so that a call's sum stays below 2^30). The tiles of all sequences lie one after another along their cost, and `walkers`
+// workgroups a key head take equal shares of it, so that tokens after few and many places, and prompts' tiles, keep the GPU equally long
+// together. A share that begins or ends inside a tile leaves a part of it, which seq_join_pages joins; one that begins in a tile's first
+// SEQ_START, or anywhere in one that costs less than `uncut`, begins with the tile. For `whole` a workgroup takes a sequence and head as they are. All of it is a function of the arrays alone: a call repeats its bits.
+constexpr int SEQ_START = 128;
+// the sum of a value over this lane and those before
+__device__ inline int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // (within rows of 16 lanes, by 1, 2, 4 and 8)
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // (a row's last lane to the next row, then the lower half's to the upper)
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+struct SeqWalk {
+  int total, share, first;            // `first`: the sequence of held[0]
+  int seq, at, lo, len, place, tiles; // the sequence at hand, the cost before it, its rows and tiles
+  int4* held;                         // (LDS, the wave's own) 64 sequences' rows, places and the cost up to their end
+
+  // the cost of the first t tiles of rows behind `place` places
+  __device__ static int cost(const SeqArgs& a, int place, int t) {
+    return (int)((int64_t)t * ((clampi(place, 0, a.max_own) + SEQ_START) >> a.unit) + (int64_t)t * (t + 1) / 2 * (a.tile_rows >> a.unit));
+  }
+  __device__ static int tiles_of(const SeqArgs& a, int len) { return (len + a.tile_rows - 1) / a.tile_rows; }
+  // sequences s0 .. s0 + 63, behind cost `before`: into LDS; the cost up to the last of them
+  __device__ int load(const SeqArgs& a, int s0, int before) {
+    const int lane = threadIdx.x & 63, i = min(s0 + lane, a.n - 1);
+    const int st = a.starts[i], en = a.starts[i + 1], p = a.places[i];
+    const int l = clampi(st, 0, a.rows), n = s0 + lane < a.n ? clampi(en, l, a.rows) - l : 0;
+    const int end = before + wave_scan(cost(a, p, tiles_of(a, n)));
+    wave_lds_order();
+    held[lane] = make_int4(l, n, p, end);
+    wave_lds_order();
+    first = s0;
+    return __builtin_amdgcn_readlane(end, 63);
+  }
+  __device__ void start(const SeqArgs& a, int4* lds) {
+    held = lds + (threadIdx.x >> 6) * 64;
+    total = load(a, 0, 0);
+    for (int s0 = 64; s0 < a.n; s0 += 64) total = load(a, s0, total);
+    share = max((total + a.walkers - 1) / a.walkers, a.least);
+  }
+  // to the sequence whose tiles hold cost x < total, from the 64 sequences held on: every x is at least the last one sought
+  __device__ void seek(const SeqArgs& a, int x) {
+    for (;;) {
+      const uint64_t has = __ballot(held[threadIdx.x & 63].w > x);
+      if (has) {
+        const int l = __builtin_ctzll(has);
+        const int4 h = held[l];
+        lo = __builtin_amdgcn_readfirstlane(h.x); len = __builtin_amdgcn_readfirstlane(h.y); place = __builtin_amdgcn_readfirstlane(h.z);
+        tiles = tiles_of(a, len);
+        at = __builtin_amdgcn_readfirstlane(h.w) - cost(a, place, tiles);
+        seq = first + l;
+        return;
+      }
+      load(a, first + 64, __builtin_amdgcn_readfirstlane(held[63].w));
+    }
+  }
+  __device__ void seek_from_start(const SeqArgs& a, int x) {
+    if (first > 0) load(a, 0, 0);
+    seek(a, x);
+  }
+  // the tile of the sequence at hand that holds cost x (at <= x)
+  __device__ int tile_at(const SeqArgs& a, int x) const {
+    if (tiles == 1) return 0;
+    const float r = a.tile_rows >> a.unit, b = (float)((clampi(place, 0, a.max_own) + SEQ_START) >> a.unit) + 0.5f * r, y = (float)(x - at);
+    int t = __builtin_amdgcn_readfirstlane(clampi((int64_t)(r > 0.f ? (sqrtf(b * b + 2 * r * y) - b) / r : y / b), 0, tiles - 1));
+    while (t > 0 && at + cost(a, place, t) > x) --t;
+    while (t + 1 < tiles && at + cost(a, place, t + 1) <= x) ++t;
+    return t;
+  }
+  // tile t's keys, in tiles of `bk`
+  __device__ int key_tiles_of(const SeqArgs& a, int t, int bk) const {
+    return (clampi((int64_t)place + min((t + 1) * a.tile_rows, len), 0, a.max_own) + bk - 1) / bk;
+  }
+  // where cost x cuts a tile whose cost is from c0 to c1: at which of its n tiles of keys
+  __device__ static int cut(const SeqArgs& a, int c0, int c1, int n, int x) {
+    if (x >= c1) return n;
+    const int in = x - c0 - (SEQ_START >> a.unit);
+    return in <= 0 || c1 - c0 < a.uncut ? 0 : min((int)((float)in * ((float)n / (float)(c1 - c0 - (SEQ_START >> a.unit)))), n);
+  }
+};
+
 // the first cache row of the page that the sequence's table names for its place k (a page outside the cache: the nearest)
 __device__ inline int64_t page_row(const SeqArgs& a, int page) { return (int64_t)clampi(page, 0, a.pages - 1) << a.page_shift; }
 template <int FORM>
@@ -151,15 +246,9 @@ __device__ inline int64_t key_row(const SeqArgs& a, const SeqItem& it, int k) {
   return r < 0 ? 0 : r >= a.cache_len ? a.cache_len - 1 : r;
 }
 
-// The row of key min(k, last), k up from the first lane's with all of the wave's in one run of 16 from a multiple of it on, so in
-// one page: its number comes by the scalar unit
-template <int FORM>
-__device__ inline int64_t wave_key_row(const SeqArgs& a, const SeqItem& it, int k, int last) {
-  if constexpr (FORM == SEQ_PAGED) {
-    const int at = min(__builtin_amdgcn_readfirstlane(k), last) >> a.page_shift;
-    const int page = ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)it.table)[min(at, a.table_cols - 1)];
-    return page_row(a, page) + (min(k, last) & ((1 << a.page_shift) - 1));
-  } else return key_row<FORM>(a, it, min(k, last));
+// the page of place k, the same for the wave, by the scalar unit
+__device__ inline int table_page(const SeqArgs& a, const SeqItem& it, int k) {
+  return ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)it.table)[min(__builtin_amdgcn_readfirstlane(k) >> a.page_shift, a.table_cols - 1)];
 }
 
 __device__ inline uint32_t pack2_rne(float lo, float hi) { return bf16_rne_f(lo) | (bf16_rne_f(hi) << 16); }
@@ -240,6 +329,15 @@ __device__ inline float* part_of(const SeqArgs& a, int64_t row, int h, int part,
   return a.part + (((row * a.heads + h) * a.parts) + part) * (hd + 2);
 }
 
+// Where pair p of the item leaves its part (a.parts > 1, or pages' item with a slot), hd + 2 floats
+template <int FORM>
+__device__ inline bool seq_parts(const SeqArgs& a, const SeqItem& it) { return FORM == SEQ_PAGED ? it.slot >= 0 : a.parts > 1; }
+template <int FORM>
+__device__ inline float* seq_part(const SeqArgs& a, const SeqItem& it, int p, int64_t row, int h, int hd) {
+  if constexpr (FORM == SEQ_PAGED) return a.part + ((int64_t)it.slot * a.slot_pairs + (p - it.pair0)) * (hd + 2);
+  else return part_of(a, row, h, it.part, hd);
+}
+
 // The wave's pairs again, one at a time over the keys k0 .. k1 - 1 that each sees and no other: a lane a key's score, then a
 // lane HD / 64 dimensions of p v.
 template <int HD, int CF, int FORM>
@@ -269,8 +367,8 @@ __device__ void attend_again(const SeqArgs& a, const SeqItem& it, int wpair, int
         for (int d = 0; d < HD / 64; ++d) o[d] = fmaf(pj, cache_value<HD, CF>(a, r, lane + 64 * d), o[d]);
       }
     }
-    if (a.parts > 1) {
-      float* pp = part_of(a, row, h, it.part, HD);
+    if (seq_parts<FORM>(a, it)) {
+      float* pp = seq_part<FORM>(a, it, p, row, h, HD);
       for (int d = 0; d < HD / 64; ++d) pp[lane + 64 * d] = o[d];
       if (lane == 0) { pp[HD] = m; pp[HD + 1] = m == -INFINITY && end > k0 ? 1.f : l; }
     } else {
@@ -297,8 +395,8 @@ __device__ inline void seq_finish(const SeqArgs& a, const SeqItem& it, int wpair
   if (p >= it.pairs) return;
   const int64_t row = it.row0 + p / a.rep;
   const int h = it.kvh * a.rep + p % a.rep;
-  if (a.parts > 1) {
-    float* pp = part_of(a, row, h, it.part, HD);
+  if (seq_parts<FORM>(a, it)) {
+    float* pp = seq_part<FORM>(a, it, p, row, h, HD);
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
@@ -364,8 +462,7 @@ __device__ inline void seq_softmax(floatx16* s, int k0, int limit, int wave_min,
 // (seq_meet).
 #define SEQ_BEGIN(BK, KG, FORM) \
   constexpr int BQ = 32 * SQ_NW / KG, PG = SQ_NW / KG; \
-  SeqItem it; \
-  if (!seq_item<BQ, FORM>(a, it)) return; \
+  (void)PG; \
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ql = lane & 31, hh = lane >> 5; \
   if (it.pair0 >= it.pairs) return; \
   [[maybe_unused]] const int kg = wave / PG; \
@@ -383,7 +480,7 @@ __device__ inline void seq_softmax(floatx16* s, int k0, int limit, int wave_min,
   wave_min = __builtin_amdgcn_readfirstlane(wave_min); wave_max = __builtin_amdgcn_readfirstlane(wave_max); keys = __builtin_amdgcn_readfirstlane(keys); \
   if (wpair >= it.pairs) wave_max = 0; \
   const int ntiles = (keys + BK - 1) / BK; \
-  const int t0 = (int)((int64_t)ntiles * it.split / it.splits), t1 = (int)((int64_t)ntiles * (it.split + 1) / it.splits); \
+  const int t0 = FORM == SEQ_PAGED ? it.t0 : (int)((int64_t)ntiles * it.split / it.splits), t1 = FORM == SEQ_PAGED ? it.t1 : (int)((int64_t)ntiles * (it.split + 1) / it.splits); \
   const int64_t qat = (it.row0 + pair / a.rep) * a.ldq + (int64_t)(it.kvh * a.rep + pair % a.rep) * HD; \
   const float scale2 = a.scale * 1.44269504088896341f; \
   const int64_t kplane = (int64_t)it.kvh * a.cache_len, vplane = (int64_t)(a.kv_heads + it.kvh) * a.cache_len; \
@@ -445,11 +542,10 @@ struct SeqTile {
 
 // QT, PT: the bf16 terms of q and of the weights; KG: the groups of waves that share a tile's keys; FORM: which entry point's
 template <int HD, int CF, int QT, int PT, int KG, int FORM>
-__global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf16_kernel(SeqArgs a) {
+__device__ __forceinline__ void seq_bf16_item(const SeqArgs& a, const SeqItem& it, uint16_t* tiles) {
   constexpr bool ASYNC = CF == FH_BF16;
   using Tile = SeqTile<HD, ASYNC>;
   constexpr int BK = 64, KLD = Tile::KLD, VLD = Tile::VLD, NS = Tile::STAGES;
-  __shared__ __attribute__((aligned(256))) uint16_t tiles[NS * Tile::SIZE];
   SEQ_BEGIN(BK, KG, FORM)
 
   // the lane's q as the product's B: step s holds dimensions 16 s + 8 hh .. + 7, each term
@@ -466,11 +562,49 @@ __global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf
   // a thread's pieces of a tile: rows pr + PSTEP j, unit pu of each (a wave's loads into LDS in order: its rows lie together)
   constexpr int PSTEP = (ASYNC ? 64 : 64 * SQ_NW) / (HD / 8);
   const int pr = ASYNC ? (64 * NP * wave + lane) / (HD / 8) : tid / (HD / 8), pu = lane % (HD / 8);
+  // (pages) a wave's rows that lie together are 16 or fewer of one page, whose number comes by the scalar unit a tile ahead: pages
+  // has those of tile t on their way, load takes them as its base and leaves the next tile's
+  constexpr int NPG = ASYNC ? 1 : NP;
+  [[maybe_unused]] int page[NPG];
+  [[maybe_unused]] const int wrow = __builtin_amdgcn_readfirstlane(pr), mask = (1 << a.page_shift) - 1;
+  auto pages = [&](int t) {
+    if constexpr (FORM == SEQ_PAGED)
+#pragma unroll
+      for (int j = 0; j < NPG; ++j) page[j] = table_page(a, it, min(t * BK + wrow + PSTEP * j, keys - 1));
+  };
   auto load = [&](int t, int b) {  // tile t's loads: into buffer b, or into registers
     const int k0 = t * BK;
+    if constexpr (FORM == SEQ_PAGED) {
+      const bool end = k0 + BK > keys;  // (rows behind the last key: its row again)
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        const int first = k0 + wrow + (ASYNC ? 0 : PSTEP * j);  // the wave's first key of the page
+        const int64_t base = page_row(a, page[ASYNC ? 0 : j]);
+        const int r = pr + PSTEP * j;
+        if (ASYNC && !end) {
+          const char* kb = (const char*)a.cache + (kplane + base + (first & mask)) * (HD * 2);
+          const char* vb = (const char*)a.cache + (vplane + base + (first & mask)) * (HD * 2);
+          uint16_t* to = tiles + b * Tile::SIZE + 512 * (NP * wave + j);
+          load_to_lds(kb, (uint32_t)((r - wrow) * HD * 2 + 16 * (pu ^ Tile::kswap(r))), to);
+          load_to_lds(vb, (uint32_t)((r - wrow) * HD * 2 + 16 * (pu ^ Tile::vswap(r))), to + BK * HD);
+          continue;
+        }
+        const int64_t row = base + (min(k0 + r, keys - 1) & mask);
+        if constexpr (ASYNC) {
+          uint16_t* to = tiles + b * Tile::SIZE + 512 * (NP * wave + j);
+          load_to_lds((const uint16_t*)a.cache + (kplane + row) * HD + 8 * (pu ^ Tile::kswap(r)), to);
+          load_to_lds((const uint16_t*)a.cache + (vplane + row) * HD + 8 * (pu ^ Tile::vswap(r)), to + BK * HD);
+        } else {
+          kraw[j] = seq_raw<HD, CF>(a, kplane + row, 8 * pu);
+          vraw[j] = seq_raw<HD, CF>(a, vplane + row, 8 * pu);
+        }
+      }
+      pages(t + 1);
+      return;
+    }
     // the tile's rows run on from its first, as they are, unless the keys end or the prefix ends in it, or it leaves the cache
     const int64_t first = (k0 < it.shared ? it.prefix : it.own) + k0;
-    const bool plain = FORM != SEQ_PAGED && k0 + BK <= keys && (k0 >= it.shared || k0 + BK <= it.shared) && first >= 0 && first + BK <= a.cache_len;
+    const bool plain = k0 + BK <= keys && (k0 >= it.shared || k0 + BK <= it.shared) && first >= 0 && first + BK <= a.cache_len;
     if (ASYNC && plain) {
       const char* kb = (const char*)a.cache + (kplane + first) * (HD * 2);
       const char* vb = (const char*)a.cache + (vplane + first) * (HD * 2);
@@ -486,7 +620,7 @@ __global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
       const int r = pr + PSTEP * j;
-      const int64_t row = plain ? first + r : wave_key_row<FORM>(a, it, k0 + r, keys - 1);
+      const int64_t row = plain ? first + r : key_row<FORM>(a, it, min(k0 + r, keys - 1));
       if constexpr (ASYNC) {
         uint16_t* to = tiles + b * Tile::SIZE + 512 * (NP * wave + j);
         load_to_lds((const uint16_t*)a.cache + (kplane + row) * HD + 8 * (pu ^ Tile::kswap(r)), to);
@@ -509,6 +643,7 @@ __global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf
       }
     }
   };
+  if (t0 < t1) pages(t0);
   // this wave's blocks of 32 keys of the tile in buffer b, whose first key is k0
   constexpr int NB = 2 / KG;
   auto work = [&](int b, int k0) {
@@ -608,20 +743,82 @@ __global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf
     }
   }
   l += __shfl_xor(l, 32, 64);
-  static_assert(KG == 1 || PG * 64 * (HD / 2 + 2) * 4 <= (int)sizeof(tiles), "the key groups' place");
+  static_assert(KG == 1 || PG * 64 * (HD / 2 + 2) * 4 <= NS * Tile::SIZE * 2, "the key groups' place");
   if constexpr (KG > 1)
     if (!seq_meet<HD>((float*)tiles, PG, kg, wave, m, l, acc)) return;
   seq_finish<HD, CF, FORM>(a, it, wpair, limit, t0 * BK, min(t1 * BK, keys), acc, m, l);
 }
 
+// A workgroup's items: its own, or over pages those of its share
+template <int BQ, int BK, int FORM, typename Work>
+__device__ __forceinline__ void seq_items(const SeqArgs& a, Work work) {
+  SeqItem it;
+  if constexpr (FORM != SEQ_PAGED) {
+    if (seq_item<BQ, FORM>(a, it)) work(it);
+  } else {
+    const int heads = a.kv_heads * a.head_tiles, me = blockIdx.x / heads, head = blockIdx.x % heads;
+    it.kvh = head / a.head_tiles;
+    it.split = it.splits = it.part = it.shared = 0; it.prefix = it.own = 0; it.step = 1;
+    __shared__ __attribute__((aligned(16))) int4 held[64 * SQ_NW];
+    SeqWalk w;
+    int t = 0, c0 = 0, x0 = 0, x1 = 0x7FFFFFFF;
+    if (a.whole) {  // a workgroup a sequence
+      const int st = a.starts[me], en = a.starts[me + 1];
+      w.seq = me; w.at = 0; w.place = a.places[me];
+      w.lo = clampi(st, 0, a.rows);
+      w.len = clampi(en, w.lo, a.rows) - w.lo;
+      w.tiles = SeqWalk::tiles_of(a, w.len);
+      if (!w.tiles) return;
+    } else {
+      w.start(a, held);
+      if ((int64_t)me * w.share >= w.total) return;
+      x0 = me * w.share;
+      x1 = (int)min((int64_t)x0 + w.share, (int64_t)w.total);
+      w.seek_from_start(a, x0);
+      t = w.tile_at(a, x0);
+      c0 = w.at + SeqWalk::cost(a, w.place, t);
+    }
+    bool again = false;
+    for (;;) {
+      const int c1 = w.at + SeqWalk::cost(a, w.place, t + 1), n = w.key_tiles_of(a, t, BK);
+      it.t0 = a.whole ? 0 : __builtin_amdgcn_readfirstlane(SeqWalk::cut(a, c0, c1, n, x0));
+      it.t1 = a.whole ? n : __builtin_amdgcn_readfirstlane(SeqWalk::cut(a, c0, c1, n, x1));
+      if (it.t0 < it.t1 || (n == 0 && x1 >= c1)) {
+        if (again) __syncthreads();  // (the last item's tiles are read)
+        again = true;
+        const int row = t * a.tile_rows;
+        it.row0 = w.lo + row;
+        it.pair0 = head % a.head_tiles * BQ;
+        it.pairs = a.head_tiles > 1 ? a.rep : min(a.tile_rows, w.len - row) * a.rep;
+        it.place0 = w.place + row;
+        it.table = a.tables + (int64_t)w.seq * a.ldt;
+        it.slot = it.t0 == 0 && it.t1 == n ? -1 : (int)(blockIdx.x * 2 + (it.t0 == 0));  // (at most two of a share: its first and its last tile)
+        work(it);
+      }
+      if (c1 >= x1) return;
+      c0 = c1;
+      if (++t == w.tiles) {
+        if (a.whole) return;
+        w.seek(a, c1);
+        t = 0;
+      }
+    }
+  }
+}
+
+template <int HD, int CF, int QT, int PT, int KG, int FORM>
+__global__ __launch_bounds__(64 * SQ_NW, HD == 64 && QT < 3 ? 3 : 2) void seq_bf16_kernel(SeqArgs a) {
+  using Tile = SeqTile<HD, CF == FH_BF16>;
+  __shared__ __attribute__((aligned(256))) uint16_t tiles[Tile::STAGES * Tile::SIZE];
+  seq_items<32 * SQ_NW / KG, 64, FORM>(a, [&](const SeqItem& it) { seq_bf16_item<HD, CF, QT, PT, KG, FORM>(a, it, tiles); });
+}
+
 // The same in fp32: 32 keys a tile. A lane's q holds dimensions HD / 2 hh .. of its half (the order of a sum's products is free),
 // so that K's row is read 16 bytes at a time; P's step r multiplies keys 8 (r / 4) + 4 hh + r % 4, V's rows as they lie.
 template <int HD, int FORM>
-__global__ __launch_bounds__(64 * SQ_NW, 2) void seq_f32_kernel(SeqArgs a) {
+__device__ __forceinline__ void seq_f32_item(const SeqArgs& a, const SeqItem& it, float (*Ks)[32 * (HD + 4)], float (*Vs)[32 * (HD + 4)]) {
   constexpr int CF = FH_F32;
   constexpr int BK = 32, LD = HD + 4;
-  __shared__ __attribute__((aligned(16))) float Ks[2][BK * LD];
-  __shared__ __attribute__((aligned(16))) float Vs[2][BK * LD];
   SEQ_BEGIN(BK, 1, FORM)
   float qf[HD / 2];
 #pragma unroll
@@ -633,15 +830,23 @@ __global__ __launch_bounds__(64 * SQ_NW, 2) void seq_f32_kernel(SeqArgs a) {
   }
   constexpr int NP = BK * HD / 8 / (64 * SQ_NW);
   SeqRaw kraw[NP], vraw[NP];
+  [[maybe_unused]] int page[NP];
+  auto pages = [&](int t) {  // (pages) as above
+    if constexpr (FORM == SEQ_PAGED)
+#pragma unroll
+      for (int j = 0; j < NP; ++j) page[j] = table_page(a, it, min(t * BK + (tid + 64 * SQ_NW * j) / (HD / 8), keys - 1));
+  };
   auto load = [&](int t) {
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      const int i = tid + 64 * SQ_NW * j, r = i / (HD / 8), c = (i % (HD / 8)) * 8;
-      const int64_t row = wave_key_row<FORM>(a, it, t * BK + r, keys - 1);
+      const int i = tid + 64 * SQ_NW * j, r = i / (HD / 8), c = (i % (HD / 8)) * 8, k = min(t * BK + r, keys - 1);
+      const int64_t row = FORM == SEQ_PAGED ? page_row(a, page[j]) + (k & ((1 << a.page_shift) - 1)) : key_row<FORM>(a, it, k);
       kraw[j] = seq_raw<HD, CF>(a, kplane + row, c);
       vraw[j] = seq_raw<HD, CF>(a, vplane + row, c);
     }
+    pages(t + 1);
   };
+  if (t0 < t1) pages(t0);
   auto store = [&](int b) {
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
@@ -683,6 +888,13 @@ __global__ __launch_bounds__(64 * SQ_NW, 2) void seq_f32_kernel(SeqArgs a) {
   }
   l += __shfl_xor(l, 32, 64);
   seq_finish<HD, CF, FORM>(a, it, wpair, limit, t0 * BK, min(t1 * BK, keys), acc, m, l);
+}
+
+template <int HD, int FORM>
+__global__ __launch_bounds__(64 * SQ_NW, 2) void seq_f32_kernel(SeqArgs a) {
+  __shared__ __attribute__((aligned(16))) float Ks[2][32 * (HD + 4)];
+  __shared__ __attribute__((aligned(16))) float Vs[2][32 * (HD + 4)];
+  seq_items<32 * SQ_NW, 32, FORM>(a, [&](const SeqItem& it) { seq_f32_item<HD, FORM>(a, it, Ks, Vs); });
 }
 
 // A pair's parts joined, a wave a pair: lane p holds part p's statistics, then a lane HD / 64 dimensions of each part's sum,
@@ -733,6 +945,112 @@ __global__ __launch_bounds__(256) void seq_join(SeqArgs a) {
   }
 }
 
+// The parts of a tile that shares cut, joined as above: a workgroup a cut, which takes the tile whose first cut it is. TOKENS: few
+// pairs of many parts, a wave a pair; otherwise HD / 4 lanes a pair, 4 parts on their way at a time.
+template <int HD, int BK, bool TOKENS>
+__global__ __launch_bounds__(TOKENS ? 512 : 1024) void seq_join_pages(SeqArgs a) {
+  constexpr int NT = TOKENS ? 512 : 1024;
+  __shared__ __attribute__((aligned(16))) int4 held[NT];
+  const int heads = a.kv_heads * a.head_tiles, head = blockIdx.x % heads, first = blockIdx.x / heads;  // the share before the cut
+  SeqWalk w;
+  w.start(a, held);
+  if ((int64_t)(first + 1) * w.share >= w.total) return;
+  const int x = (first + 1) * w.share;
+  w.seek_from_start(a, x);
+  const int t = w.tile_at(a, x), n = w.key_tiles_of(a, t, BK);
+  const int c0 = w.at + SeqWalk::cost(a, w.place, t), c1 = w.at + SeqWalk::cost(a, w.place, t + 1);
+  auto cut = [&](int i) { return SeqWalk::cut(a, c0, c1, n, (int)min((int64_t)i * w.share, (int64_t)w.total)); };  // where share i begins
+  const int k = cut(first + 1);
+  if (k <= 0 || k >= n || cut(first) > 0) return;
+  // the parts: of share `first`, from the tile's first key on, and of those behind it up to the one that ends it
+  int last = first + 1;
+  while (cut(last + 1) < n) ++last;
+  const int parts = last - first + 1, lane = threadIdx.x & 63, row = t * a.tile_rows;
+  const int pair0 = head % a.head_tiles * a.slot_pairs, pairs = min(a.slot_pairs, (a.head_tiles > 1 ? a.rep : min(a.tile_rows, w.len - row) * a.rep) - pair0);
+  auto part = [&](int i, int p) { return a.part + ((int64_t)(((first + i) * heads + head) * 2 + (i == 0)) * a.slot_pairs + p) * (HD + 2); };
+  auto some_of = [&](int i) { return cut(first + i) < cut(first + i + 1); };  // (a share may get no key of the tile)
+  auto put_at = [&](int p, int d) {
+    return (int64_t)(w.lo + row + (pair0 + p) / a.rep) * a.ldo + (int64_t)(head / a.head_tiles * a.rep + (pair0 + p) % a.rep) * HD + d;
+  };
+  constexpr int D = TOKENS ? HD / 64 : 4, L = HD / D;  // a lane's dimensions, a pair's lanes
+  for (int p = threadIdx.x / L; p < pairs; p += NT / L) {
+    float top = -INFINITY, den = 0.f, o[D];
+    bool any = false;
+#pragma unroll
+    for (int d = 0; d < D; ++d) o[d] = 0.f;
+    const int d0 = threadIdx.x % L * D;
+    if constexpr (TOKENS) {
+      for (int i0 = 0; i0 < parts; i0 += 64) {
+        const bool in = i0 + lane < parts && some_of(i0 + lane);
+        const float2 st = in ? *(const float2*)(part(i0 + lane, p) + HD) : make_float2(-INFINITY, 0.f);
+        const float now = fmaxf(top, wave_max(st.x));
+        const bool none = st.y == 0.f && st.x == -INFINITY;
+        const float f = any ? __builtin_amdgcn_exp2f(top - now) : 0.f;
+        const float wt = none ? 0.f : __builtin_amdgcn_exp2f(st.x - now);
+        den = (any ? den * f : 0.f) + wave_sum(none ? 0.f : wt * st.y);
+#pragma unroll
+        for (int d = 0; d < D; ++d) o[d] = any ? o[d] * f : 0.f;
+        const uint64_t some = __ballot(!none && in);
+        for (int i = 0; i < min(64, parts - i0); i += 8) {
+          float v[8][D];
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int d = 0; d < D; ++d) v[u][d] = part(min(i0 + i + u, parts - 1), p)[d0 + d];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const float wp = __shfl(wt, (i + u) & 63, 64);
+            if (some >> ((i + u) & 63) & 1)
+#pragma unroll
+              for (int d = 0; d < D; ++d) o[d] = fmaf(wp, v[u][d], o[d]);
+          }
+        }
+        any = any || some;
+        top = now;
+      }
+    } else {
+      for (int i0 = 0; i0 < parts; i0 += 4) {
+        float2 st[4], v[4][2];
+        bool some[4];
+        float now = top;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float* pp = part(min(i0 + u, parts - 1), p);
+          st[u] = *(const float2*)(pp + HD);
+          v[u][0] = *(const float2*)(pp + d0); v[u][1] = *(const float2*)(pp + d0 + 2);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          some[u] = i0 + u < parts && some_of(i0 + u) && !(st[u].y == 0.f && st[u].x == -INFINITY);
+          if (some[u]) now = fmaxf(now, st[u].x);
+        }
+        if (any) {
+          const float f = __builtin_amdgcn_exp2f(top - now);
+          den *= f;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) o[d] *= f;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (some[u]) {
+            const float wt = __builtin_amdgcn_exp2f(st[u].x - now);
+            den = fmaf(wt, st[u].y, den);
+            o[0] = fmaf(wt, v[u][0].x, o[0]); o[1] = fmaf(wt, v[u][0].y, o[1]); o[2] = fmaf(wt, v[u][1].x, o[2]); o[3] = fmaf(wt, v[u][1].y, o[3]);
+            any = true;
+          }
+        top = now;
+      }
+    }
+    const float inv = any ? 1.f / den : 0.f;
+    const int64_t at = put_at(p, d0);
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (a.o_bf16) ((uint16_t*)a.o)[at + d] = (uint16_t)bf16_rne_f(o[d] * inv);
+      else ((float*)a.o)[at + d] = o[d] * inv;
+    }
+  }
+}
+
 template <int HD, int CF, int KG, int FORM>
 static void launch_seq(unsigned blocks, hipStream_t s, const SeqArgs& a) {
   const dim3 g(blocks), b(64 * SQ_NW);
@@ -763,7 +1081,15 @@ static void launch_seq(int cf, int pairs, unsigned blocks, hipStream_t s, const 
     case FH_BFP8: launch_seq<HD, FH_BFP8, PAGES>(pairs, blocks, s, a); break;
     default: launch_seq<HD, FH_BFP4, PAGES>(pairs, blocks, s, a); break;
   }
-  if (a.parts > 1) hipLaunchKernelGGL(seq_join<HD>, dim3((unsigned)((a.rows * a.heads + 3) / 4)), dim3(256), 0, s, a);
+  if constexpr (PAGES) {
+    const dim3 g((unsigned)((a.walkers - 1) * a.kv_heads * a.head_tiles));
+    const bool tokens = pairs == 64;
+    if (a.parts > 1) {
+      if (cf == FH_F32) hipLaunchKernelGGL((seq_join_pages<HD, 32, false>), g, dim3(1024), 0, s, a);
+      else if (tokens) hipLaunchKernelGGL((seq_join_pages<HD, 64, true>), g, dim3(512), 0, s, a);
+      else hipLaunchKernelGGL((seq_join_pages<HD, 64, false>), g, dim3(1024), 0, s, a);
+    }
+  } else if (a.parts > 1) hipLaunchKernelGGL(seq_join<HD>, dim3((unsigned)((a.rows * a.heads + 3) / 4)), dim3(256), 0, s, a);
 }
 
 template <bool PAGES>

@@ -190,7 +190,7 @@ def test_repeats_streams_and_graphs(cuda):
   one, many = ints(range(n + 1)), ints([0, 2, 5, 5, 6, 20, 21, 22, 39, 40])
   spots = [ints(rng.integers(0, 600, n)) for _ in range(3)]
   tabs = [torch.from_numpy(rng.permutation(400)[:n * 40].reshape(n, 40).astype(np.int32)).cuda() for _ in range(3)]
-  ws = torch.full((1 << 24,), 255, dtype=torch.uint8, device="cuda")  # (NaN bytes)
+  ws = ops().attention_paged_workspace(40, n, heads, kv, hd, 640).fill_(255)  # (NaN bytes)
   dec = lambda p, t, o: ops().attention_paged(q[:n], cache, heads, kv, hd, one, p, t, 16, 640, workspace=ws, o=o)
   pre = lambda p, t, o: ops().attention_paged(q, cache, heads, kv, hd, many, p, t, 16, 640, workspace=ws, o=o)
   eager = [(dec(a, t, None).clone(), pre(a, t, None).clone()) for a, t in zip(spots, tabs)]
