@@ -21,7 +21,7 @@ typedef __attribute__((__vector_size__(4 * sizeof(float)))) float lr_floatx4;
 
 constexpr int LR_ROWS = 64;        // rows a tile
 constexpr int LR_WAVES = 4;
-constexpr int LR_COLS = 64;        // columns of u a workgroup of the first kernel
+constexpr int LR_WIDTH = 256;      // columns of y a workgroup of the second: 512 is 3% faster for 4096 rows, 12% slower for 500
 constexpr int LR_MAX_PARTS = 4;    // parts of a fused projection
 constexpr int LR_MAX_RANK = 128;
 
@@ -48,22 +48,40 @@ __device__ inline void lr_terms(const float (&x)[8], lr_bf16x8 (&t)[N]) {
   }
 }
 
-// 8 values from p + at as N bf16 terms (bf16 ones: one); zeros where not `in` (at is inside the buffer all the same)
-template <bool BF, int N>
-__device__ inline void lr_load(const void* p, int64_t at, bool in, lr_bf16x8 (&t)[N]) {
-  if constexpr (BF) {
-    uint4 w = *(const uint4*)((const uint16_t*)p + at);
-    if (!in) w = make_uint4(0, 0, 0, 0);
-    t[0] = *(const lr_bf16x8*)&w;
-  } else {
-    const float4 a = *(const float4*)((const float*)p + at), b = *(const float4*)((const float*)p + at + 4);
-    float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    if (!in)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = 0.f;
-    lr_terms<N>(f, t);
+// 8 values as loaded, and as N bf16 terms (bf16 ones: one); zeros where not `in` (what was loaded is inside the buffer all the same)
+template <bool BF>
+struct LrRaw {
+  uint4 a, b;
+  __device__ void load(const void* p, int64_t at) {
+    if constexpr (BF) a = *(const uint4*)((const uint16_t*)p + at);
+    else { a = *(const uint4*)((const float*)p + at); b = *(const uint4*)((const float*)p + at + 4); }
   }
-}
+  __device__ void values(float (&f)[8]) const {
+    if constexpr (BF) {
+      const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(u[i] << 16); f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u); }
+    } else {
+      const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(u[i]);
+    }
+  }
+  template <int N>
+  __device__ void terms(bool in, lr_bf16x8 (&t)[N]) const {
+    if constexpr (BF) {
+      const uint4 w = in ? a : make_uint4(0, 0, 0, 0);
+      t[0] = *(const lr_bf16x8*)&w;
+    } else {
+      float f[8];
+      values(f);
+      if (!in)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = 0.f;
+      lr_terms<N>(f, t);
+    }
+  }
+};
 
 // the products of two operands in terms that matter: those whose terms' places sum to less than the longer operand's count
 template <int NA, int NB>
@@ -111,87 +129,91 @@ __device__ inline int lr_nth(uint64_t rows, int n) {
   return at;
 }
 
-// u[part][row][c] = the part of K's products of x's row and A's row c
-template <bool XB, bool WB, int XT, int WT>
-__global__ __launch_bounds__(64 * LR_WAVES) void lora_shrink(LoraArgs a) {
-  __shared__ __attribute__((aligned(16))) float sums[LR_WAVES - 1][LR_ROWS * LR_COLS];
-  const int split = blockIdx.x % a.splits, group = blockIdx.x / a.splits, c0 = group * LR_COLS;
+// A workgroup's part of u for one adapter: MB blocks of 16 rows, CB of 16 columns. A wave takes 64 of K at a time, every load of them on
+// its way before the first product; the waves' sums meet in LDS, in order.
+template <bool XB, bool WB, int XT, int WT, int CB, int MB>
+__device__ __forceinline__ void shrink_rows(const LoraArgs& a, int64_t t0, uint64_t rows, int n, int adapter, int split, int c0, float* sums) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-  const int cols = min(LR_COLS, a.C - c0), cb = (cols + 15) / 16;
+  const int cols = min(16 * CB, a.C - c0);
   const int k0 = split * a.kstep, k1 = (int)min((int64_t)k0 + a.kstep, a.K);
+  lr_floatx4 acc[MB][CB];
+  int64_t xat[MB], wat[CB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i) {
+    xat[i] = (t0 + lr_nth(rows, min(16 * i + r, n - 1))) * a.ldx;
+#pragma unroll
+    for (int j = 0; j < CB; ++j) acc[i][j] = lr_floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll
+  for (int j = 0; j < CB; ++j) wat[j] = ((int64_t)adapter * a.C + c0 + min(16 * j + r, cols - 1)) * a.K;
+  const int kw = (a.kstep / 64 + LR_WAVES - 1) / LR_WAVES * 64, kb = k0 + kw * wave, ke = min(kb + kw, k1);  // the wave's
+  for (int k = kb; k < ke; k += 64) {
+    LrRaw<XB> x[2][MB];
+    LrRaw<WB> w[2][CB];
+    bool in[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int kk = k + 32 * h + 8 * g;
+      in[h] = kk < ke;
+      const int at = in[h] ? kk : 0;
+#pragma unroll
+      for (int j = 0; j < CB; ++j) w[h][j].load(a.a, wat[j] + at);
+#pragma unroll
+      for (int i = 0; i < MB; ++i) x[h][i].load(a.x, xat[i] + at);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      lr_bf16x8 xf[MB][XT];
+#pragma unroll
+      for (int i = 0; i < MB; ++i) x[h][i].template terms<XT>(in[h], xf[i]);
+#pragma unroll
+      for (int j = 0; j < CB; ++j) {
+        lr_bf16x8 wf[WT];
+        w[h][j].template terms<WT>(in[h], wf);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) acc[i][j] = lr_mfma<XT, WT>(xf[i], wf, acc[i][j]);
+      }
+    }
+  }
+  // lane (r, g) holds rows 16 i + 4 g .. + 3 of column 16 j + r; a wave adds up every fourth block
+  constexpr int BLOCKS = MB * CB;
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < CB; ++j) *(lr_floatx4*)(sums + ((wave * BLOCKS + i * CB + j) * 64 + lane) * 4) = acc[i][j];
+  __syncthreads();
+  for (int b = wave; b < BLOCKS; b += LR_WAVES) {
+    const int i = b / CB, j = b % CB;
+    lr_floatx4 v[LR_WAVES];
+#pragma unroll
+    for (int w = 0; w < LR_WAVES; ++w) v[w] = *(const lr_floatx4*)(sums + ((w * BLOCKS + b) * 64 + lane) * 4);
+    const lr_floatx4 t = v[0] + v[1] + v[2] + v[3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int m = 16 * i + 4 * g + e;
+      if (m < n && 16 * j + r < cols) a.u[((int64_t)split * a.rows + t0 + lr_nth(rows, m)) * a.C + c0 + 16 * j + r] = t[e];
+    }
+  }
+  __syncthreads();  // (sums are read)
+}
+
+// u[part][row][c] = the part of K's products of x's row and A's row c
+template <bool XB, bool WB, int XT, int WT, int CB>
+__global__ __launch_bounds__(64 * LR_WAVES) void lora_shrink(LoraArgs a) {
+  __shared__ __attribute__((aligned(16))) float sums[LR_WAVES * 4 * CB * 256];
+  const int split = blockIdx.x % a.splits, c0 = blockIdx.x / a.splits * 16 * CB;
   LoraTile tile(a, blockIdx.z);
   int adapter;
   uint64_t rows;
   while (tile.next(a.share, blockIdx.y, adapter, rows)) {
     if (adapter < 0) continue;
-    const int n = __builtin_popcountll(rows), mb = (n + 15) / 16;
-    const int64_t wbase = (int64_t)adapter * a.C * a.K;
-    lr_floatx4 acc[4][4];
-    int64_t xat[4], wat[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      xat[i] = (tile.t0 + lr_nth(rows, min(16 * i + r, n - 1))) * a.ldx;
-      wat[i] = wbase + (int64_t)(c0 + min(16 * i + r, cols - 1)) * a.K;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = lr_floatx4{0.f, 0.f, 0.f, 0.f};
-    }
-    for (int k = k0 + 64 * wave; k < k1; k += 64 * LR_WAVES)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int kk = k + 32 * h + 8 * g;
-        const bool in = kk < k1;
-        const int at = in ? kk : 0;
-        lr_bf16x8 xf[4][XT];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < mb) lr_load<XB, XT>(a.x, xat[i] + at, in, xf[i]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j < cb) {
-            lr_bf16x8 wf[WT];
-            lr_load<WB, WT>(a.a, wat[j] + at, in, wf);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (i < mb) acc[i][j] = lr_mfma<XT, WT>(xf[i], wf, acc[i][j]);
-          }
-      }
-    // the waves' sums, in order; lane (r, g) holds rows 16 i + 4 g .. + 3 of column 16 j + r
-    if (wave > 0)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (i < mb && j < cb) *(lr_floatx4*)&sums[wave - 1][((i * 4 + j) * 64 + lane) * 4] = acc[i][j];
-    __syncthreads();
-    if (wave == 0)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (i < mb && j < cb) {
-#pragma unroll
-            for (int w = 0; w < LR_WAVES - 1; ++w) acc[i][j] += *(const lr_floatx4*)&sums[w][((i * 4 + j) * 64 + lane) * 4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int m = 16 * i + 4 * g + e, c = 16 * j + r;
-              if (m < n && c < cols) a.u[((int64_t)split * a.rows + tile.t0 + lr_nth(rows, m)) * a.C + c0 + c] = acc[i][j][e];
-            }
-          }
-    __syncthreads();
+    const int n = __builtin_popcountll(rows);
+    if (n <= 16) shrink_rows<XB, WB, XT, WT, CB, 1>(a, tile.t0, rows, n, adapter, split, c0, sums);
+    else if (n <= 32) shrink_rows<XB, WB, XT, WT, CB, 2>(a, tile.t0, rows, n, adapter, split, c0, sums);
+    else shrink_rows<XB, WB, XT, WT, CB, 4>(a, tile.t0, rows, n, adapter, split, c0, sums);
   }
 }
 
-__device__ inline void lr_read8(const void* p, bool bf, int64_t at, float (&f)[8]) {
-  if (bf) {
-    const uint4 w = *(const uint4*)((const uint16_t*)p + at);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(u[i] << 16); f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u); }
-  } else {
-    const float4 u = *(const float4*)((const float*)p + at), v = *(const float4*)((const float*)p + at + 4);
-    f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w; f[4] = v.x; f[5] = v.y; f[6] = v.z; f[7] = v.w;
-  }
-}
 template <bool BF>
 __device__ inline void lr_write8(void* p, int64_t at, const float (&f)[8]) {
   if constexpr (BF) {
@@ -205,20 +227,113 @@ __device__ inline void lr_write8(void* p, int64_t at, const float (&f)[8]) {
   }
 }
 
-// y = residual + scale u B^T: a workgroup a chunk of a part's columns. B's rows are the product's rows and x's rows its
-// columns: two blocks of 16 of B's rows are rows 8 (r / 4) + r % 4 and those 4 on, so that a lane ends with 8 consecutive columns of
-// y's row, 16 or 32 bytes.
-template <bool WB, bool YB, int UT, int WT>
-__global__ __launch_bounds__(64 * LR_WAVES) void lora_expand(LoraArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint16_t us[];  // [UT][64][ldu] u's terms
+// u of an adapter's rows in LDS as terms: 8 of a row's at a time, the parts of K in order, 8 of them on their way
+template <int UT>
+__device__ __forceinline__ void expand_u(const LoraArgs& a, int64_t t0, uint64_t rows, int n, int adapter, int part, uint16_t* us, int ldu) {
+  const int steps = (a.rank + 31) / 32;
+  const float sc = a.scale ? a.scale[adapter] : 1.f;
+  for (int i = threadIdx.x; i < n * 4 * steps; i += 64 * LR_WAVES) {
+    const int m = i / (4 * steps), k = i % (4 * steps) * 8;
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (k < a.rank) {
+      const float* p = a.u + (t0 + lr_nth(rows, m)) * a.C + part * a.rank + k;
+      for (int s = 0; s < a.splits; s += 8) {
+        LrRaw<false> v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e].load(p, min(s + e, a.splits - 1) * a.rows * a.C);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float w[8];
+          v[e].values(w);
+          if (s + e < a.splits)
+#pragma unroll
+            for (int d = 0; d < 8; ++d) f[d] += w[d];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= sc;
+    }
+    lr_bf16x8 t[UT];
+    lr_terms<UT>(f, t);
+#pragma unroll
+    for (int e = 0; e < UT; ++e) *(lr_bf16x8*)(us + (e * LR_ROWS + m) * ldu + k) = t[e];
+  }
+}
+
+// One adapter's rows, the chunk's columns n0 .. n1: y = residual + u B^T, MB blocks of 16 rows at a time. A wave takes whole 128-byte lines of
+// each row. B's rows are the product's rows and x's its columns: two blocks of 16 of B's rows are rows 8 (r / 4) + r % 4 and those 4
+// on, so that a lane ends with 8 consecutive columns of y's row, 16 or 32 bytes.
+template <bool WB, bool YB, int UT, int WT, int MB>
+__device__ __forceinline__ void expand_rows(const LoraArgs& a, int64_t t0, uint64_t rows, int n, int adapter, int n0, int n1, const uint16_t* us, int ldu) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+  const int steps = (a.rank + 31) / 32;
+  constexpr int CG = YB ? 2 : 1;
+  const int64_t wbase = (int64_t)adapter * a.N * a.rank;
+  for (int m0 = 0; m0 < n; m0 += 16 * MB) {
+    int64_t row[MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) row[i] = t0 + lr_nth(rows, min(m0 + 16 * i + r, n - 1));
+    for (int c = n0 + 32 * CG * wave; c < n1; c += 32 * CG * LR_WAVES) {
+      LrRaw<YB> res[MB][CG];
+      if (a.residual)
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int q = 0; q < CG; ++q) res[i][q].load(a.residual, row[i] * a.ldr + min(c + 32 * q + 8 * g, n1 - 8));
+      lr_floatx4 acc[MB][CG][2];
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int q = 0; q < CG; ++q) acc[i][q][0] = acc[i][q][1] = lr_floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < steps; ++s) {
+        const int k = 32 * s + 8 * g;
+        LrRaw<WB> b[CG][2];
+#pragma unroll
+        for (int q = 0; q < CG; ++q)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) b[q][e].load(a.b, wbase + (int64_t)min(c + 32 * q + 8 * (r >> 2) + 4 * e + (r & 3), n1 - 1) * a.rank + (k < a.rank ? k : 0));
+        lr_bf16x8 uf[MB][UT];
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int e = 0; e < UT; ++e) uf[i][e] = *(const lr_bf16x8*)(us + (e * LR_ROWS + min(m0 + 16 * i + r, n - 1)) * ldu + k);
+#pragma unroll
+        for (int q = 0; q < CG; ++q)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            lr_bf16x8 bf[WT];
+            b[q][e].template terms<WT>(k < a.rank, bf);
+#pragma unroll
+            for (int i = 0; i < MB; ++i) acc[i][q][e] = lr_mfma<WT, UT>(bf, uf[i], acc[i][q][e]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int q = 0; q < CG; ++q) {
+          const int col = c + 32 * q + 8 * g;  // the lane's 8 columns of y
+          float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          if (a.residual) res[i][q].values(f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] += acc[i][q][e >> 2][e & 3];
+          if (m0 + 16 * i + r < n && col < n1) lr_write8<YB>(a.y, row[i] * a.ldy + col, f);
+        }
+    }
+  }
+}
+
+// y = residual + scale u B^T: a workgroup a chunk of a part's columns
+template <bool WB, bool YB, int UT, int WT>
+__global__ __launch_bounds__(64 * LR_WAVES, WB ? 4 : 3) void lora_expand(LoraArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint16_t us[];  // [UT][64][ldu] u's terms
   int part = 0;
   while (part + 1 < a.parts && (int)blockIdx.x >= a.chunk0[part + 1]) ++part;
   const int n0 = a.col0[part] + (blockIdx.x - a.chunk0[part]) * a.width, n1 = min(n0 + a.width, a.col0[part + 1]);
-  const int steps = (a.rank + 31) / 32, ldu = 32 * steps + 8;
+  const int ldu = 32 * ((a.rank + 31) / 32) + 8;
   LoraTile tile(a, blockIdx.z);
   int adapter;
   uint64_t rows;
+  bool again = false;
   while (tile.next(a.share, blockIdx.y, adapter, rows)) {
     const int n = __builtin_popcountll(rows);
     if (adapter < 0) {  // the residual, or zeros
@@ -227,69 +342,21 @@ __global__ __launch_bounds__(64 * LR_WAVES) void lora_expand(LoraArgs a) {
       for (int i = threadIdx.x; i < n * pieces; i += 64 * LR_WAVES) {
         const int64_t t = tile.t0 + lr_nth(rows, i / pieces), c = n0 + i % pieces * 8;
         float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (a.residual) lr_read8(a.residual, YB, t * a.ldr + c, f);
+        if (a.residual) {
+          LrRaw<YB> x;
+          x.load(a.residual, t * a.ldr + c);
+          x.values(f);
+        }
         lr_write8<YB>(a.y, t * a.ldy + c, f);
       }
       continue;
     }
-    __syncthreads();  // (the last adapter's u is read)
-    const float sc = a.scale ? a.scale[adapter] : 1.f;
-    for (int i = threadIdx.x; i < n * 4 * steps; i += 64 * LR_WAVES) {  // 8 of a row's u at a time: the parts of K, in order
-      const int m = i / (4 * steps), k = i % (4 * steps) * 8;
-      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (k < a.rank) {
-        const float* p = a.u + (tile.t0 + lr_nth(rows, m)) * a.C + part * a.rank + k;
-        for (int s = 0; s < a.splits; ++s, p += a.rows * a.C) {
-          const float4 v = *(const float4*)p, w = *(const float4*)(p + 4);
-          f[0] += v.x; f[1] += v.y; f[2] += v.z; f[3] += v.w; f[4] += w.x; f[5] += w.y; f[6] += w.z; f[7] += w.w;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= sc;
-      }
-      lr_bf16x8 t[UT];
-      lr_terms<UT>(f, t);
-#pragma unroll
-      for (int e = 0; e < UT; ++e) *(lr_bf16x8*)(us + (e * LR_ROWS + m) * ldu + k) = t[e];
-    }
+    if (again) __syncthreads();  // (the last adapter's u is read)
+    again = true;
+    expand_u<UT>(a, tile.t0, rows, n, adapter, part, us, ldu);
     __syncthreads();
-    const int mb = (n + 15) / 16;
-    int64_t row[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) row[i] = tile.t0 + lr_nth(rows, min(16 * i + r, n - 1));
-    const int64_t wbase = (int64_t)adapter * a.N * a.rank;
-    for (int c = n0 + 32 * wave; c < n1; c += 32 * LR_WAVES) {
-      const int col = c + 8 * g;  // the lane's 8 columns of y
-      const int64_t w0 = wbase + (int64_t)min(c + 8 * (r >> 2) + (r & 3), n1 - 1) * a.rank;
-      const int64_t w1 = wbase + (int64_t)min(c + 8 * (r >> 2) + 4 + (r & 3), n1 - 1) * a.rank;
-      lr_floatx4 acc[4][2];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = lr_floatx4{0.f, 0.f, 0.f, 0.f};
-      for (int s = 0; s < steps; ++s) {
-        const int k = 32 * s + 8 * g;
-        const bool in = k < a.rank;
-        lr_bf16x8 b0[WT], b1[WT];
-        lr_load<WB, WT>(a.b, w0 + (in ? k : 0), in, b0);
-        lr_load<WB, WT>(a.b, w1 + (in ? k : 0), in, b1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < mb) {
-            lr_bf16x8 uf[UT];
-#pragma unroll
-            for (int e = 0; e < UT; ++e) uf[e] = *(const lr_bf16x8*)(us + (e * LR_ROWS + min(16 * i + r, n - 1)) * ldu + k);
-            acc[i][0] = lr_mfma<WT, UT>(b0, uf, acc[i][0]);
-            acc[i][1] = lr_mfma<WT, UT>(b1, uf, acc[i][1]);
-          }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (16 * i + r < n && col < n1) {
-          float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          if (a.residual) lr_read8(a.residual, YB, row[i] * a.ldr + col, f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] += acc[i][e >> 2][e & 3];
-          lr_write8<YB>(a.y, row[i] * a.ldy + col, f);
-        }
-    }
+    if (n <= 16) expand_rows<WB, YB, UT, WT, 1>(a, tile.t0, rows, n, adapter, n0, n1, us, ldu);
+    else expand_rows<WB, YB, UT, WT, 2>(a, tile.t0, rows, n, adapter, n0, n1, us, ldu);
   }
 }
 
@@ -305,8 +372,15 @@ static int lora_splits(int64_t rows, int64_t K) {
 template <bool XB, bool WB, bool YB>
 static void launch_lora(hipStream_t s, const LoraArgs& a) {
   constexpr int T = YB ? 2 : 3, XT = XB ? 1 : T, WT = WB ? 1 : T;
-  const unsigned tiles = (unsigned)((a.rows + LR_ROWS - 1) / LR_ROWS), groups = (unsigned)((a.C + LR_COLS - 1) / LR_COLS);
-  hipLaunchKernelGGL((lora_shrink<XB, WB, XT, WT>), dim3(a.splits * groups, a.share, tiles), dim3(64 * LR_WAVES), 0, s, a);
+  // u's columns in equal groups of up to 4 blocks of 16
+  const unsigned tiles = (unsigned)((a.rows + LR_ROWS - 1) / LR_ROWS), blocks = (a.C + 15) / 16, groups = (blocks + 3) / 4, cb = (blocks + groups - 1) / groups;
+  const dim3 g(a.splits * groups, a.share, tiles), b(64 * LR_WAVES);
+  switch (cb) {
+    case 1: hipLaunchKernelGGL((lora_shrink<XB, WB, XT, WT, 1>), g, b, 0, s, a); break;
+    case 2: hipLaunchKernelGGL((lora_shrink<XB, WB, XT, WT, 2>), g, b, 0, s, a); break;
+    case 3: hipLaunchKernelGGL((lora_shrink<XB, WB, XT, WT, 3>), g, b, 0, s, a); break;
+    default: hipLaunchKernelGGL((lora_shrink<XB, WB, XT, WT, 4>), g, b, 0, s, a); break;
+  }
   const int ldu = 32 * ((a.rank + 31) / 32) + 8;
   hipLaunchKernelGGL((lora_expand<WB, YB, T, WT>), dim3(a.chunk0[a.parts], a.share, tiles), dim3(64 * LR_WAVES), (size_t)T * LR_ROWS * ldu * 2, s, a);
 }
@@ -357,7 +431,7 @@ extern "C" int fh_lora(const void* x, int x_dtype, int64_t ldx, int64_t rows, in
   l.u = (float*)workspace; l.residual = residual; l.ldr = residual ? ldr : ldy; l.y = y; l.ldy = ldy;
   const int64_t tiles = (rows + LR_ROWS - 1) / LR_ROWS;
   l.share = (int)(tiles > 16 ? 1 : std::min<int64_t>(std::min<int64_t>(adapters + 1LL, rows), LR_ROWS));
-  l.width = 256;
+  l.width = LR_WIDTH;
   int chunks = 0;
   for (int p = 0; p < parts; ++p) { l.chunk0[p] = chunks; chunks += (int)((part_cols[p] + l.width - 1) / l.width); }
   l.chunk0[parts] = chunks;

@@ -2,7 +2,7 @@
 explicit argtypes and restype for every entry point, a status code turned into an exception with the library's own
 message. Pointers are plain integers (a torch tensor's data_ptr()), streams the raw hipStream_t (a torch stream's
 cuda_stream). Loading fails loudly when the library is missing: there is no CPU fallback."""
-import ctypes, os, pathlib
+import ctypes, os, pathlib, struct
 
 HERE = pathlib.Path(__file__).resolve().parent
 PATH = pathlib.Path(os.environ.get("FERRITE_HIP_LIB", HERE / "libferrite_hip.so"))
@@ -69,6 +69,7 @@ SIGNATURES = {
   "fh_attention_paged": ([P, I, L, P, I, L, L, I, I, I, I, P, P, P, L, L, I, L, P, I, L, P, S, P], I),
   "fh_lora_workspace_bytes": ([L, L, I, I], S),
   "fh_lora": ([P, I, L, L, L, P, P, I, I, I, I, ctypes.POINTER(L), P, P, P, L, P, I, L, P, S, P], I),
+  "fh_call": ([I, ctypes.c_char_p], I),
   "fh_rms_rows": ([P, L, L, L, P, ctypes.c_float, I, P, I, L, P], I),
   "fh_moe_route": ([P, L, I, L, P, ctypes.c_float, I, P, I, I, I, I, P, P, P, P], I),
   "fh_moe_workspace_bytes": ([I, I, L, L], S),
@@ -92,6 +93,10 @@ SIGNATURES = {
   "fh_put_rows": ([P, L, L, L, P, L, L, L, P, L, L, P], I),
 }
 
+# the entry points that go by fh_call: their number there, and their arguments' packing
+ARRAYS = {name: (i, struct.Struct("=" + "".join("d" if t is ctypes.c_float else "q" for t in SIGNATURES[name][0])).pack)
+          for i, name in enumerate(("fh_rope_append_paged", "fh_attention_paged", "fh_lora"))}
+
 _lib = None
 
 
@@ -111,6 +116,14 @@ def load():
 def call(name, *args):
   """Calls an entry point that returns a status; a negative one raises with fh_last_error()'s message."""
   rc = getattr(_lib or load(), name)(*args)
+  if rc < 0: raise ERRORS.get(rc, RuntimeError)(_lib.fh_last_error().decode())
+  return rc
+
+
+def call_array(name, *args):
+  """call for an entry point of fh_call's, every argument a plain number (0 for no pointer)."""
+  entry, pack = ARRAYS[name]
+  rc = (_lib or load()).fh_call(entry, pack(*args))
   if rc < 0: raise ERRORS.get(rc, RuntimeError)(_lib.fh_last_error().decode())
   return rc
 

@@ -484,15 +484,22 @@ def attention_decode_shared(q, cache, heads, kv_heads, head_dim, places, first_r
 
 
 def _paged_operands(what, starts, p0, tables, page, length):
-  """The arguments that say where packed rows' sequences lie in a cache of `length` rows in pages: tables' rows and columns."""
+  """The arguments that say where packed rows' sequences lie in a cache of `length` rows in pages: the sequences, tables' rows and columns."""
   n = p0.numel()
   _vector(what, "starts", starts, (n + 1,))
   _vector(what, "p0", p0, (n,))
   shape, st = tables.shape, tables.stride()
   if tables.dtype is not _I32 or len(shape) != 2 or shape[0] != n or shape[1] < 1 or (shape[1] > 1 and st[1] != 1) or (n > 1 and st[0] < shape[1]):
     raise ValueError(f"{what}: tables is [{n}][pages a sequence] {_I32} with contiguous rows")
-  if length % page if page > 0 else True: raise ValueError(f"{what}: a cache of {length} rows is not whole pages of {page}")
+  if page < 1 or length % page: raise ValueError(f"{what}: a cache of {length} rows is not whole pages of {page}")
   return n, max(st[0], shape[1]), shape[1]
+
+
+def _out_rows(what, name, t, shape):
+  """The rows apart of t, fp32 or bf16 rows of `shape` (one row's stride may be anything)."""
+  ld, unit = t.stride()
+  if t.dtype not in _TORCH or t.shape != shape or unit != 1: raise ValueError(f"{what}: {name} is [{shape[0]}][{shape[1]}] fp32 or bf16 with contiguous rows")
+  return ld if shape[0] > 1 else shape[1]
 
 
 def rope_append_paged(qkv, cache, heads, kv_heads, head_dim, cos, sin, starts, p0, tables, page, q_norm=None, k_norm=None, eps=1e-5, centered=False,
@@ -512,22 +519,19 @@ def rope_append_paged(qkv, cache, heads, kv_heads, head_dim, cos, sin, starts, p
   if (cos is None) != (sin is None): raise ValueError(f"{what}: cos and sin go together")
   turns = 0
   if cos is not None:
-    if cos.dim() != 2 or cos.shape[1] != head_dim or cos.shape != sin.shape: raise ValueError(f"{what}: cos and sin are [places][{head_dim}] fp32")
-    turns = cos.shape[0]
-    _vector(what, "cos", cos, cos.shape, _F32)
-    _vector(what, "sin", sin, cos.shape, _F32)
-  if q is None: q = torch.zeros(T, heads * head_dim, dtype=out_dtype, device=qkv.device)
-  if q.dtype not in _TORCH or q.shape != (T, heads * head_dim) or q.stride()[1] != 1: raise ValueError(f"{what}: q is [{T}][{heads * head_dim}] fp32 or bf16 with contiguous rows")
+    shape = cos.shape
+    if len(shape) != 2 or shape[1] != head_dim: raise ValueError(f"{what}: cos and sin are [places][{head_dim}] fp32")
+    turns = shape[0]
+    _vector(what, "cos", cos, shape, _F32)
+    _vector(what, "sin", sin, shape, _F32)
+  shape = (T, heads * head_dim)
+  if q is None: q = torch.zeros(shape, dtype=out_dtype, device=qkv.device)
+  ldq = _out_rows(what, "q", q, shape)
   _here(what, qkv, data, starts, p0, tables, q_norm, k_norm, cos, sin, q)
-  lib.call("fh_rope_append_paged", qkv.data_ptr(), _TORCH[qkv.dtype], _rows_apart(qkv), T, n, heads, kv_heads, head_dim, _ptr(q_norm), _ptr(k_norm), eps, int(centered),
-           _ptr(cos), _ptr(sin), turns, starts.data_ptr(), p0.data_ptr(), tables.data_ptr(), ldt, cols, page, q.data_ptr(), _TORCH[q.dtype],
-           _rows_apart(q), data.data_ptr(), dtype, length, _stream())
+  lib.call_array("fh_rope_append_paged", qkv.data_ptr(), _TORCH[qkv.dtype], qkv.stride()[0] if T > 1 else qkv.shape[1], T, n, heads, kv_heads, head_dim, _ptr(q_norm) or 0,
+                 _ptr(k_norm) or 0, eps, int(centered), _ptr(cos) or 0, _ptr(sin) or 0, turns, starts.data_ptr(), p0.data_ptr(), tables.data_ptr(), ldt, cols, page,
+                 q.data_ptr(), _TORCH[q.dtype], ldq, data.data_ptr(), dtype, length, _stream())
   return q
-
-
-def _rows_apart(t):
-  """A [rows][cols] operand's row stride (one row's may be anything)."""
-  return t.stride()[0] if t.shape[0] > 1 else t.shape[1]
 
 
 @functools.lru_cache(maxsize=1024)
@@ -535,8 +539,8 @@ def _paged_bytes(*sizes): return lib.load().fh_attention_paged_workspace_bytes(*
 
 
 def attention_paged_workspace(rows, sequences, heads, kv_heads, head_dim, max_context, device="cuda"):
-  """fh_attention_paged's workspace for calls of no more rows, sequences, heads and context, uninitialised (a workspace needs no
-  clearing)."""
+  """fh_attention_paged's workspace for calls of no more rows, sequences, heads (of as many key heads) and context, uninitialised (a
+  workspace needs no clearing)."""
   n = _paged_bytes(rows, sequences, heads, kv_heads, head_dim, max_context)
   return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
 
@@ -551,19 +555,20 @@ def attention_paged(q, cache, heads, kv_heads, head_dim, starts, p0, tables, pag
   T = _rows_operand(what, q, cols)
   data, dtype, length = _cache_of(what, cache, kv_heads, head_dim)
   n, ldt, pages = _paged_operands(what, starts, p0, tables, page, length)
-  if o is None: o = torch.zeros(T, cols, dtype=out_dtype, device=q.device)
-  if o.dtype not in _TORCH or o.shape != (T, cols) or o.stride()[1] != 1: raise ValueError(f"{what}: o is fp32 or bf16 rows of q's shape")
-  ws, need = None, _paged_bytes(T, n, heads, kv_heads, head_dim, max_context)
+  shape = (T, cols)
+  if o is None: o = torch.zeros(shape, dtype=out_dtype, device=q.device)
+  ldo = _out_rows(what, "o", o, shape)
+  ws, need = 0, _paged_bytes(T, n, heads, kv_heads, head_dim, max_context)
   if need:
     if workspace is None: workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     ws, need = workspace.data_ptr(), workspace.numel() * workspace.element_size()
   _here(what, q, data, starts, p0, tables, o, workspace)
-  lib.call("fh_attention_paged", q.data_ptr(), _TORCH[q.dtype], _rows_apart(q), data.data_ptr(), dtype, length, T, n, heads, kv_heads, head_dim,
-           starts.data_ptr(), p0.data_ptr(), tables.data_ptr(), ldt, pages, page, max_context, o.data_ptr(), _TORCH[o.dtype], _rows_apart(o), ws, need, _stream())
+  lib.call_array("fh_attention_paged", q.data_ptr(), _TORCH[q.dtype], q.stride()[0] if T > 1 else cols, data.data_ptr(), dtype, length, T, n, heads, kv_heads, head_dim,
+                 starts.data_ptr(), p0.data_ptr(), tables.data_ptr(), ldt, pages, page, max_context, o.data_ptr(), _TORCH[o.dtype], ldo, ws, need, _stream())
   return o
 
 
-@dataclass
+@dataclass(frozen=True)
 class Adapters:
   """Low-rank adapters of a projection [K] -> [N] whose columns are `parts` runs (q, k and v; gate and up; or one): a [adapters][parts
   rank][K], each part's `rank` rows after the last one's, and b [adapters][N][rank], contiguous fp32 or bf16 alike, rank and K
@@ -572,6 +577,17 @@ class Adapters:
   b: torch.Tensor
   scale: torch.Tensor | None
   parts: tuple
+
+  def __post_init__(self):
+    a, b, parts = self.a, self.b, tuple(int(c) for c in self.parts)
+    if a.dim() != 3 or b.dim() != 3 or a.dtype not in _TORCH or b.dtype != a.dtype or not a.is_contiguous() or not b.is_contiguous():
+      raise ValueError("lora: adapters a [n][parts rank][K] and b [n][N][rank], contiguous, fp32 or bf16 alike")
+    (n, C, K), N, r = a.shape, b.shape[1], b.shape[2]
+    if n < 1 or b.shape[0] != n or C != r * len(parts) or N != sum(parts): raise ValueError(f"lora: adapters a {tuple(a.shape)} and b {tuple(b.shape)} for parts of {parts} columns")
+    if self.scale is not None: _vector("lora", "scale", self.scale, (n,), _F32)
+    object.__setattr__(self, "parts", parts)
+    cols = (ctypes.c_int64 * len(parts))(*parts)
+    object.__setattr__(self, "_call", (K, N, r, (_TORCH[a.dtype], n, r, len(parts), ctypes.addressof(cols)), cols))  # (what a call passes of the sizes)
 
   @property
   def rank(self): return self.b.shape[2]
@@ -598,18 +614,13 @@ def pack_adapters(matrices, parts, scales=None, dtype=torch.bfloat16, device="cu
   return Adapters(a.view(len(matrices), len(parts) * r, K), b, s, tuple(parts))
 
 
-def lora_workspace(rows, adapters, device="cuda"):
-  """fh_lora's workspace for calls of no more rows with these adapters, uninitialised (a workspace needs no clearing)."""
-  n = lib.load().fh_lora_workspace_bytes(rows, adapters.a.shape[2], adapters.rank, len(adapters.parts))
-  return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
-
-
-@functools.lru_cache(maxsize=256)
-def _columns(parts): return (ctypes.c_int64 * len(parts))(*parts)
-
-
 @functools.lru_cache(maxsize=1024)
 def _lora_bytes(*sizes): return lib.load().fh_lora_workspace_bytes(*sizes)
+
+
+def lora_workspace(rows, adapters, device="cuda"):
+  """fh_lora's workspace for calls of no more rows with these adapters, uninitialised (a workspace needs no clearing)."""
+  return torch.empty(max(_lora_bytes(rows, adapters.a.shape[2], adapters.rank, len(adapters.parts)), 256), dtype=torch.uint8, device=device)
 
 
 def lora(x, adapters, ids, residual=None, out=None, workspace=None, out_dtype=torch.float32):
@@ -617,23 +628,20 @@ def lora(x, adapters, ids, residual=None, out=None, workspace=None, out_dtype=to
   bf16) with i = ids[t] (int32 on the GPU, read when the kernels run); a row whose id is none of the adapters' keeps its residual.
   residual [T][N] (fp32 or bf16, out's type) may be out itself; None: zeros."""
   what = "lora"
-  a, b = adapters.a, adapters.b
-  parts = tuple(adapters.parts)
-  if a.dim() != 3 or b.dim() != 3 or a.dtype not in _TORCH or b.dtype != a.dtype or not a.is_contiguous() or not b.is_contiguous():
-    raise ValueError(f"{what}: adapters a [n][parts rank][K] and b [n][N][rank], contiguous, fp32 or bf16 alike")
-  (n, C, K), N, r = a.shape, b.shape[1], b.shape[2]
-  if n < 1 or b.shape[0] != n or C != r * len(parts) or N != sum(parts): raise ValueError(f"{what}: adapters a {tuple(a.shape)} and b {tuple(b.shape)} for parts of {parts} columns")
+  a, b, scale = adapters.a, adapters.b, adapters.scale
+  K, N, r, sizes, _ = adapters._call
   T = _rows_operand(what, x, K)
   _vector(what, "ids", ids, (T,))
-  if adapters.scale is not None: _vector(what, "scale", adapters.scale, (n,), _F32)
-  if out is None: out = torch.empty(T, N, dtype=out_dtype if residual is None else residual.dtype, device=x.device)
-  for t in (out,) if residual is None else (out, residual):
-    if t.dtype not in _TORCH or t.dtype != out.dtype or t.shape != (T, N) or t.stride()[1] != 1: raise ValueError(f"{what}: residual and out are [{T}][{N}] fp32 or bf16 alike with contiguous rows")
-  if workspace is None: workspace = torch.empty(_lora_bytes(T, K, r, len(parts)), dtype=torch.uint8, device=x.device)
-  _here(what, x, a, b, adapters.scale, ids, residual, out, workspace)
-  lib.call("fh_lora", x.data_ptr(), _TORCH[x.dtype], _rows_apart(x), T, K, a.data_ptr(), b.data_ptr(), _TORCH[a.dtype], n, r, len(parts), _columns(parts),
-           _ptr(adapters.scale), ids.data_ptr(), _ptr(residual), 0 if residual is None else _rows_apart(residual), out.data_ptr(), _TORCH[out.dtype], _rows_apart(out),
-           workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream())
+  shape = (T, N)
+  if out is None: out = torch.empty(shape, dtype=out_dtype if residual is None else residual.dtype, device=x.device)
+  ldo, res, ldr = _out_rows(what, "out", out, shape), 0, 0
+  if residual is not None:
+    res, ldr = residual.data_ptr(), _out_rows(what, "residual", residual, shape)
+    if residual.dtype != out.dtype: raise ValueError(f"{what}: residual and out are of one type")
+  if workspace is None: workspace = torch.empty(_lora_bytes(T, K, r, len(adapters.parts)), dtype=torch.uint8, device=x.device)
+  _here(what, x, a, b, scale, ids, residual, out, workspace)
+  lib.call_array("fh_lora", x.data_ptr(), _TORCH[x.dtype], x.stride()[0] if T > 1 else K, T, K, a.data_ptr(), b.data_ptr(), *sizes, _ptr(scale) or 0, ids.data_ptr(), res, ldr, out.data_ptr(), _TORCH[out.dtype], ldo,
+                 workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream())
   return out
 
 
