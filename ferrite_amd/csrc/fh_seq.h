@@ -982,6 +982,14 @@ __global__ __launch_bounds__(TOKENS ? 512 : 1024) void seq_join_pages(SeqArgs a)
     if constexpr (TOKENS) {
       for (int i0 = 0; i0 < parts; i0 += 64) {
         const bool in = i0 + lane < parts && some_of(i0 + lane);
+        float v[8][D];
+        auto load = [&](int i) {
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int d = 0; d < D; ++d) v[u][d] = part(min(i0 + i + u, parts - 1), p)[d0 + d];
+        };
+        load(0);  // (on their way with the statistics)
         const float2 st = in ? *(const float2*)(part(i0 + lane, p) + HD) : make_float2(-INFINITY, 0.f);
         const float now = fmaxf(top, wave_max(st.x));
         const bool none = st.y == 0.f && st.x == -INFINITY;
@@ -992,11 +1000,7 @@ __global__ __launch_bounds__(TOKENS ? 512 : 1024) void seq_join_pages(SeqArgs a)
         for (int d = 0; d < D; ++d) o[d] = any ? o[d] * f : 0.f;
         const uint64_t some = __ballot(!none && in);
         for (int i = 0; i < min(64, parts - i0); i += 8) {
-          float v[8][D];
-#pragma unroll
-          for (int u = 0; u < 8; ++u)
-#pragma unroll
-            for (int d = 0; d < D; ++d) v[u][d] = part(min(i0 + i + u, parts - 1), p)[d0 + d];
+          if (i) load(i);
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
             const float wp = __shfl(wt, (i + u) & 63, 64);
