@@ -26,6 +26,11 @@ then the final norm and the output layer for the last row only (fh_gemv_bfp), an
 Many prompts go in together (prefill_batch): their rows packed one after another through the same matmuls, the attention
 fh_attention_prefill_packed. A batch whose sequences begin alike keeps that prefix once (share_prefix): its rows' attention is
 fh_attention_decode_shared, their own slots hold what follows the prefix.
+
+A service whose sequences' lengths are anybody's guess keeps them in pages of the same cache, and its requests may bring low-rank adapters
+(step_pages; page_step for a decode step replayed as one HIP graph). qkv is then a plain product, which fh_lora adds each row's adapter to;
+fh_rope_append_paged turns it and puts k and v into the rows' pages, and the attention is fh_attention_paged. o, gate_up and down take
+fh_lora behind their products the same way.
 """
 import math
 from types import SimpleNamespace
@@ -439,12 +444,116 @@ class Decoder:
       ops.rms_rows(x, L.norm2, c.eps, c.centered, out=xn)
       ops.gemm(xn, L.gate_up, ops.epilogue(lib.EP_SILU_GATE, split=c.ffn), out=h)
       ops.gemm(h, L.down, ops.epilogue(lib.EP_RESIDUAL, residual=x), out=x)
-    # each prompt's last row: the final norm and the output layer (bf16 rows on the matrix cores from three prompts on)
-    xl = ops.gather_rows(x, last_t)
+    return self._last_rows(x, last_t, n)
+
+  def _page_layout(self, what, places, lens, tables, page):
+    """The tables [n][pages] of sequences whose rows are at places[i] .. places[i] + lens[i] - 1, checked: pages that the cache has (-1
+    behind those that a sequence needs), and no page that rows are put into another's."""
+    pages = self.slots * self.part // page if page > 0 else 0
+    if page < 16 or page & (page - 1) or self.slots * self.part % page: raise ValueError(f"{what}: pages of 16, 32, 64, ... rows of a cache of {self.slots * self.part}")
+    n = len(lens)
+    if len(tables) != n or places.shape != (n,): raise ValueError(f"{what}: {n} places and tables")
+    if (places < 0).any() or (places + lens > self.c.places).any(): raise ValueError(f"{what}: a place outside RoPE's tables")
+    need = -(-(places + lens) // page)
+    out = np.full((n, max(int(need.max()), max(len(t) for t in tables))), -1, np.int64)
+    for i, t in enumerate(tables):
+      if len(t) < need[i]: raise ValueError(f"{what}: sequence {i} needs {need[i]} pages, not {len(t)}")
+      out[i, :len(t)] = t
+    col = np.arange(out.shape[1])[None]
+    used = col < need[:, None]
+    if ((out[used] < 0) | (out[used] >= pages)).any(): raise ValueError(f"{what}: a page outside 0..{pages - 1}")
+    written = out[used & (col >= (places // page)[:, None])]
+    if (np.bincount(out[used], minlength=pages)[written] > 1).any(): raise ValueError(f"{what}: a page that rows are put into is another's too")
+    return out
+
+  def _page_rows(self, P, T, n, ids, starts, p0, last, of, tables, page, most, ws, adapters):
+    """The model over T packed rows of n sequences whose keys and values lie in pages: each sequence's last row's logits and pick. of:
+    each row's adapter, where there are any."""
+    c, hd = self.c, self.hd
+    x, ssq, xn, q, att, h = P.x[:T], P.ssq[:T], P.xn[:T], P.q[:T], P.att[:T], P.h[:T]
+    lora_ws = P.lora_ws if adapters else None
+    ops.embed_rows(self.embed, ids, x, ssq)
+    for l, L in enumerate(self.layers):
+      ad = adapters[l] if adapters else {}
+      ops.rms_rows(x, L.norm1, c.eps, c.centered, out=xn)
+      qkv = ops.gemm(xn, L.qkv, out=P.qkv[:T])
+      if "qkv" in ad: ops.lora(xn, ad["qkv"], of, residual=qkv, out=qkv, workspace=lora_ws)
+      ops.rope_append_paged(qkv, self.cache[l], c.heads, c.kv, hd, self.cos, self.sin, starts, p0, tables, page, q=q)
+      ops.attention_paged(q, self.cache[l], c.heads, c.kv, hd, starts, p0, tables, page, most, workspace=ws, o=att)
+      ops.gemm(att, L.o, ops.epilogue(lib.EP_RESIDUAL, residual=x), out=x)
+      if "o" in ad: ops.lora(att, ad["o"], of, residual=x, out=x, workspace=lora_ws)
+      ops.rms_rows(x, L.norm2, c.eps, c.centered, out=xn)
+      if "gate_up" in ad:
+        gu = ops.gemm(xn, L.gate_up, out=P.gu[:T])
+        ops.lora(xn, ad["gate_up"], of, residual=gu, out=gu, workspace=lora_ws)
+        ops.silu_gate_rows(gu, c.ffn, h)
+      else:
+        ops.gemm(xn, L.gate_up, ops.epilogue(lib.EP_SILU_GATE, split=c.ffn), out=h)
+      ops.gemm(h, L.down, ops.epilogue(lib.EP_RESIDUAL, residual=x), out=x)
+      if "down" in ad: ops.lora(h, ad["down"], of, residual=x, out=x, workspace=lora_ws)
+    return self._last_rows(x, last, n)
+
+  def _page_buffers(self, T, adapters):
+    c, hd, dev = self.c, self.hd, self.device
+    e = lambda *s, dtype=torch.float32: torch.empty(*s, dtype=dtype, device=dev)
+    b = torch.bfloat16
+    P = SimpleNamespace(T=T, x=e(T, c.dim), ssq=e(T, c.dim // 16), xn=e(T, c.dim, dtype=b), qkv=e(T, self.qkv_cols), q=e(T, c.heads * hd), att=e(T, c.heads * hd, dtype=b), h=e(T, c.ffn, dtype=b))
+    if adapters:
+      given = [a for ad in adapters for a in ad.values()]
+      if any("gate_up" in ad for ad in adapters): P.gu = e(T, 2 * c.ffn)
+      P.lora_ws = max((ops.lora_workspace(T, a, dev) for a in given), key=lambda t: t.numel())
+    return P
+
+  def _check_adapters(self, what, adapters):
+    c, qkv = self.c, (self.c.heads * self.hd, self.c.kv * self.hd, self.c.kv * self.hd)
+    shapes = dict(qkv=(c.dim, qkv), o=(c.heads * self.hd, (c.dim,)), gate_up=(c.dim, (c.ffn, c.ffn)), down=(c.ffn, (c.dim,)))
+    if adapters is None or not any(adapters): return None
+    if len(adapters) != c.layers: raise ValueError(f"{what}: adapters for each of {c.layers} blocks")
+    for ad in adapters:
+      for name, a in ad.items():
+        if name not in shapes or (a.a.shape[2], a.parts) != shapes[name]: raise ValueError(f"{what}: {name}'s adapters, [{a.a.shape[2]}] -> {a.parts}, are not of {shapes.get(name, 'qkv, o, gate_up or down')}")
+    return adapters
+
+  def step_pages(self, tokens, places, tables, page=64, adapters=None, of=None):
+    """A step over sequences whose keys and values lie in pages of the cache (its slots * context rows cut into pages of `page`, 16, 32,
+    64, ...), as many tokens of each as there are: whole prompts, chunks of them and single tokens in one call. Sequence i's tokens
+    are at places places[i], places[i] + 1, ..., its place p in page tables[i][p // page]; sequences may begin with the same pages (a common
+    prompt), but what rows are put into is one's own. The pages are the caller's to hand out, and so are the rows of slots that
+    they lie in. adapters: for each block a dict of ops.Adapters, of any of "qkv" (parts q, k, v), "o", "gate_up" (gate, up) and "down"; of: each
+    sequence's (-1: none). Returns each sequence's last token's logits ([n][vocab] fp32) and greedy picks ([n] int32), within the
+    rounding of bf16 rows and fp32 sums of prefill's."""
+    c, what = self.c, "step_pages"
+    ops.attention_heads_ok(c.heads, c.kv, self.hd)
+    n = len(tokens)
+    lens = np.array([len(t) for t in tokens], np.int64)
+    if n < 1 or (lens < 1).any(): raise ValueError(f"{what}: at least a token of each sequence")
+    places = np.asarray(places, np.int64)
+    tab = self._page_layout(what, places, lens, tables, page)
+    adapters = self._check_adapters(what, adapters)
+    T, starts = int(lens.sum()), np.concatenate([[0], np.cumsum(lens)])
+    of = np.full(n, -1, np.int64) if of is None else np.asarray(of, np.int64)
+    if of.shape != (n,): raise ValueError(f"{what}: {n} sequences' adapters")
+    ints = np.concatenate([np.concatenate([np.asarray(t, np.int64) for t in tokens]), starts, places, starts[1:] - 1, np.repeat(of, lens), tab.reshape(-1)]).astype(np.int32)
+    held = torch.empty(ints.size, dtype=torch.int32, device=self.device)
+    if ints.size <= PUT_MAX: ops.put_i32(ints, held)
+    else: held.copy_(torch.from_numpy(ints))
+    ids, st, p0, last, rows_of, t = held.split([T, n + 1, n, n, T, tab.size])
+    most = int((places + lens).max())
+    ws = ops.attention_paged_workspace(T, n, c.heads, c.kv, self.hd, most, self.device)
+    return self._page_rows(self._page_buffers(T, adapters), T, n, ids, st, p0, last, rows_of, t.view(n, -1), page, most, ws, adapters)
+
+  def page_step(self, n, pages, page=64, adapters=None):
+    """step_pages for n sequences of one token each with up to `pages` pages, captured once and replayed (PageStep)."""
+    return PageStep(self, n, pages, page, adapters)
+
+  def _last_rows(self, x, last, n):
+    """The final norm and the output layer of rows `last` of x (bf16 rows on the matrix cores from three on): logits and picks."""
+    c = self.c
+    xl = ops.gather_rows(x, last)
     few = n < 3
     xl = ops.rms_rows(xl, self.norm, c.eps, c.centered, out_dtype=torch.float32 if few else torch.bfloat16)
-    logits = torch.empty(n, c.vocab, dtype=torch.float32, device=dev)
-    parts = torch.empty(n, c.vocab // 16, dtype=torch.int64, device=dev)
+    logits = torch.empty(n, c.vocab, dtype=torch.float32, device=self.device)
+    parts = torch.empty(n, c.vocab // 16, dtype=torch.int64, device=self.device)
     (ops.gemv if few else ops.gemm)(xl, self.head, ops.epilogue(lib.EP_STORE, argmax_parts=parts), out=logits)
     return logits, ops.argmax_parts(parts)
 
@@ -491,6 +600,56 @@ class Decoder:
     if inv_temp is not None and not isinstance(inv_temp, torch.Tensor):
       inv_temp = torch.as_tensor(inv_temp, dtype=torch.float32, device=self.device).reshape(-1)
     return ops.logit_heads(logits, k, inv_temp)
+
+
+class PageStep:
+  """A decode step of `n` sequences over a Decoder's cache in pages (Decoder.page_step), replayed as one HIP graph: their tokens, places,
+  pages and adapters are data. A sequence of the batch that nobody holds steps a page of its own."""
+
+  def __init__(self, dec, n, pages, page, adapters):
+    ops.attention_heads_ok(dec.c.heads, dec.c.kv, dec.hd)
+    if n < 1 or pages < 1: raise ValueError("page_step: at least a sequence and a page")
+    if page < 16 or page & (page - 1) or dec.slots * dec.part % page: raise ValueError(f"page_step: pages of 16, 32, 64, ... rows of a cache of {dec.slots * dec.part}")
+    self.dec, self.n, self.pages, self.page, self.adapters, self.graph = dec, n, pages, page, dec._check_adapters("page_step", adapters), None
+    c, dev = dec.c, dec.device
+    self._int = torch.zeros(2 * n + n * pages + n, dtype=torch.int32, device=dev)
+    self.ids, self.p0, self.of, self.tables = self._int.split([n, n, n, n * pages])
+    self.tables = self.tables.view(n, pages)
+    self.starts = torch.arange(n + 1, dtype=torch.int32, device=dev)
+    self.bufs = dec._page_buffers(n, self.adapters)
+    self.ws = ops.attention_paged_workspace(n, n, c.heads, c.kv, dec.hd, pages * page, dev)
+
+  def _step(self):
+    return self.dec._page_rows(self.bufs, self.n, self.n, self.ids, self.starts, self.p0, self.starts[:self.n], self.of, self.tables, self.page,
+                               self.pages * self.page, self.ws, self.adapters)
+
+  def set(self, tokens, places, tables, of=None):
+    """The sequences' next tokens, places and pages, and their adapters (-1, or none given: none)."""
+    n = self.n
+    places = np.asarray(places, np.int64)
+    tab = self.dec._page_layout("page_step", places, np.ones(n, np.int64), tables, self.page)
+    if tab.shape[1] > self.pages: raise ValueError(f"page_step: up to {self.pages} pages a sequence, not {tab.shape[1]}")
+    tokens, of = np.asarray(tokens, np.int64), np.full(n, -1) if of is None else np.asarray(of, np.int64)
+    if tokens.shape != (n,) or of.shape != (n,): raise ValueError(f"page_step: {n} tokens and adapters")
+    wide = np.full((n, self.pages), -1, np.int64)
+    wide[:, :tab.shape[1]] = tab
+    ints = np.concatenate([tokens, places, of, wide.reshape(-1)]).astype(np.int32)
+    if ints.size <= PUT_MAX: ops.put_i32(ints, self._int)
+    else: self._int.copy_(torch.from_numpy(ints))
+
+  def step(self, tokens=None, places=None, tables=None, of=None, replay=True):
+    """One step: the logits ([n][vocab] fp32) and greedy picks ([n] int32); a replayed step's are the graph's, as they are until the
+    next."""
+    if tokens is not None: self.set(tokens, places, tables, of)
+    if not replay: return self._step()
+    if self.graph is None:
+      self._step()  # warm: every kernel loaded before capture
+      torch.cuda.synchronize(self.dec.device)
+      g = torch.cuda.CUDAGraph()
+      with torch.cuda.graph(g): self.out = self._step()
+      self.graph = g
+    self.graph.replay()
+    return self.out
 
 
 def numpy_weights(w):
