@@ -318,8 +318,8 @@ int fh_attention_decode_shared(const void* q, int q_dtype, const void* cache, in
  * NULL for none), and turned as FH_EP_ROPE_KV turns them by their place's row of cos_tab and sin_tab ([rope_rows][head_dim], a place
  * outside reads the nearest row; both NULL: not turned); q out (FH_F32 or FH_BF16), k and v into the cache at their place's row,
  * rounded as FH_EP_ROPE_KV's put. A place past the table or a page outside the cache writes no key or value. For projections
- * whose q, k and v are not final in the product (an adapter's part is added first), and for models with normed heads. qkv's
- * and q's rows are aligned to 4 values; norms, tables of angles and the cache to 16 bytes. */
+ * whose q, k and v are not final in the product (an adapter's part is added first), and for models with normed heads. q may be qkv's
+ * own q columns (ldq = ldx). qkv's and q's rows are aligned to 4 values; norms, tables of angles and the cache to 16 bytes. */
 int fh_rope_append_paged(const void* qkv, int x_dtype, int64_t ldx, int64_t rows, int sequences, int heads, int kv_heads,
                          int head_dim, const float* q_norm, const float* k_norm, float eps, int centered,
                          const float* cos_tab, const float* sin_tab, int64_t rope_rows, const int32_t* starts,

@@ -203,3 +203,31 @@ def test_append_graph_and_stream(cuda):
     with torch.cuda.stream(side): call(c2, q2)
     torch.cuda.synchronize()
     assert torch.equal(c1, c2) and torch.equal(q1, q2)
+
+
+def test_append_in_place_and_many_rows(cuda):
+  # q in qkv's own columns; rows of many sequences, several a workgroup, among them rows that are nobody's
+  rng = np.random.default_rng(11)
+  T, lens = 3333, [1] * 40 + [700, 0, 1300] + [3] * 20 + [900]
+  starts = np.concatenate([[7], 7 + np.cumsum(lens)])
+  before = rng.integers(0, 90, len(lens))
+  counts = [-(-(a + int(b)) // 16) for a, b in zip(lens, before)]
+  ids, at, tables = rng.permutation(sum(counts)), 0, np.full((len(lens), max(counts)), -1)
+  for i, c in enumerate(counts):
+    tables[i, :c] = ids[at:at + c]
+    at += c
+  x = torch.from_numpy(rng.normal(0, 1, (T, 8 * 64)).astype(np.float32)).cuda()
+  ang = torch.from_numpy(rng.normal(0, 1, (1400, 64)).astype(np.float32)).cuda()
+  args = (4, 2, 64, torch.cos(ang), torch.sin(ang), ints(starts), ints(before), ints(tables), 16)
+  c1, c2 = (torch.zeros(4, 16 * len(ids), 64, device="cuda") for _ in range(2))
+  want = ops().rope_append_paged(x, c1, *args, q=torch.full((T, 256), 7.0, device="cuda"))
+  y = x.clone()
+  ops().rope_append_paged(y, c2, *args, q=y[:, :256])
+  used = slice(7, int(starts[-1]))
+  assert torch.equal(y[used, :256], want[used]) and torch.equal(y[:, 256:], x[:, 256:]) and torch.equal(c1, c2)
+  assert torch.equal(y[:7], x[:7]) and torch.equal(y[starts[-1]:], x[starts[-1]:]) and (want[:7] == 7).all() and (want[starts[-1]:] == 7).all()
+  # v's rows are at their places, bit for bit
+  for s in (0, 40, 42, 50, len(lens) - 1):
+    p = int(before[s]) + np.arange(lens[s])
+    rows = torch.from_numpy(tables[s, p // 16] * 16 + p % 16).cuda()
+    assert torch.equal(c1[2:, rows].transpose(0, 1).reshape(lens[s], 128), x[starts[s]:starts[s + 1], 384:])
