@@ -151,16 +151,18 @@ __device__ __forceinline__ void shrink_rows(const LoraArgs& a, int64_t t0, uint6
     LrRaw<XB> x[2][MB];
     LrRaw<WB> w[2][CB];
     bool in[2];
+    int at[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int kk = k + 32 * h + 8 * g;
       in[h] = kk < ke;
-      const int at = in[h] ? kk : 0;
-#pragma unroll
-      for (int j = 0; j < CB; ++j) w[h][j].load(a.a, wat[j] + at);
-#pragma unroll
-      for (int i = 0; i < MB; ++i) x[h][i].load(a.x, xat[i] + at);
+      at[h] = in[h] ? kk : 0;
     }
+    // (a line's halves one after the other: far apart, each would be fetched anew)
+#pragma unroll
+    for (int j = 0; j < CB; ++j) { w[0][j].load(a.a, wat[j] + at[0]); w[1][j].load(a.a, wat[j] + at[1]); }
+#pragma unroll
+    for (int i = 0; i < MB; ++i) { x[0][i].load(a.x, xat[i] + at[0]); x[1][i].load(a.x, xat[i] + at[1]); }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       lr_bf16x8 xf[MB][XT];

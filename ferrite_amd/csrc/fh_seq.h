@@ -948,8 +948,8 @@ __global__ __launch_bounds__(256) void seq_join(SeqArgs a) {
 // The parts of a tile that shares cut, joined as above: a workgroup a cut, which takes the tile whose first cut it is. TOKENS: few
 // pairs of many parts, a wave a pair; otherwise HD / 4 lanes a pair, 4 parts on their way at a time.
 template <int HD, int BK, bool TOKENS>
-__global__ __launch_bounds__(TOKENS ? 512 : 1024) void seq_join_pages(SeqArgs a) {
-  constexpr int NT = TOKENS ? 512 : 1024;
+__global__ __launch_bounds__(TOKENS || HD == 64 ? 512 : 1024) void seq_join_pages(SeqArgs a) {
+  constexpr int NT = TOKENS || HD == 64 ? 512 : 1024;
   __shared__ __attribute__((aligned(16))) int4 held[NT];
   const int heads = a.kv_heads * a.head_tiles, head = blockIdx.x % heads, first = blockIdx.x / heads;  // the share before the cut
   SeqWalk w;
@@ -1089,9 +1089,9 @@ static void launch_seq(int cf, int pairs, unsigned blocks, hipStream_t s, const 
     const dim3 g((unsigned)((a.walkers - 1) * a.kv_heads * a.head_tiles));
     const bool tokens = pairs == 64;
     if (a.parts > 1) {
-      if (cf == FH_F32) hipLaunchKernelGGL((seq_join_pages<HD, 32, false>), g, dim3(1024), 0, s, a);
+      if (cf == FH_F32) hipLaunchKernelGGL((seq_join_pages<HD, 32, false>), g, dim3(HD == 64 ? 512 : 1024), 0, s, a);
       else if (tokens) hipLaunchKernelGGL((seq_join_pages<HD, 64, true>), g, dim3(512), 0, s, a);
-      else hipLaunchKernelGGL((seq_join_pages<HD, 64, false>), g, dim3(1024), 0, s, a);
+      else hipLaunchKernelGGL((seq_join_pages<HD, 64, false>), g, dim3(HD == 64 ? 512 : 1024), 0, s, a);
     }
   } else if (a.parts > 1) hipLaunchKernelGGL(seq_join<HD>, dim3((unsigned)((a.rows * a.heads + 3) / 4)), dim3(256), 0, s, a);
 }
