@@ -5,12 +5,17 @@
 // Two launches: u = x A^T, its K cut into parts that different workgroups sum (u is narrow: without them one prompt tile would be
 // one workgroup), then y = residual + scale u B^T, which adds the parts in order as it takes them. A workgroup takes 64
 // consecutive rows and goes through the adapters among them, each with its own rows gathered, 16 a matrix operand: a packed
-// prompt's rows are one adapter's, a decode step's as many as there are users, shared out among workgroups.
+// prompt's rows are one adapter's, a decode step's as many as there are users, shared out among workgroups. A few rows by small
+// matrices take one launch (lora_few).
 //
 // Both matrices' operands are 8 consecutive values along their inner axis, which is the axis that a checkpoint's rows run
 // along, so x, A and B go from memory to the matrix cores' registers as they lie. Products are bf16's with fp32 sums
 // (v_mfma_f32_16x16x32_bf16): bf16 values go in as they are, fp32 ones (x, u, an fp32 adapter) as two bf16 terms for bf16 output
 // (2^-16 of themselves, less than the output's own rounding, 2^-8) and as three for fp32 output (2^-24).
+//
+// What bounds it (MI355X): the bytes, and for few rows the chain of loads. Beside an 8B model's gate and up, rank 32, 4096 rows of 4 adapters, bf16:
+// 147 us for 510 MB, 24 of them u, the rest y's 470 MB read and written at 3.9 TB/s where a copy reaches 5.1; 333 fp32 rows of 6 adapters by 3456
+// 21 us; beside its q, k and v, rank 16, 32 rows of 24 adapters 12.5 us for 11 MB, two launches of 5 and 7.
 #include <algorithm>
 #include "fh_common.h"
 
@@ -22,6 +27,7 @@ typedef __attribute__((__vector_size__(4 * sizeof(float)))) float lr_floatx4;
 constexpr int LR_ROWS = 64;        // rows a tile
 constexpr int LR_WAVES = 4;
 constexpr int LR_WIDTH = 256;      // columns of y a workgroup of the second: 512 is 3% faster for 4096 rows, 12% slower for 500
+constexpr int LR_FEW_WIDTH = 512;  // of lora_few
 constexpr int LR_MAX_PARTS = 4;    // parts of a fused projection
 constexpr int LR_MAX_RANK = 128;
 
@@ -362,6 +368,131 @@ __global__ __launch_bounds__(64 * LR_WAVES, WB ? 4 : 3) void lora_expand(LoraArg
   }
 }
 
+// A decode step's few rows in one launch: a workgroup of 16 waves adds up u for its adapter's part itself, though the others of the
+// part's columns do the same, and goes on to its columns. Worth it while the part's rows of A (LR_FEW_BYTES at most) take a workgroup less than
+// the second launch. The first columns' residual and B are on their way meanwhile; 16 rows at a time.
+constexpr int LR_FEW_WAVES = 16;
+template <bool XB, bool WB, bool YB, int XT, int WT, int UT, int CB>
+__global__ __launch_bounds__(64 * LR_FEW_WAVES) void lora_few(LoraArgs a) {
+  constexpr int H = XB && WB && CB <= 2 ? 4 : 2, STEP = 32 * LR_FEW_WAVES;  // loads of 32 of K together; columns a round
+  __shared__ __attribute__((aligned(16))) float sums[LR_FEW_WAVES * CB * 256];
+  __shared__ __attribute__((aligned(16))) uint16_t us[UT * 16 * (16 * CB + 32 + 8)];  // u's terms, whole steps of 32 columns
+  int part = 0;
+  while (part + 1 < a.parts && (int)blockIdx.x >= a.chunk0[part + 1]) ++part;
+  const int n0 = a.col0[part] + (blockIdx.x - a.chunk0[part]) * a.width, n1 = min(n0 + a.width, a.col0[part + 1]);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+  const int steps = (a.rank + 31) / 32, ldu = 32 * steps + 8;
+  const int kw = (int)((a.K + 64 * LR_FEW_WAVES - 1) / (64 * LR_FEW_WAVES)) * 64, kb = kw * wave, ke = (int)min((int64_t)kb + kw, a.K);
+  LoraTile tile(a, blockIdx.z);
+  int adapter;
+  uint64_t rows;
+  while (tile.next(a.share, blockIdx.y, adapter, rows)) {
+    const int n = __builtin_popcountll(rows);
+    if (adapter < 0) {  // the residual, or zeros
+      if (a.residual == a.y) continue;
+      const int pieces = (n1 - n0) / 8;
+      for (int i = threadIdx.x; i < n * pieces; i += 64 * LR_FEW_WAVES) {
+        const int64_t t = tile.t0 + lr_nth(rows, i / pieces), c = n0 + i % pieces * 8;
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (a.residual) {
+          LrRaw<YB> x;
+          x.load(a.residual, t * a.ldr + c);
+          x.values(f);
+        }
+        lr_write8<YB>(a.y, t * a.ldy + c, f);
+      }
+      continue;
+    }
+    const float sc = a.scale ? a.scale[adapter] : 1.f;
+    const int64_t abase = ((int64_t)adapter * a.C + part * a.rank) * a.K, bbase = (int64_t)adapter * a.N * a.rank;
+    for (int m0 = 0; m0 < n; m0 += 16) {
+      const int64_t row = tile.t0 + lr_nth(rows, min(m0 + r, n - 1));
+      LrRaw<YB> res;
+      LrRaw<WB> b[2];
+      auto load_b = [&](int c, int k) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) b[e].load(a.b, bbase + (int64_t)min(c + 8 * (r >> 2) + 4 * e + (r & 3), n1 - 1) * a.rank + (k < a.rank ? k : 0));
+      };
+      auto load = [&](int c) {
+        if (a.residual) res.load(a.residual, row * a.ldr + min(c + 8 * g, n1 - 8));
+        load_b(c, 8 * g);
+      };
+      int c = n0 + 32 * wave;
+      load(c);  // (a chunk's last waves may have no columns: the last ones')
+      lr_floatx4 acc[CB];
+#pragma unroll
+      for (int j = 0; j < CB; ++j) acc[j] = lr_floatx4{0.f, 0.f, 0.f, 0.f};
+      const int64_t xat = row * a.ldx;
+      for (int k = kb; k < ke; k += 32 * H) {
+        LrRaw<XB> x[H];
+        LrRaw<WB> w[H][CB];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const int at = k + 32 * h + 8 * g < ke ? k + 32 * h + 8 * g : 0;
+          x[h].load(a.x, xat + at);
+#pragma unroll
+          for (int j = 0; j < CB; ++j) w[h][j].load(a.a, abase + (int64_t)min(16 * j + r, a.rank - 1) * a.K + at);
+        }
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const bool in = k + 32 * h + 8 * g < ke;
+          lr_bf16x8 xf[XT];
+          x[h].template terms<XT>(in, xf);
+#pragma unroll
+          for (int j = 0; j < CB; ++j) {
+            lr_bf16x8 wf[WT];
+            w[h][j].template terms<WT>(in, wf);
+            acc[j] = lr_mfma<XT, WT>(xf, wf, acc[j]);
+          }
+        }
+      }
+      // the waves' sums, in order; lane (r, g) holds rows 4 g .. + 3 of column 16 j + r
+#pragma unroll
+      for (int j = 0; j < CB; ++j) *(lr_floatx4*)(sums + ((wave * CB + j) * 64 + lane) * 4) = acc[j];
+      __syncthreads();  // (and the last rows' u is read)
+      for (int i = threadIdx.x; i < 16 * 32 * steps; i += 64 * LR_FEW_WAVES) {
+        const int m = i / (32 * steps), k = i % (32 * steps);
+        float v = 0.f;
+        if (k < a.rank) {
+          const float* p = sums + ((k >> 4) * 64 + (m >> 2) * 16 + (k & 15)) * 4 + (m & 3);
+#pragma unroll
+          for (int w = 0; w < LR_FEW_WAVES; ++w) v += p[w * CB * 256];
+          v *= sc;
+        }
+#pragma unroll
+        for (int e = 0; e < UT; ++e) {
+          const __bf16 t = (__bf16)v;
+          us[(e * 16 + m) * ldu + k] = *(const uint16_t*)&t;
+          v -= (float)t;
+        }
+      }
+      __syncthreads();
+      for (; c < n1; c += STEP) {
+        lr_floatx4 o[2] = {lr_floatx4{0.f, 0.f, 0.f, 0.f}, lr_floatx4{0.f, 0.f, 0.f, 0.f}};
+        for (int s = 0; s < steps; ++s) {
+          const int k = 32 * s + 8 * g;
+          if (s) load_b(c, k);
+          lr_bf16x8 uf[UT];
+#pragma unroll
+          for (int e = 0; e < UT; ++e) uf[e] = *(const lr_bf16x8*)(us + (e * 16 + r) * ldu + k);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            lr_bf16x8 bf[WT];
+            b[e].template terms<WT>(k < a.rank, bf);
+            o[e] = lr_mfma<WT, UT>(bf, uf, o[e]);
+          }
+        }
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (a.residual) res.values(f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] += o[e >> 2][e & 3];
+        if (c + STEP < n1) load(c + STEP);
+        if (m0 + r < n && c + 8 * g < n1) lr_write8<YB>(a.y, row * a.ldy + c + 8 * g, f);
+      }
+    }
+  }
+}
+
 // Parts of K: whole steps of 256 (a wave's 64 each), as many as keep the parts' rows within 16384, so that u's parts stay a
 // small share of what a call moves and a decode step's few rows still fill the GPU.
 constexpr int LR_MAX_SPLITS = 32;
@@ -371,9 +502,24 @@ static int lora_splits(int64_t rows, int64_t K) {
   return (int)std::max<int64_t>(1, std::min(most, LR_SPLIT_ROWS / rows));
 }
 
+// One launch where a part's rows of A are at most LR_FEW_BYTES and those of all adapters that the rows may have LR_FEW_ALL: smollm's q, k
+// and v of 1 row 8.0 -> 5.1 us, an 8B o of 4 rows with as many adapters 9.1 either way, its q, k and v of 32 with 24 12.5 against 15.2.
+constexpr int64_t LR_FEW_BYTES = 160 << 10, LR_FEW_ALL = 1 << 20;
+static bool lora_is_few(int64_t rows, int64_t K, int rank, int adapters, int w_dtype) {
+  const int64_t bytes = rank * K * (w_dtype == FH_F32 ? 4 : 2);
+  return rows <= LR_ROWS && rank <= 64 && bytes <= LR_FEW_BYTES && bytes * std::min<int64_t>(rows, adapters) <= LR_FEW_ALL;
+}
+
 template <bool XB, bool WB, bool YB>
-static void launch_lora(hipStream_t s, const LoraArgs& a) {
+static void launch_lora(bool few, hipStream_t s, const LoraArgs& a) {
   constexpr int T = YB ? 2 : 3, XT = XB ? 1 : T, WT = WB ? 1 : T;
+  if (few) {
+    const dim3 g(a.chunk0[a.parts], a.share, 1), b(64 * LR_FEW_WAVES);
+    if (a.rank <= 16) hipLaunchKernelGGL((lora_few<XB, WB, YB, XT, WT, T, 1>), g, b, 0, s, a);
+    else if (a.rank <= 32) hipLaunchKernelGGL((lora_few<XB, WB, YB, XT, WT, T, 2>), g, b, 0, s, a);
+    else hipLaunchKernelGGL((lora_few<XB, WB, YB, XT, WT, T, 4>), g, b, 0, s, a);
+    return;
+  }
   // u's columns in equal groups of up to 4 blocks of 16
   const unsigned tiles = (unsigned)((a.rows + LR_ROWS - 1) / LR_ROWS), blocks = (a.C + 15) / 16, groups = (blocks + 3) / 4, cb = (blocks + groups - 1) / groups;
   const dim3 g(a.splits * groups, a.share, tiles), b(64 * LR_WAVES);
@@ -424,6 +570,7 @@ extern "C" int fh_lora(const void* x, int x_dtype, int64_t ldx, int64_t rows, in
       (residual && ldr % (y_dtype == FH_F32 ? 4 : 8)) || (((uintptr_t)x | (uintptr_t)a_w | (uintptr_t)b_w | (uintptr_t)y | (uintptr_t)residual) & 15))
     return no(FH_EINVAL, "rows at least K and N, 16-byte aligned, as the adapters");
   if (residual == y && ldr != ldy) return no(FH_EINVAL, "a residual that is y itself has y's rows");
+  const bool few = lora_is_few(rows, K, rank, adapters, w_dtype);
   l.splits = lora_splits(rows, K);
   const size_t need = (size_t)l.splits * rows * rank * parts * sizeof(float);
   if (!workspace || ws_bytes < need || ((uintptr_t)workspace & 15)) return no(FH_EINVAL, "a 16-byte aligned workspace of fh_lora_workspace_bytes");
@@ -433,21 +580,21 @@ extern "C" int fh_lora(const void* x, int x_dtype, int64_t ldx, int64_t rows, in
   l.u = (float*)workspace; l.residual = residual; l.ldr = residual ? ldr : ldy; l.y = y; l.ldy = ldy;
   const int64_t tiles = (rows + LR_ROWS - 1) / LR_ROWS;
   l.share = (int)(tiles > 16 ? 1 : std::min<int64_t>(std::min<int64_t>(adapters + 1LL, rows), LR_ROWS));
-  l.width = LR_WIDTH;
+  l.width = few ? LR_FEW_WIDTH : LR_WIDTH;
   int chunks = 0;
   for (int p = 0; p < parts; ++p) { l.chunk0[p] = chunks; chunks += (int)((part_cols[p] + l.width - 1) / l.width); }
   l.chunk0[parts] = chunks;
   const hipStream_t s = as_stream(stream);
   const int form = (x_dtype == FH_BF16) * 4 + (w_dtype == FH_BF16) * 2 + (y_dtype == FH_BF16);
   switch (form) {
-    case 0: launch_lora<false, false, false>(s, l); break;
-    case 1: launch_lora<false, false, true>(s, l); break;
-    case 2: launch_lora<false, true, false>(s, l); break;
-    case 3: launch_lora<false, true, true>(s, l); break;
-    case 4: launch_lora<true, false, false>(s, l); break;
-    case 5: launch_lora<true, false, true>(s, l); break;
-    case 6: launch_lora<true, true, false>(s, l); break;
-    default: launch_lora<true, true, true>(s, l); break;
+    case 0: launch_lora<false, false, false>(few, s, l); break;
+    case 1: launch_lora<false, false, true>(few, s, l); break;
+    case 2: launch_lora<false, true, false>(few, s, l); break;
+    case 3: launch_lora<false, true, true>(few, s, l); break;
+    case 4: launch_lora<true, false, false>(few, s, l); break;
+    case 5: launch_lora<true, false, true>(few, s, l); break;
+    case 6: launch_lora<true, true, false>(few, s, l); break;
+    default: launch_lora<true, true, true>(few, s, l); break;
   }
   return check_launch("fh_lora");
 }

@@ -365,6 +365,7 @@ def _rows_operand(what, q, cols):
 def _here(what, *ts):
   """Each tensor (or None) on the current GPU, whose stream the call goes to (the first is a tensor on a GPU)."""
   d = ts[0].get_device()
+  if d < 0: _dev(*ts)
   if _device() not in (None, d): raise ValueError(f"{what}: tensors must be on the current GPU")
   for t in ts:
     if t is not None and t.get_device() != d: raise ValueError(f"{what}: tensors must be on one GPU")
@@ -483,23 +484,40 @@ def attention_decode_shared(q, cache, heads, kv_heads, head_dim, places, first_r
   return o
 
 
-def _paged_operands(what, starts, p0, tables, page, length):
-  """The arguments that say where packed rows' sequences lie in a cache of `length` rows in pages: the sequences, tables' rows and columns."""
-  n = p0.numel()
-  _vector(what, "starts", starts, (n + 1,))
-  _vector(what, "p0", p0, (n,))
-  shape, st = tables.shape, tables.stride()
-  if tables.dtype is not _I32 or len(shape) != 2 or shape[0] != n or shape[1] < 1 or (shape[1] > 1 and st[1] != 1) or (n > 1 and st[0] < shape[1]):
-    raise ValueError(f"{what}: tables is [{n}][pages a sequence] {_I32} with contiguous rows")
+# What the calls below check of an operand and pass of it, each read once: a tensor's attributes are most of a small call's time.
+def _rows_of(what, name, t, rows, cols):
+  """(pointer, dtype, rows apart, rows) of t, fp32 or bf16 [rows][cols] (rows None: any) with contiguous rows; one row's stride may be anything."""
+  shape, st, dtype = t.shape, t.stride(), _TORCH.get(t.dtype)
+  if dtype is None or len(st) != 2 or st[1] != 1 or shape[1] != cols or shape[0] < 1 or (rows is not None and shape[0] != rows):
+    raise ValueError(f"{what}: {name} is [{'rows' if rows is None else rows}][{cols}] fp32 or bf16 with contiguous rows, not {tuple(shape)} {t.dtype}")
+  return t.data_ptr(), dtype, st[0] if shape[0] > 1 else cols, shape[0]
+
+
+def _whole(what, name, t, n, dtype=_I32):
+  """The pointer of t, n contiguous values."""
+  if t.dtype is not dtype or t.numel() != n or not t.is_contiguous(): raise ValueError(f"{what}: {name} is {n} contiguous {dtype} on the GPU")
+  return t.data_ptr()
+
+
+def _pages_cache(what, cache, kv_heads, head_dim, page):
+  """(the cache's tensor, its pointer, dtype, rows) of a contiguous cache of kv_heads heads of head_dim in whole pages."""
+  if isinstance(cache, BfpCache): data, dtype, length = _cache_of(what, cache, kv_heads, head_dim)
+  else:
+    data, shape, dtype = cache, cache.shape, _TORCH.get(cache.dtype)
+    if dtype is None or len(shape) != 3 or shape[0] != 2 * kv_heads or shape[2] != head_dim or not data.is_contiguous():
+      raise ValueError(f"{what}: a contiguous cache [{2 * kv_heads}][len][{head_dim}], not {tuple(shape)} {cache.dtype}")
+    length = shape[1]
   if page < 1 or length % page: raise ValueError(f"{what}: a cache of {length} rows is not whole pages of {page}")
-  return n, max(st[0], shape[1]), shape[1]
+  return data, data.data_ptr(), dtype, length
 
 
-def _out_rows(what, name, t, shape):
-  """The rows apart of t, fp32 or bf16 rows of `shape` (one row's stride may be anything)."""
-  ld, unit = t.stride()
-  if t.dtype not in _TORCH or t.shape != shape or unit != 1: raise ValueError(f"{what}: {name} is [{shape[0]}][{shape[1]}] fp32 or bf16 with contiguous rows")
-  return ld if shape[0] > 1 else shape[1]
+def _tables_of(what, starts, p0, tables):
+  """(sequences, starts, p0, tables, tables' rows apart, their columns): where packed rows' sequences lie in a cache in pages."""
+  shape, st = tables.shape, tables.stride()
+  if tables.dtype is not _I32 or len(st) != 2 or shape[0] < 1 or shape[1] < 1 or (shape[1] > 1 and st[1] != 1) or (shape[0] > 1 and st[0] < shape[1]):
+    raise ValueError(f"{what}: tables is [sequences][pages a sequence] {_I32} with contiguous rows")
+  n, cols = shape
+  return n, _whole(what, "starts", starts, n + 1), _whole(what, "p0", p0, n), tables.data_ptr(), st[0] if n > 1 else cols, cols
 
 
 def rope_append_paged(qkv, cache, heads, kv_heads, head_dim, cos, sin, starts, p0, tables, page, q_norm=None, k_norm=None, eps=1e-5, centered=False,
@@ -511,26 +529,22 @@ def rope_append_paged(qkv, cache, heads, kv_heads, head_dim, cos, sin, starts, p
   [sequences + 1], p0 and tables [sequences][pages] are int32 on the GPU, read when the kernel runs. page is 16, 32, 64, ... q keeps its
   rows that are no sequence's; a new q has zeros there. A place or page outside writes no key or value."""
   what = "rope_append_paged"
-  T = _rows_operand(what, qkv, (heads + 2 * kv_heads) * head_dim)
-  data, dtype, length = _cache_of(what, cache, kv_heads, head_dim)
-  n, ldt, cols = _paged_operands(what, starts, p0, tables, page, length)
-  if q_norm is not None: _vector(what, "q_norm", q_norm, (head_dim,), _F32)
-  if k_norm is not None: _vector(what, "k_norm", k_norm, (head_dim,), _F32)
+  x, xdt, ldx, T = _rows_of(what, "qkv", qkv, None, (heads + 2 * kv_heads) * head_dim)
+  data, c, cdt, length = _pages_cache(what, cache, kv_heads, head_dim, page)
+  n, st, pl, tab, ldt, cols = _tables_of(what, starts, p0, tables)
+  qn = 0 if q_norm is None else _whole(what, "q_norm", q_norm, head_dim, _F32)
+  kn = 0 if k_norm is None else _whole(what, "k_norm", k_norm, head_dim, _F32)
   if (cos is None) != (sin is None): raise ValueError(f"{what}: cos and sin go together")
-  turns = 0
+  turns = co = si = 0
   if cos is not None:
-    shape = cos.shape
-    if len(shape) != 2 or shape[1] != head_dim: raise ValueError(f"{what}: cos and sin are [places][{head_dim}] fp32")
-    turns = shape[0]
-    _vector(what, "cos", cos, shape, _F32)
-    _vector(what, "sin", sin, shape, _F32)
-  shape = (T, heads * head_dim)
-  if q is None: q = torch.zeros(shape, dtype=out_dtype, device=qkv.device)
-  ldq = _out_rows(what, "q", q, shape)
+    if cos.dim() != 2: raise ValueError(f"{what}: cos and sin are [places][{head_dim}] fp32")
+    turns = len(cos)
+    co, si = _whole(what, "cos", cos, turns * head_dim, _F32), _whole(what, "sin", sin, turns * head_dim, _F32)
+  if q is None: q = torch.zeros(T, heads * head_dim, dtype=out_dtype, device=qkv.device)
+  to, qdt, ldq, _ = _rows_of(what, "q", q, T, heads * head_dim)
   _here(what, qkv, data, starts, p0, tables, q_norm, k_norm, cos, sin, q)
-  lib.call_array("fh_rope_append_paged", qkv.data_ptr(), _TORCH[qkv.dtype], qkv.stride()[0] if T > 1 else qkv.shape[1], T, n, heads, kv_heads, head_dim, _ptr(q_norm) or 0,
-                 _ptr(k_norm) or 0, eps, int(centered), _ptr(cos) or 0, _ptr(sin) or 0, turns, starts.data_ptr(), p0.data_ptr(), tables.data_ptr(), ldt, cols, page,
-                 q.data_ptr(), _TORCH[q.dtype], ldq, data.data_ptr(), dtype, length, _stream())
+  lib.call_array("fh_rope_append_paged", x, xdt, ldx, T, n, heads, kv_heads, head_dim, qn, kn, eps, centered, co, si, turns, st, pl, tab, ldt, cols, page, to, qdt, ldq, c, cdt,
+                 length, _stream())
   return q
 
 
@@ -552,19 +566,18 @@ def attention_paged(q, cache, heads, kv_heads, head_dim, starts, p0, tables, pag
   below 0 sees nothing and gives zeros."""
   what = "attention_paged"
   cols = heads * head_dim
-  T = _rows_operand(what, q, cols)
-  data, dtype, length = _cache_of(what, cache, kv_heads, head_dim)
-  n, ldt, pages = _paged_operands(what, starts, p0, tables, page, length)
-  shape = (T, cols)
-  if o is None: o = torch.zeros(shape, dtype=out_dtype, device=q.device)
-  ldo = _out_rows(what, "o", o, shape)
+  x, xdt, ldx, T = _rows_of(what, "q", q, None, cols)
+  data, c, cdt, length = _pages_cache(what, cache, kv_heads, head_dim, page)
+  n, st, pl, tab, ldt, pages = _tables_of(what, starts, p0, tables)
+  if o is None: o = torch.zeros(T, cols, dtype=out_dtype, device=q.device)
+  to, odt, ldo, _ = _rows_of(what, "o", o, T, cols)
   ws, need = 0, _paged_bytes(T, n, heads, kv_heads, head_dim, max_context)
   if need:
     if workspace is None: workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    ws, need = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    ws, need = workspace.data_ptr(), workspace.nbytes
   _here(what, q, data, starts, p0, tables, o, workspace)
-  lib.call_array("fh_attention_paged", q.data_ptr(), _TORCH[q.dtype], q.stride()[0] if T > 1 else cols, data.data_ptr(), dtype, length, T, n, heads, kv_heads, head_dim,
-                 starts.data_ptr(), p0.data_ptr(), tables.data_ptr(), ldt, pages, page, max_context, o.data_ptr(), _TORCH[o.dtype], ldo, ws, need, _stream())
+  lib.call_array("fh_attention_paged", x, xdt, ldx, c, cdt, length, T, n, heads, kv_heads, head_dim, st, pl, tab, ldt, pages, page, max_context, to, odt, ldo, ws, need,
+                 _stream())
   return o
 
 
@@ -630,18 +643,19 @@ def lora(x, adapters, ids, residual=None, out=None, workspace=None, out_dtype=to
   what = "lora"
   a, b, scale = adapters.a, adapters.b, adapters.scale
   K, N, r, sizes, _ = adapters._call
-  T = _rows_operand(what, x, K)
-  _vector(what, "ids", ids, (T,))
-  shape = (T, N)
-  if out is None: out = torch.empty(shape, dtype=out_dtype if residual is None else residual.dtype, device=x.device)
-  ldo, res, ldr = _out_rows(what, "out", out, shape), 0, 0
-  if residual is not None:
-    res, ldr = residual.data_ptr(), _out_rows(what, "residual", residual, shape)
-    if residual.dtype != out.dtype: raise ValueError(f"{what}: residual and out are of one type")
+  xp, xdt, ldx, T = _rows_of(what, "x", x, None, K)
+  of = _whole(what, "ids", ids, T)
+  if out is None: out = torch.empty(T, N, dtype=out_dtype if residual is None else residual.dtype, device=x.device)
+  to, odt, ldo, _ = _rows_of(what, "out", out, T, N)
+  res = ldr = 0
+  if residual is out: res, ldr = to, ldo
+  elif residual is not None:
+    res, rdt, ldr, _ = _rows_of(what, "residual", residual, T, N)
+    if rdt != odt: raise ValueError(f"{what}: residual and out are of one type")
   if workspace is None: workspace = torch.empty(_lora_bytes(T, K, r, len(adapters.parts)), dtype=torch.uint8, device=x.device)
   _here(what, x, a, b, scale, ids, residual, out, workspace)
-  lib.call_array("fh_lora", x.data_ptr(), _TORCH[x.dtype], x.stride()[0] if T > 1 else K, T, K, a.data_ptr(), b.data_ptr(), *sizes, _ptr(scale) or 0, ids.data_ptr(), res, ldr, out.data_ptr(), _TORCH[out.dtype], ldo,
-                 workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream())
+  lib.call_array("fh_lora", xp, xdt, ldx, T, K, a.data_ptr(), b.data_ptr(), *sizes, 0 if scale is None else scale.data_ptr(), of, res, ldr, to, odt, ldo, workspace.data_ptr(),
+                 workspace.nbytes, _stream())
   return out
 
 
