@@ -273,7 +273,7 @@ extern "C" int fh_attention_paged(const void* q, int q_dtype, int64_t ldq, const
   a.page_shift = __builtin_ctz((unsigned)page);
   a.pages = (int)(cache_len >> a.page_shift);
   a.table_cols = (int)std::min<int64_t>(table_cols, 1 << 30);
-  max_context = std::min(max_context, (int64_t)a.table_cols << a.page_shift);
+  max_context = std::min({max_context, (int64_t)a.table_cols << a.page_shift, (int64_t)1 << 30});
   a.max_own = max_context;
   a.rep = heads / kv_heads;
   a.cache_exps = (const uint8_t*)cache + kv_exps_at(cache_dtype, kv_heads, cache_len, head_dim);
@@ -288,7 +288,7 @@ extern "C" int fh_attention_paged(const void* q, int q_dtype, int64_t ldq, const
   a.walkers = a.whole ? sequences : std::max(1, (few ? SQ_CUS * 128 / head_dim : paged_slots(head_dim)) / (kv_heads * a.head_tiles));
   // (the costs' unit: their sum stays below 2^30)
   const int64_t tiles = rows / a.tile_rows + std::min<int64_t>(sequences, rows), cost = max_context + SEQ_START + a.tile_rows;
-  while ((double)tiles * (double)((cost + rows) >> a.unit) >= (double)(1 << 30) && a.unit < 30) ++a.unit;
+  while ((double)tiles * (double)(((cost + rows) >> a.unit) + 1) >= (double)(1 << 30) && a.unit < 30) ++a.unit;
   a.least = std::max(1, (small ? PG_LEAST_TOKENS : PG_LEAST) >> a.unit);
   a.uncut = small ? 0 : PG_UNCUT * head_dim / 128 >> a.unit;
   a.parts = a.walkers > 1 && !a.whole && cost >> a.unit >= a.uncut ? 2 : 1;

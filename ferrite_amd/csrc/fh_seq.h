@@ -175,7 +175,8 @@ struct SeqWalk {
 
   // the cost of the first t tiles of rows behind `place` places
   __device__ static int cost(const SeqArgs& a, int place, int t) {
-    return (int)((int64_t)t * ((clampi(place, 0, a.max_own) + SEQ_START) >> a.unit) + (int64_t)t * (t + 1) / 2 * (a.tile_rows >> a.unit));
+    return (int)((int64_t)t * (((clampi(place, 0, a.max_own) + SEQ_START) >> a.unit) + 1) +  // (a unit at least beyond SEQ_START's)
+                  (int64_t)t * (t + 1) / 2 * (a.tile_rows >> a.unit));
   }
   __device__ static int tiles_of(const SeqArgs& a, int len) { return (len + a.tile_rows - 1) / a.tile_rows; }
   // sequences s0 .. s0 + 63, behind cost `before`: into LDS; the cost up to the last of them
@@ -219,7 +220,7 @@ struct SeqWalk {
   // the tile of the sequence at hand that holds cost x (at <= x)
   __device__ int tile_at(const SeqArgs& a, int x) const {
     if (tiles == 1) return 0;
-    const float r = a.tile_rows >> a.unit, b = (float)((clampi(place, 0, a.max_own) + SEQ_START) >> a.unit) + 0.5f * r, y = (float)(x - at);
+    const float r = a.tile_rows >> a.unit, b = (float)(((clampi(place, 0, a.max_own) + SEQ_START) >> a.unit) + 1) + 0.5f * r, y = (float)(x - at);
     int t = __builtin_amdgcn_readfirstlane(clampi((int64_t)(r > 0.f ? (sqrtf(b * b + 2 * r * y) - b) / r : y / b), 0, tiles - 1));
     while (t > 0 && at + cost(a, place, t) > x) --t;
     while (t + 1 < tiles && at + cost(a, place, t + 1) <= x) ++t;
