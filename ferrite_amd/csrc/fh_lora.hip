@@ -14,8 +14,8 @@
 // (2^-16 of themselves, less than the output's own rounding, 2^-8) and as three for fp32 output (2^-24).
 //
 // What bounds it (MI355X): the bytes, and for few rows the chain of loads. Beside an 8B model's gate and up, rank 32, 4096 rows of 4 adapters, bf16:
-// 147 us for 510 MB, 24 of them u, the rest y's 470 MB read and written at 3.9 TB/s where a copy reaches 5.1; 333 fp32 rows of 6 adapters by 3456
-// 21 us; beside its q, k and v, rank 16, 32 rows of 24 adapters 12.5 us for 11 MB, two launches of 5 and 7.
+// 136 us for 510 MB, 22 of them u, the rest y's 470 MB read and written at 4.2 TB/s where a copy reaches 5.1; 333 fp32 rows of 6 adapters by 3456
+// 20 us; beside its q, k and v, rank 16, 32 rows of 24 adapters 12.5 us for 11 MB, two launches of 5 and 7.
 #include <algorithm>
 #include "fh_common.h"
 
@@ -153,6 +153,52 @@ __device__ __forceinline__ void shrink_rows(const LoraArgs& a, int64_t t0, uint6
 #pragma unroll
   for (int j = 0; j < CB; ++j) wat[j] = ((int64_t)adapter * a.C + c0 + min(16 * j + r, cols - 1)) * a.K;
   const int kw = (a.kstep / 64 + LR_WAVES - 1) / LR_WAVES * 64, kb = k0 + kw * wave, ke = min(kb + kw, k1);  // the wave's
+  if constexpr (XB && WB && MB > 1) {
+    // many rows: 8 lanes in a row fetch 128 bytes in a row of x or A, the next 64 of K while these go through LDS to the operands' layout,
+    // 16 bytes u of a row at u ^ (row / 2) % 8: 4096 rows of 4096 by 64 columns 24.5 -> 21.6 us
+    uint16_t* tile = (uint16_t*)sums + wave * (16 * (MB + CB) * 64);
+    const int part = lane & 7;
+    int64_t at[2 * MB + 2 * CB];
+#pragma unroll
+    for (int i = 0; i < 2 * MB; ++i) at[i] = (t0 + lr_nth(rows, min(8 * i + (lane >> 3), n - 1))) * a.ldx;
+#pragma unroll
+    for (int j = 0; j < 2 * CB; ++j) at[2 * MB + j] = ((int64_t)adapter * a.C + c0 + min(8 * j + (lane >> 3), cols - 1)) * a.K;
+    uint4 v[2 * MB + 2 * CB];
+    auto load = [&](int k) {
+      const bool in = k + 8 * part < ke;
+      const int from = in ? k + 8 * part : 0;
+#pragma unroll
+      for (int i = 0; i < 2 * (MB + CB); ++i) {
+        v[i] = *(const uint4*)((const uint16_t*)(i < 2 * MB ? a.x : a.a) + at[i] + from);
+        if (!in) v[i] = make_uint4(0, 0, 0, 0);
+      }
+    };
+    if (kb < ke) load(kb);
+    for (int k = kb; k < ke; k += 64) {
+      wave_lds_order();  // (the last tile is read)
+#pragma unroll
+      for (int i = 0; i < 2 * (MB + CB); ++i) {
+        const int row = 8 * i + (lane >> 3);
+        *(uint4*)(tile + row * 64 + 8 * (part ^ (row >> 1 & 7))) = v[i];
+      }
+      if (k + 64 < ke) load(k + 64);
+      wave_lds_order();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        auto operand = [&](int block) { return *(const lr_bf16x8*)(tile + (16 * block + r) * 64 + 8 * ((4 * h + g) ^ (r >> 1 & 7))); };
+        lr_bf16x8 xf[MB];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) xf[i] = operand(i);
+#pragma unroll
+        for (int j = 0; j < CB; ++j) {
+          const lr_bf16x8 wf = operand(MB + j);
+#pragma unroll
+          for (int i = 0; i < MB; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i], wf, acc[i][j], 0, 0, 0);
+        }
+      }
+    }
+    __syncthreads();  // (the tiles' place is the sums')
+  } else
   for (int k = kb; k < ke; k += 64) {
     LrRaw<XB> x[2][MB];
     LrRaw<WB> w[2][CB];
@@ -208,7 +254,7 @@ __device__ __forceinline__ void shrink_rows(const LoraArgs& a, int64_t t0, uint6
 // u[part][row][c] = the part of K's products of x's row and A's row c
 template <bool XB, bool WB, int XT, int WT, int CB>
 __global__ __launch_bounds__(64 * LR_WAVES) void lora_shrink(LoraArgs a) {
-  __shared__ __attribute__((aligned(16))) float sums[LR_WAVES * 4 * CB * 256];
+  __shared__ __attribute__((aligned(16))) float sums[LR_WAVES * (XB && WB && CB < 4 ? 512 * (4 + CB) : 4 * CB * 256)];  // (the waves' sums, or their tiles)
   const int split = blockIdx.x % a.splits, c0 = blockIdx.x / a.splits * 16 * CB;
   LoraTile tile(a, blockIdx.z);
   int adapter;
@@ -268,26 +314,31 @@ __device__ __forceinline__ void expand_u(const LoraArgs& a, int64_t t0, uint64_t
   }
 }
 
-// One adapter's rows, the chunk's columns n0 .. n1: y = residual + u B^T, MB blocks of 16 rows at a time. A wave takes whole 128-byte lines of
-// each row. B's rows are the product's rows and x's its columns: two blocks of 16 of B's rows are rows 8 (r / 4) + r % 4 and those 4
-// on, so that a lane ends with 8 consecutive columns of y's row, 16 or 32 bytes.
+// One adapter's rows, the chunk's columns n0 .. n1: y = residual + u B^T, MB blocks of 16 rows at a time. B's rows are the product's rows and
+// x's its columns: two blocks of 16 of B's rows are rows 8 (r / 4) + r % 4 and those 4 on, so that a lane ends with 8 consecutive columns
+// of x's row r. They go through LDS (`tile`, the wave's own) to where 8 lanes in a row hold 128 bytes in a row of y: as the products leave them,
+// each lane's 16 bytes in a row of their own, 4096 rows of 28672 take 123 us rather than 113.
+template <bool YB, int MB>
+struct LrTile {
+  static constexpr int COLS = YB ? 64 : 32, LD = COLS + 4, SIZE = 16 * MB * LD;  // floats
+};
 template <bool WB, bool YB, int UT, int WT, int MB>
-__device__ __forceinline__ void expand_rows(const LoraArgs& a, int64_t t0, uint64_t rows, int n, int adapter, int n0, int n1, const uint16_t* us, int ldu) {
+__device__ __forceinline__ void expand_rows(const LoraArgs& a, int64_t t0, uint64_t rows, int n, int adapter, int n0, int n1, const uint16_t* us, int ldu, float* tile) {
+  using Tile = LrTile<YB, MB>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int steps = (a.rank + 31) / 32;
-  constexpr int CG = YB ? 2 : 1;
+  constexpr int CG = Tile::COLS / 32, V = YB ? 8 : 4, IT = 2 * MB;  // a lane's columns of 16 bytes; rounds of 8 rows
   const int64_t wbase = (int64_t)adapter * a.N * a.rank;
   for (int m0 = 0; m0 < n; m0 += 16 * MB) {
-    int64_t row[MB];
+    int64_t row[IT];  // the rows whose 16 bytes the lane moves
 #pragma unroll
-    for (int i = 0; i < MB; ++i) row[i] = t0 + lr_nth(rows, min(m0 + 16 * i + r, n - 1));
-    for (int c = n0 + 32 * CG * wave; c < n1; c += 32 * CG * LR_WAVES) {
-      LrRaw<YB> res[MB][CG];
+    for (int i = 0; i < IT; ++i) row[i] = t0 + lr_nth(rows, min(m0 + 8 * i + (lane >> 3), n - 1));
+    for (int c = n0 + Tile::COLS * wave; c < n1; c += Tile::COLS * LR_WAVES) {
+      const int col = c + V * (lane & 7);
+      uint4 res[IT];
       if (a.residual)
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int q = 0; q < CG; ++q) res[i][q].load(a.residual, row[i] * a.ldr + min(c + 32 * q + 8 * g, n1 - 8));
+        for (int i = 0; i < IT; ++i) res[i] = *(const uint4*)((const char*)a.residual + (row[i] * a.ldr + min(col, n1 - V)) * (YB ? 2 : 4));
       lr_floatx4 acc[MB][CG][2];
 #pragma unroll
       for (int i = 0; i < MB; ++i)
@@ -315,17 +366,33 @@ __device__ __forceinline__ void expand_rows(const LoraArgs& a, int64_t t0, uint6
             for (int i = 0; i < MB; ++i) acc[i][q][e] = lr_mfma<WT, UT>(bf, uf[i], acc[i][q][e]);
           }
       }
+      wave_lds_order();  // (the last columns are read)
 #pragma unroll
       for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int q = 0; q < CG; ++q) {
-          const int col = c + 32 * q + 8 * g;  // the lane's 8 columns of y
-          float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          if (a.residual) res[i][q].values(f);
+        for (int q = 0; q < CG; ++q)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] += acc[i][q][e >> 2][e & 3];
-          if (m0 + 16 * i + r < n && col < n1) lr_write8<YB>(a.y, row[i] * a.ldy + col, f);
+          for (int e = 0; e < 2; ++e) *(lr_floatx4*)(tile + (16 * i + r) * Tile::LD + 32 * q + 8 * g + 4 * e) = acc[i][q][e];
+      wave_lds_order();
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const float* from = tile + (8 * i + (lane >> 3)) * Tile::LD + V * (lane & 7);
+        if (m0 + 8 * i + (lane >> 3) >= n || col >= n1) continue;
+        uint32_t w[4] = {res[i].x, res[i].y, res[i].z, res[i].w};
+        if (!a.residual) w[0] = w[1] = w[2] = w[3] = 0;
+        const lr_floatx4 f = *(const lr_floatx4*)from;
+        if constexpr (YB) {
+          const lr_floatx4 h = *(const lr_floatx4*)(from + 4);
+          const float v[8] = {f[0], f[1], f[2], f[3], h[0], h[1], h[2], h[3]};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e] = bf16_rne_f(__uint_as_float(w[e] << 16) + v[2 * e]) | (bf16_rne_f(__uint_as_float(w[e] & 0xFFFF0000u) + v[2 * e + 1]) << 16);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) + f[e]);
         }
+        *(uint4*)((char*)a.y + (row[i] * a.ldy + col) * (YB ? 2 : 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
     }
   }
 }
@@ -334,6 +401,7 @@ __device__ __forceinline__ void expand_rows(const LoraArgs& a, int64_t t0, uint6
 template <bool WB, bool YB, int UT, int WT>
 __global__ __launch_bounds__(64 * LR_WAVES, WB ? 4 : 3) void lora_expand(LoraArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint16_t us[];  // [UT][64][ldu] u's terms
+  __shared__ __attribute__((aligned(16))) float turn[LR_WAVES * LrTile<YB, 2>::SIZE];
   int part = 0;
   while (part + 1 < a.parts && (int)blockIdx.x >= a.chunk0[part + 1]) ++part;
   const int n0 = a.col0[part] + (blockIdx.x - a.chunk0[part]) * a.width, n1 = min(n0 + a.width, a.col0[part + 1]);
@@ -363,8 +431,9 @@ __global__ __launch_bounds__(64 * LR_WAVES, WB ? 4 : 3) void lora_expand(LoraArg
     again = true;
     expand_u<UT>(a, tile.t0, rows, n, adapter, part, us, ldu);
     __syncthreads();
-    if (n <= 16) expand_rows<WB, YB, UT, WT, 1>(a, tile.t0, rows, n, adapter, n0, n1, us, ldu);
-    else expand_rows<WB, YB, UT, WT, 2>(a, tile.t0, rows, n, adapter, n0, n1, us, ldu);
+    float* mine = turn + (threadIdx.x >> 6) * LrTile<YB, 2>::SIZE;
+    if (n <= 16) expand_rows<WB, YB, UT, WT, 1>(a, tile.t0, rows, n, adapter, n0, n1, us, ldu, mine);
+    else expand_rows<WB, YB, UT, WT, 2>(a, tile.t0, rows, n, adapter, n0, n1, us, ldu, mine);
   }
 }
 
@@ -496,7 +565,7 @@ __global__ __launch_bounds__(64 * LR_FEW_WAVES) void lora_few(LoraArgs a) {
 // Parts of K: whole steps of 256 (a wave's 64 each), as many as keep the parts' rows within 16384, so that u's parts stay a
 // small share of what a call moves and a decode step's few rows still fill the GPU.
 constexpr int LR_MAX_SPLITS = 32;
-constexpr int64_t LR_SPLIT_ROWS = 16384;
+constexpr int64_t LR_SPLIT_ROWS = 16384;  // (32768: 4096 rows 136 -> 146 us)
 static int lora_splits(int64_t rows, int64_t K) {
   const int64_t most = std::min<int64_t>(LR_MAX_SPLITS, (K + 255) / 256);
   return (int)std::max<int64_t>(1, std::min(most, LR_SPLIT_ROWS / rows));
