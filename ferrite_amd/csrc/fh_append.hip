@@ -182,10 +182,11 @@ __global__ __launch_bounds__(1024) void append_kernel(AppendArgs a) {
   }
 }
 
+static int append_threads(int heads, int kv_heads, int head_dim) { return std::min(1024, ((heads + 2 * kv_heads) * (head_dim / 8) + 63) / 64 * 64); }
+
 template <int HD, int CF>
 static void launch_append(bool bf, hipStream_t s, const AppendArgs& a) {
-  const int lanes = (a.heads + 2 * a.kv_heads) * (HD / 8);
-  const dim3 b(std::min(1024, (lanes + 63) / 64 * 64));
+  const dim3 b(append_threads(a.heads, a.kv_heads, HD));
   auto launch = [&](auto rows) {
     constexpr int R = decltype(rows)::value;
     const dim3 g((unsigned)((a.rows + R - 1) / R));
@@ -235,6 +236,9 @@ extern "C" int fh_rope_append_paged(const void* qkv, int x_dtype, int64_t ldx, i
     return no(FH_EINVAL, "rows at least their heads, qkv's and q's aligned to 4 values, the cache to 16 bytes");
   if (((uintptr_t)q_norm & 15) || ((uintptr_t)k_norm & 15) || ((uintptr_t)cos_tab & 15) || ((uintptr_t)sin_tab & 15))
     return no(FH_EINVAL, "norms and tables 16-byte aligned");
+  if (q == qkv && rows > 1 && (ldq != ldx || q_dtype != x_dtype)) return no(FH_EINVAL, "q in qkv's own columns has qkv's type and its rows");
+  // (a grid's work-items are counted in 32 bits)
+  if (rows * append_threads(heads, kv_heads, head_dim) >= (1LL << 32)) return no(FH_EUNSUP, "too many rows for one grid");
   AppendArgs a = {};
   a.x = qkv; a.ldx = ldx; a.rows = rows; a.n = sequences; a.heads = heads; a.kv_heads = kv_heads;
   a.q_norm = q_norm; a.k_norm = k_norm; a.eps = eps; a.centered = centered;

@@ -571,12 +571,14 @@ static int lora_splits(int64_t rows, int64_t K) {
   return (int)std::max<int64_t>(1, std::min(most, LR_SPLIT_ROWS / rows));
 }
 
-// One launch where a part's rows of A are at most LR_FEW_BYTES and those of all adapters that the rows may have LR_FEW_ALL: smollm's q, k
-// and v of 1 row 8.0 -> 5.1 us, an 8B o of 4 rows with as many adapters 9.1 either way, its q, k and v of 32 with 24 12.5 against 15.2.
+// One launch where a part's rows of A are at most LR_FEW_BYTES, those of all adapters that the rows may have LR_FEW_ALL, and the rank 32, 16 of
+// fp32 weights (more do not fit the registers of 16 waves): smollm's q, k and v of 1 row 8.0 -> 5.1 us; of 16 rows with 8 adapters
+// of rank 32 9.7 -> 8.2, of rank 64 10.5 against 9.7 but 10.2 -> 11.9 at K of 1024, in fp32 of rank 16 11.7 -> 8.8, of rank 32 12.2 against 13.1;
+// an 8B o of 4 rows with as many adapters 9.1 either way, its q, k and v of 32 with 24 12.5 against 15.2.
 constexpr int64_t LR_FEW_BYTES = 160 << 10, LR_FEW_ALL = 1 << 20;
 static bool lora_is_few(int64_t rows, int64_t K, int rank, int adapters, int w_dtype) {
   const int64_t bytes = rank * K * (w_dtype == FH_F32 ? 4 : 2);
-  return rows <= LR_ROWS && rank <= 64 && bytes <= LR_FEW_BYTES && bytes * std::min<int64_t>(rows, adapters) <= LR_FEW_ALL;
+  return rows <= LR_ROWS && rank <= (w_dtype == FH_F32 ? 16 : 32) && bytes <= LR_FEW_BYTES && bytes * std::min<int64_t>(rows, adapters) <= LR_FEW_ALL;
 }
 
 template <bool XB, bool WB, bool YB>
@@ -584,9 +586,8 @@ static void launch_lora(bool few, hipStream_t s, const LoraArgs& a) {
   constexpr int T = YB ? 2 : 3, XT = XB ? 1 : T, WT = WB ? 1 : T;
   if (few) {
     const dim3 g(a.chunk0[a.parts], a.share, 1), b(64 * LR_FEW_WAVES);
-    if (a.rank <= 16) hipLaunchKernelGGL((lora_few<XB, WB, YB, XT, WT, T, 1>), g, b, 0, s, a);
-    else if (a.rank <= 32) hipLaunchKernelGGL((lora_few<XB, WB, YB, XT, WT, T, 2>), g, b, 0, s, a);
-    else hipLaunchKernelGGL((lora_few<XB, WB, YB, XT, WT, T, 4>), g, b, 0, s, a);
+    if (!WB || a.rank <= 16) hipLaunchKernelGGL((lora_few<XB, WB, YB, XT, WT, T, 1>), g, b, 0, s, a);
+    else if constexpr (WB) hipLaunchKernelGGL((lora_few<XB, WB, YB, XT, WT, T, 2>), g, b, 0, s, a);
     return;
   }
   // u's columns in equal groups of up to 4 blocks of 16
@@ -643,6 +644,7 @@ extern "C" int fh_lora(const void* x, int x_dtype, int64_t ldx, int64_t rows, in
   l.splits = lora_splits(rows, K);
   const size_t need = (size_t)l.splits * rows * rank * parts * sizeof(float);
   if (!workspace || ws_bytes < need || ((uintptr_t)workspace & 15)) return no(FH_EINVAL, "a 16-byte aligned workspace of fh_lora_workspace_bytes");
+  if (x == y) return no(FH_EINVAL, "y is not x (a row's x is read until its last column is done)");
   l.x = x; l.ldx = ldx; l.rows = rows; l.K = K; l.a = a_w; l.b = b_w; l.scale = scale; l.ids = ids;
   l.adapters = adapters; l.rank = rank; l.parts = parts; l.C = rank * parts; l.N = (int)N;
   l.kstep = (int)((K + 64 * l.splits - 1) / (64 * l.splits)) * 64;

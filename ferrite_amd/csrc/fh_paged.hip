@@ -1,6 +1,13 @@
 // Attention of ragged rows over a KV cache in pages: prompts, chunks of them and single tokens in one call. A sequence's place p
 // lies at row table[p / page] page + p % page of the cache, and a query at place p sees places 0 .. p:
-// o = sum_k softmax_k(q k / sqrt(hd)) v.
+// o = sum_k softmax_k(q k / sqrt(hd)) v. Tiles of (row, head of a key head) pairs against tiles of keys with an online softmax, as
+// packed prompts have them (fh_seq.h); what is its own is the pages' reads, how the work is shared (SeqWalk) and token_kernel.
+// What bounds it (MI355X; 32 heads of 128, 8 key heads, bf16 cache; kernels alone): a decode step the reads, 48 tokens after up to
+// 8000 places 160 us (890 MB: 5.5 TB/s, a plain read's rate) and 5 the join of the shares' parts; with fewer keys the chain of a
+// table's page, its rows and the two products: 16 after up to 2000 18 us and 4 (53 MB, 10 at that rate), one launch for 4 short
+// ones 7.3. Prompts the products: 24 of up to 512 rows or single tokens after up to 4000 places 202 us (95 GF of pairs, 180 with the
+// weights' second term and the unseen pairs of a tile: 890 TFLOP/s) and 20 the join (58 MB of parts). A bfp8 cache's runs are decoded by
+// every workgroup that reads them: 11 of up to 250, 16 heads of 64, 28 us and 15.
 #include "fh_seq.h"
 
 namespace fh {
@@ -284,7 +291,8 @@ extern "C" int fh_attention_paged(const void* q, int q_dtype, int64_t ldq, const
   a.tile_rows = std::max(1, pairs / a.rep);
   a.head_tiles = (a.rep + pairs - 1) / pairs;
   a.slot_pairs = (int)std::min<int64_t>(pairs, rows * a.rep);
-  a.whole = tokens && rows <= sequences && max_context <= (few ? PG_WHOLE_FEW : PG_WHOLE);
+  a.whole = tokens && rows <= sequences && max_context <= (few ? PG_WHOLE_FEW : PG_WHOLE) &&
+            (int64_t)sequences * kv_heads * a.head_tiles < (1 << 24);  // (a grid's work-items are counted in 32 bits)
   a.walkers = a.whole ? sequences : std::max(1, (few ? SQ_CUS * 128 / head_dim : paged_slots(head_dim)) / (kv_heads * a.head_tiles));
   // (the costs' unit: their sum stays below 2^30)
   const int64_t tiles = rows / a.tile_rows + std::min<int64_t>(sequences, rows), cost = max_context + SEQ_START + a.tile_rows;
@@ -298,7 +306,6 @@ extern "C" int fh_attention_paged(const void* q, int q_dtype, int64_t ldq, const
   if (a.parts > 1 && (!workspace || ws_bytes < parts_bytes(2 * blocks * a.slot_pairs, head_dim) || ((uintptr_t)workspace & 15)))
     return fail(FH_EINVAL, "fh_attention_paged: a 16-byte aligned workspace of fh_attention_paged_workspace_bytes");
   if (few) {
-    if (blocks >= (1LL << 31)) return fail(FH_EUNSUP, "fh_attention_paged: too many rows for one grid");
     if (head_dim == 128) launch_tokens<128>((unsigned)blocks, as_stream(stream), a);
     else launch_tokens<64>((unsigned)blocks, as_stream(stream), a);
     return check_launch(fn);

@@ -965,7 +965,7 @@ __global__ __launch_bounds__(TOKENS || HD == 64 ? 512 : 1024) void seq_join_page
   if (k <= 0 || k >= n || cut(first) > 0) return;
   // the parts: of share `first`, from the tile's first key on, and of those behind it up to the one that ends it
   int last = first + 1;
-  while (cut(last + 1) < n) ++last;
+  while (last + 1 < a.walkers && cut(last + 1) < n) ++last;
   const int parts = last - first + 1, lane = threadIdx.x & 63, row = t * a.tile_rows;
   const int pair0 = head % a.head_tiles * a.slot_pairs, pairs = min(a.slot_pairs, (a.head_tiles > 1 ? a.rep : min(a.tile_rows, w.len - row) * a.rep) - pair0);
   auto part = [&](int i, int p) { return a.part + ((int64_t)(((first + i) * heads + head) * 2 + (i == 0)) * a.slot_pairs + p) * (HD + 2); };

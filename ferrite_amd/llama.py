@@ -614,7 +614,7 @@ class PageStep:
     c, dev = dec.c, dec.device
     self._int = torch.zeros(2 * n + n * pages + n, dtype=torch.int32, device=dev)
     self.ids, self.p0, self.of, self.tables = self._int.split([n, n, n, n * pages])
-    self.tables = self.tables.view(n, pages)
+    self.tables = self.tables.view(n, pages).fill_(-1)  # (a step before any set puts nothing into the cache)
     self.starts = torch.arange(n + 1, dtype=torch.int32, device=dev)
     self.bufs = dec._page_buffers(n, self.adapters)
     self.ws = ops.attention_paged_workspace(n, n, c.heads, c.kv, dec.hd, pages * page, dev)

@@ -602,6 +602,8 @@ class Adapters:
     cols = (ctypes.c_int64 * len(parts))(*parts)
     object.__setattr__(self, "_call", (K, N, r, (_TORCH[a.dtype], n, r, len(parts), ctypes.addressof(cols)), cols))  # (what a call passes of the sizes)
 
+  def __reduce__(self): return Adapters, (self.a, self.b, self.scale, self.parts)  # (a copy has sizes of its own)
+
   @property
   def rank(self): return self.b.shape[2]
 

@@ -1,6 +1,6 @@
 """What the operators over a cache in pages and the low-rank adapters refuse, on the host before any launch (no GPU needed: every call
 here fails its checks), and their workspaces' sizes."""
-import ctypes
+import copy, ctypes, pickle
 import pytest
 import torch
 from ferrite_amd import lib, ops
@@ -49,10 +49,11 @@ def test_attention_refuses(kw, err):
   (dict(n=0), ValueError), (dict(heads=0), ValueError), (dict(kv=0), ValueError), (dict(hd=96), NotImplementedError), (dict(xd=lib.BFP8), ValueError), (dict(qd=lib.BF16_T16), ValueError),
   (dict(cd=lib.I32), NotImplementedError), (dict(sin=None), ValueError), (dict(turns=0), ValueError), (dict(page=8), NotImplementedError), (dict(page=64), ValueError),
   (dict(len=8), ValueError), (dict(len=1 << 30), NotImplementedError), (dict(cols=0), ValueError), (dict(ldt=5), ValueError), (dict(ldx=767), ValueError), (dict(ldx=764), ValueError),
-  (dict(ldq=510), ValueError), (dict(x=P + 4), ValueError), (dict(q=P + 4), ValueError), (dict(cache=P + 8), ValueError), (dict(qn=P + 4), ValueError), (dict(cos=P + 8), ValueError)])
+  (dict(ldq=510), ValueError), (dict(x=P + 4), ValueError), (dict(q=P + 4), ValueError), (dict(cache=P + 8), ValueError), (dict(qn=P + 4), ValueError), (dict(cos=P + 8), ValueError),
+  (dict(), ValueError), (dict(ldq=768, qd=lib.BF16), ValueError), (dict(ldq=768, rows=1 << 25), NotImplementedError)])
 def test_append_refuses(kw, err):
   lib.load()
-  with pytest.raises(err, match="fh_rope_append_paged"): append(**kw)
+  with pytest.raises(err, match="fh_rope_append_paged"): append(**kw)  # (the last but two: q in qkv's columns with rows of its own)
 
 
 @needs_lib
@@ -63,10 +64,11 @@ def test_append_refuses(kw, err):
   (dict(parts=5, cols=(8,) * 5), NotImplementedError), (dict(cols=(32, 12)), NotImplementedError), (dict(cols=(32, 0)), NotImplementedError),
   (dict(cols=(1 << 29, 1 << 29)), NotImplementedError), (dict(xd=lib.BFP8), ValueError), (dict(wd=lib.BFP8), ValueError), (dict(yd=lib.BF16_T16), ValueError),
   (dict(ldx=56), ValueError), (dict(ldx=66), ValueError), (dict(ldy=40), ValueError), (dict(ldy=50), ValueError), (dict(ldr=44), ValueError), (dict(ldr=52), ValueError),
-  (dict(x=P + 8), ValueError), (dict(b=P + 8), ValueError), (dict(y=P + 8, res=None), ValueError), (dict(ws=None), ValueError), (dict(wb=16), ValueError), (dict(ws=P + 8), ValueError)])
+  (dict(x=P + 8), ValueError), (dict(b=P + 8), ValueError), (dict(y=P + 8, res=None), ValueError), (dict(ws=None), ValueError), (dict(wb=16), ValueError), (dict(ws=P + 8), ValueError),
+  (dict(), ValueError)])
 def test_lora_refuses(kw, err):
   lib.load()
-  with pytest.raises(err, match="fh_lora"): lora(**kw)
+  with pytest.raises(err, match="fh_lora"): lora(**kw)  # (the last: y is x)
 
 
 @needs_lib
@@ -94,3 +96,12 @@ def test_python_refuses_what_is_not_on_the_gpu_or_misshapen():
   with pytest.raises(ValueError, match="on the GPU"): ops.lora(q, ops.Adapters(torch.zeros(1, 8, 128), torch.zeros(1, 8, 8), None, (8,)), i(4))
   with pytest.raises(ValueError, match="parts"): ops.lora(q, ops.Adapters(torch.zeros(1, 8, 128), torch.zeros(1, 8, 8), None, (16,)), i(4))
   with pytest.raises(ValueError, match="alike"): ops.lora(q, ops.Adapters(torch.zeros(1, 8, 128), torch.zeros(1, 8, 8, dtype=torch.bfloat16), None, (8,)), i(4))
+
+
+def test_a_copy_of_adapters_has_sizes_of_its_own():
+  # (a call passes the parts' address: a copy's must outlive the adapters that it was made from)
+  ad = ops.Adapters(torch.zeros(2, 16, 64), torch.zeros(2, 24, 8), None, (16, 8))
+  for other in (copy.copy(ad), copy.deepcopy(ad), pickle.loads(pickle.dumps(ad))):
+    cols = other._call[4]
+    assert other.parts == ad.parts and tuple(cols) == (16, 8) and cols is not ad._call[4]
+    assert other._call[3][4] == ctypes.addressof(cols) != ad._call[3][4]
