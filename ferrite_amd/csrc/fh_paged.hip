@@ -246,8 +246,12 @@ using namespace fh;
 // (token_kernel: PG_WHOLE_FEW) places takes a workgroup a sequence and key head instead and needs no second launch: 8 sequences of up to
 // 500 11.7 us, shared out 13.8; 16 of up to 2000 30.5, 23.1. The rest is what was measured best: the least share of a workgroup, and
 // the cost from which a tile of 128 pairs of 128 dimensions is cut (its parts are 66 KB each, written and read: 16 prompts of up to 300 38 us,
-// with every tile cut 55; a cost of 960 instead 4 of up to 2048 156 -> 149).
+// with every tile cut 55). Prompts of tiles enough for every workgroup that the GPU holds, no sequence of which may outweigh the others' (PG_EACH:
+// rows a sequence times rounds of tiles against max_context), go a tile a workgroup as they come, a sequence's longest first, without cuts
+// or a join: 16 of 100 to 400 rows 54 -> 45 us, 4 of 1024 to 2048 185 -> 158, one of 2048 96 -> 85, 16 of 512 after up to 4000 places 600 -> 531;
+// but 8 of these 233 -> 243, 6 of them beside 24 tokens 272 -> 304, and over an fp32 cache 4 of up to 1500 575 -> 717.
 constexpr int PG_WHOLE = 448, PG_WHOLE_FEW = 1024, PG_LEAST_TOKENS = 128, PG_LEAST = 256, PG_UNCUT = 512;
+constexpr int PG_EACH = 4;
 static int paged_slots(int head_dim) { return SQ_CUS * (head_dim == 64 ? 3 : 2); }
 
 extern "C" size_t fh_attention_paged_workspace_bytes(int64_t rows, int sequences, int heads, int kv_heads, int head_dim,
@@ -300,6 +304,10 @@ extern "C" int fh_attention_paged(const void* q, int q_dtype, int64_t ldq, const
   a.least = std::max(1, (small ? PG_LEAST_TOKENS : PG_LEAST) >> a.unit);
   a.uncut = small ? 0 : PG_UNCUT * head_dim / 128 >> a.unit;
   a.parts = a.walkers > 1 && !a.whole && cost >> a.unit >= a.uncut ? 2 : 1;
+  const double each = (double)tiles * kv_heads * a.head_tiles, rounds = each / paged_slots(head_dim);
+  if (!small && rounds >= 1 && each < (1 << 24) && max_context < (1 << 29) && rounds * PG_EACH * rows >= (double)max_context * sequences) {
+    a.unit = 30; a.least = 1; a.walkers = (int)tiles; a.parts = 1;  // (a cost of 1 a tile, a share of one)
+  }
   if (a.parts == 1) a.uncut = 0x7FFFFFFF;
   a.part = (float*)workspace;
   const int64_t blocks = (int64_t)a.walkers * kv_heads * a.head_tiles;

@@ -757,7 +757,8 @@ __device__ __forceinline__ void seq_items(const SeqArgs& a, Work work) {
   if constexpr (FORM != SEQ_PAGED) {
     if (seq_item<BQ, FORM>(a, it)) work(it);
   } else {
-    const int heads = a.kv_heads * a.head_tiles, me = blockIdx.x / heads, head = blockIdx.x % heads;
+    const int heads = a.kv_heads * a.head_tiles, head = blockIdx.x % heads;
+    const int me = a.parts > 1 ? blockIdx.x / heads : a.walkers - 1 - blockIdx.x / heads;  // (without cuts: a sequence's longest tile first)
     it.kvh = head / a.head_tiles;
     it.split = it.splits = it.part = it.shared = 0; it.prefix = it.own = 0; it.step = 1;
     __shared__ __attribute__((aligned(16))) int4 held[64 * SQ_NW];

@@ -90,6 +90,16 @@ def test_strides_and_rows_behind(cuda):
     assert (got[:5] == 7).all() and (got[5 + sum(lens):] == 7).all()
 
 
+@pytest.mark.parametrize("heads,kv,hd,fmt,q,o", [(64, 64, 128, "bf16", "bf16", "bf16"), (80, 80, 64, "bf16", "fp32", "fp32"), (64, 64, 128, "bfp8", "fp32", "bf16"),
+                                                 (80, 80, 64, "bfp4", "bf16", "fp32")])
+def test_many_tiles(cuda, heads, kv, hd, fmt, q, o):
+  # more tiles of prompts than workgroups that the GPU holds: a tile a workgroup, with sequences of none and one among them
+  lens, before = [300, 1, 0, 129, 128, 142], [0, 30, 5, 0, 17, 0]
+  got, want, tol = paged(20, heads, kv, hd, lens, before, 16, fmt, q, o, ahead=3, pad=9)
+  S.check(got, want, tol, (heads, hd, fmt))
+  assert (got[:3] == 7).all() and (got[3 + sum(lens):] == 7).all()
+
+
 def test_long_contexts(cuda):
   # few rows after many (the keys' long axis), with the bound of the context far above what is there
   got, want, tol = paged(4, 8, 2, 128, [3, 40], [2000, 1111], 64, slack=3000)
