@@ -69,6 +69,7 @@ SIGNATURES = {
   "fh_attention_paged": ([P, I, L, P, I, L, L, I, I, I, I, P, P, P, L, L, I, L, P, I, L, P, S, P], I),
   "fh_lora_workspace_bytes": ([L, L, I, I], S),
   "fh_lora": ([P, I, L, L, L, P, P, I, I, I, I, ctypes.POINTER(L), P, P, P, L, P, I, L, P, S, P], I),
+  "fh_silu_gate_rows": ([P, I, L, L, L, P, I, L, P], I),
   "fh_call": ([I, ctypes.c_char_p], I),
   "fh_rms_rows": ([P, L, L, L, P, ctypes.c_float, I, P, I, L, P], I),
   "fh_moe_route": ([P, L, I, L, P, ctypes.c_float, I, P, I, I, I, I, P, P, P, P], I),

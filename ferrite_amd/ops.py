@@ -803,20 +803,13 @@ def logit_rules(logits, tokens=None, lengths=None, prompt_lengths=None, repetiti
 
 
 def silu_gate_rows(x, split, out):
-  """silu(gate) * up of rows x [T][2 split] (fp32 or bf16: gate's columns, then up's) into out [T][split] (fp32 or bf16): FH_EP_SILU_GATE
-  for a product that something is added to first (fh_map)."""
-  _dev(x, out)
-  if x.dtype not in _TORCH or out.dtype not in _TORCH or x.shape[1] != 2 * split or out.shape != (x.shape[0], split) or x.stride(1) != 1 or out.stride(1) != 1:
-    raise ValueError(f"silu_gate_rows: x [T][{2 * split}] and out [T][{split}], fp32 or bf16 with contiguous rows")
-  p = lib.Program()
-  g, u, imm = 16, 17, lib.OPND_IMM
-  steps = [("mul", g, imm, -1.0), ("exp", 0, 0, 0.0), ("add", 1, imm, 1.0), ("recip", 2, 2, 0.0), ("mul", g, 3, 0.0), ("mul", 4, u, 0.0)]
-  p.n_ops, p.n_inputs = len(steps), 2
-  for i, (op, a, b, v) in enumerate(steps): p.op[i], p.a[i], p.b[i], p.imm[i] = lib.OP[op], a, b, v
-  for i in range(2):
-    p.input[i], p.in_dtype[i] = x.data_ptr() + i * split * x.element_size(), _TORCH[x.dtype]
-    p.in_stride[i][1], p.in_stride[i][2] = x.stride(0), 1
-  lib.call("fh_map", ctypes.byref(p), _ptr(out), _TORCH[out.dtype], 1, x.shape[0], split, x.shape[0] * out.stride(0), out.stride(0), _stream())
+  """silu(gate) * up of rows x [T][2 split] (fp32 or bf16: gate's columns, then up's) into out [T][split] (fp32 or bf16), which is not x:
+  FH_EP_SILU_GATE for a product that something is added to first (fh_silu_gate_rows)."""
+  what = "silu_gate_rows"
+  xp, xdt, ldx, T = _rows_of(what, "x", x, None, 2 * split)
+  to, odt, ldo, _ = _rows_of(what, "out", out, T, split)
+  _here(what, x, out)
+  lib.call("fh_silu_gate_rows", xp, xdt, ldx, T, split, to, odt, ldo, _stream())
   return out
 
 

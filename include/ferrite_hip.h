@@ -353,7 +353,11 @@ int fh_lora(const void* x, int x_dtype, int64_t ldx, int64_t rows, int64_t K, co
             int rank, int parts, const int64_t* part_cols, const float* scale, const int32_t* ids, const void* residual, int64_t ldr,
             void* y, int y_dtype, int64_t ldy, void* workspace, size_t ws_bytes, void* stream);
 
-/* The three calls above with their arguments in an array, in order, 8 bytes each (integers and pointers as int64_t, eps as a double):
+/* y[row][c] = silu(x[row][c]) x[row][split + c], rows [rows][ldx] and [rows][ldy] FH_F32 or FH_BF16: FH_EP_SILU_GATE for a product that adapters
+ * are added to first (models/llama.py:266-275). split a multiple of 8, rows 16-byte aligned; y does not overlap x. */
+int fh_silu_gate_rows(const void* x, int x_dtype, int64_t ldx, int64_t rows, int64_t split, void* y, int y_dtype, int64_t ldy, void* stream);
+
+/* fh_rope_append_paged, fh_attention_paged and fh_lora with their arguments in an array, in order, 8 bytes each (integers and pointers as int64_t, eps as a double):
  * for bindings that convert arguments one by one (ctypes: 5 to 6 us of a call of 22 to 28, 1.5 us for the array). */
 #define FH_CALL_ROPE_APPEND_PAGED 0
 #define FH_CALL_ATTENTION_PAGED 1

@@ -190,3 +190,18 @@ def test_pack_adapters(cuda):
   assert ((got - want).abs() <= tol).all()
   with pytest.raises(ValueError): ops().pack_adapters([[(m(4, 96), m(32, 4))]], (32, 16))
   with pytest.raises(ValueError): ops().pack_adapters([[(m(4, 96), m(30, 4)), None]], (32, 16))
+
+
+@pytest.mark.parametrize("x,o", [("fp32", "bf16"), ("bf16", "fp32"), ("fp32", "fp32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("T,split", [(1, 8), (3, 1544), (70, 264)])
+def test_silu_gate_rows(cuda, T, split, x, o):
+  # expf within 2 units (2^-22 of it), its sum, the quotient and the product a rounding each (2^-24), o's own: 2^-21 with room
+  dt = dict(fp32=torch.float32, bf16=torch.bfloat16)
+  buf = (torch.randn(T, 2 * split + 16, device="cuda") * 8).to(dt[x])
+  out = torch.full((T, split + 8), 7.0, dtype=dt[o], device="cuda")
+  buf[0, 0], buf[0, split] = -200., 3.  # (a gate whose exponential overflows: 0)
+  got = ops().silu_gate_rows(buf[:, :2 * split], split, out[:, :split])
+  g, u = buf[:, :split].double().cpu(), buf[:, split:2 * split].double().cpu()
+  want = g * torch.sigmoid(g) * u
+  tol = want.abs() * (2.0 ** -21 + torch.finfo(dt[o]).eps / 2) + 2.0 ** -126
+  assert ((got.double().cpu() - want).abs() <= tol).all() and (out[:, split:] == 7).all()

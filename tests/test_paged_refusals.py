@@ -72,6 +72,17 @@ def test_lora_refuses(kw, err):
 
 
 @needs_lib
+@pytest.mark.parametrize("kw,err", [
+  (dict(x=None), ValueError), (dict(y=None), ValueError), (dict(rows=0), ValueError), (dict(split=0), ValueError), (dict(xd=lib.BFP8), ValueError), (dict(yd=lib.BF16_T16), ValueError),
+  (dict(split=12), NotImplementedError), (dict(ldx=60), ValueError), (dict(ldx=66), ValueError), (dict(ldy=28), ValueError), (dict(ldy=34), ValueError), (dict(x=P + 8), ValueError),
+  (dict(y=P + 8), ValueError), (dict(rows=1 << 40), NotImplementedError)])
+def test_silu_gate_refuses(kw, err):
+  lib.load()
+  a = dict(x=P, xd=lib.F32, ldx=64, rows=4, split=32, y=P + 1024, yd=lib.F32, ldy=32) | kw
+  with pytest.raises(err, match="fh_silu_gate_rows"): lib.call("fh_silu_gate_rows", *a.values(), None)
+
+
+@needs_lib
 def test_workspace_sizes():
   L = lib.load()
   pg, lo = L.fh_attention_paged_workspace_bytes, L.fh_lora_workspace_bytes
