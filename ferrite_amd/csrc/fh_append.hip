@@ -236,7 +236,7 @@ extern "C" int fh_rope_append_paged(const void* qkv, int x_dtype, int64_t ldx, i
     return no(FH_EINVAL, "rows at least their heads, qkv's and q's aligned to 4 values, the cache to 16 bytes");
   if (((uintptr_t)q_norm & 15) || ((uintptr_t)k_norm & 15) || ((uintptr_t)cos_tab & 15) || ((uintptr_t)sin_tab & 15))
     return no(FH_EINVAL, "norms and tables 16-byte aligned");
-  if (q == qkv && rows > 1 && (ldq != ldx || q_dtype != x_dtype)) return no(FH_EINVAL, "q in qkv's own columns has qkv's type and its rows");
+  if (q == qkv && (q_dtype != x_dtype || (rows > 1 && ldq != ldx))) return no(FH_EINVAL, "q in qkv's own columns has qkv's type and its rows");
   // (a grid's work-items are counted in 32 bits)
   if (rows * append_threads(heads, kv_heads, head_dim) >= (1LL << 32)) return no(FH_EUNSUP, "too many rows for one grid");
   AppendArgs a = {};

@@ -1,0 +1,37 @@
+"""The Decoder's steps over a cache in pages, on the host (no GPU: its buffers on the CPU, the integers that a launch would carry written
+there): what a step is given, and what is refused before anything runs; and a put whose q would lie over rows not yet read."""
+import numpy as np
+import pytest
+import torch
+from ferrite_amd import lib, llama as G, ops
+from oracle import llama as OL
+from test_paged_refusals import append
+
+needs_lib = pytest.mark.skipif(not lib.PATH.exists(), reason="libferrite_hip.so not built")
+pytestmark = needs_lib
+
+
+@pytest.fixture
+def decoder(monkeypatch):
+  """A Decoder of two blocks without weights: 4 slots of 96 places, 24 pages of 16."""
+  monkeypatch.setattr(ops, "put_i32", lambda values, out: out.copy_(torch.from_numpy(np.ascontiguousarray(values, np.int32)).view(out.shape)))
+  c = OL.smollm(layers=2, vocab=256, places=400)
+  gc = G.model(**{k: getattr(c, k) for k in ("dim", "heads", "kv", "layers", "eps", "theta", "vocab", "ffn", "places", "rope", "tied")})
+  d = G.Decoder.__new__(G.Decoder)
+  d.c, d.mode, d.batch, d.context, d.device = gc, "bfp8", 3, 96, torch.device("cpu")
+  d.hd = G.head(gc)
+  d.qkv_cols = (gc.heads + 2 * gc.kv) * d.hd
+  d._buffers("bf16", 3, 96, 4)
+  return d
+
+
+def adapters(n, K, parts, rank=8):
+  return ops.Adapters(torch.zeros(n, rank * len(parts), K), torch.zeros(n, sum(parts), rank), None, parts)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(xd=lib.BF16, qd=lib.F32), dict(qd=lib.BF16), dict(rows=1, qd=lib.BF16), dict(rows=1, xd=lib.BF16),
+                                dict(rows=1, xd=lib.BF16, qd=lib.F32, ldq=768)])
+def test_q_over_rows_of_another_type_is_refused(kw):
+  # (a wave's q would land on columns that another wave has not read, one row's too)
+  lib.load()
+  with pytest.raises(ValueError, match="qkv's own columns"): append(**kw)
