@@ -73,11 +73,11 @@ __device__ inline void norm_turn(const AppendArgs& a, const float* w, int64_t tu
 #pragma unroll
     for (int m = 1; m < HD / 8; m <<= 1) ss += __shfl_xor(ss, m, 64);
     const F mean = ss * F(1.0 / HD) + F(a.eps);
+    // Squares that overflow give a mean of infinity and 0, as in the framework's other norms. (The chip's reciprocal root with a step of
+    // Newton's is 1.5% faster, 3517 rows of 8B's, but the step is 0 times infinity there, and the root takes no number below the normal ones.)
     F r;
-    if constexpr (sizeof(F) == 4) {  // (the chip's reciprocal root, within a unit, and a step of Newton's)
-      r = __builtin_amdgcn_rsqf(mean);
-      r = r * fmaf(-0.5f * mean * r, r, 1.5f);
-    } else r = F(1) / sqrt(mean);
+    if constexpr (sizeof(F) == 4) r = 1.f / sqrtf(mean);
+    else r = F(1) / sqrt(mean);
     const F c = a.centered ? F(1) : F(0);
     const float4 wu = *(const float4*)(w + 4 * l), wv = *(const float4*)(w + HD / 2 + 4 * l);
     const float wx[4] = {wu.x, wu.y, wu.z, wu.w}, wy[4] = {wv.x, wv.y, wv.z, wv.w};

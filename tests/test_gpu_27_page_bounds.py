@@ -1,0 +1,50 @@
+"""The cache in pages and the adapters where their other tests do not go; each test says what it holds to."""
+import numpy as np
+import pytest
+import torch
+import seq_cases as S
+from test_gpu_23_paged import ints, ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("fmt", ["fp32", "bf16", "bfp8", "bfp4"])
+@pytest.mark.parametrize("hd,x,T", [(64, "fp32", 5), (128, "bf16", 5), (128, "fp32", 1100)])
+def test_a_heads_norm_whose_squares_overflow(cuda, fmt, hd, x, T):
+  # A head of values past 2^64: the mean of their squares is infinite in 32 bits and the norm 0, as the framework's other norms give;
+  # a block float's keys, normed in 64 bits, are the formula's (values alike: 1). The other heads and rows keep their bits.
+  print(f"huge {fmt} {hd} {x} {T}", flush=True)
+  rng = np.random.default_rng(91)
+  heads, kv, pages = 3, 2, -(-T // 16)
+  rows = torch.from_numpy(rng.normal(0, 1, (T, heads + 2 * kv, hd)).astype(np.float32)).to(S.DTYPE[x]).cuda()
+  huge = rows.clone()
+  huge[2 % T, 1], huge[2 % T, heads] = 2.0 ** 65, -2.0 ** 66
+  w, out = torch.ones(hd, device="cuda"), []
+  for v in (rows, huge):
+    cache = ops().kv_cache(2 * kv, 16 * pages, hd, fmt)
+    (cache.data if fmt in ("bfp8", "bfp4") else cache).zero_()
+    q = ops().rope_append_paged(v.view(T, -1), cache, heads, kv, hd, None, None, ints([0, T]), ints([0]), ints(range(pages)).view(1, -1), 16, q_norm=w, k_norm=w, eps=1e-5)
+    if fmt in ("bfp8", "bfp4"):
+      n = 2 * kv * 16 * pages
+      wide = hd if fmt == "bfp8" else hd // 2
+      held = (cache.data[:n * wide].view(2 * kv, -1, wide).clone(), cache.data[n * wide:].view(2 * kv, -1, hd // 16).clone())
+    else: held = (cache.clone(),)
+    out.append((q.view(T, heads, hd), held))
+  (q0, c0), (q1, c1) = out
+  at = 2 % T
+  assert (q1[at, 1] == 0).all() and torch.isfinite(q1).all()
+  # values whose squares vanish, with no eps: a mean of 2^-140, below the normal numbers, and 1
+  tiny = torch.full((1, (heads + 2 * kv) * hd), 2.0 ** -70, device="cuda").to(S.DTYPE[x])
+  q = ops().rope_append_paged(tiny, ops().kv_cache(2 * kv, 16, hd, fmt), heads, kv, hd, None, None, ints([0, 1]), ints([0]), ints([0]).view(1, 1), 16, q_norm=w, k_norm=w, eps=0.0)
+  assert float((q - 1).abs().max()) <= 24 * 2.0 ** -24
+  keep = torch.ones(T, heads, dtype=torch.bool, device="cuda")
+  keep[at, 1] = False
+  assert torch.equal(q0[keep], q1[keep])
+  for a, b in zip(c0, c1):
+    keep = torch.ones(a.shape[:2], dtype=torch.bool, device="cuda")
+    keep[0, at] = False
+    assert torch.equal(a[keep], b[keep])
+  if fmt in S.DTYPE: assert (c1[0][0, at] == 0).all()
+  else:  # -1: whole steps of 2^-6 or 2^-2 under the exponent of 1, two to a byte in bfp4
+    m = c1[0][0, at]
+    assert (c1[1][0, at] == 127).all() and (m == (256 - 64 if fmt == "bfp8" else 0xCC)).all()
