@@ -624,18 +624,24 @@ class PageStep:
                                self.pages * self.page, self.ws, self.adapters)
 
   def set(self, tokens, places, tables, of=None):
-    """The sequences' next tokens, places and pages, and their adapters (-1, or none given: none)."""
+    """The sequences' next tokens (the host's, or integers on the GPU as they are: a step's own picks), places and pages, and their
+    adapters (-1, or none given: none)."""
     n = self.n
     places = np.asarray(places, np.int64)
     tab = self.dec._page_layout("page_step", places, np.ones(n, np.int64), tables, self.page)
     if tab.shape[1] > self.pages: raise ValueError(f"page_step: up to {self.pages} pages a sequence, not {tab.shape[1]}")
-    tokens, of = np.asarray(tokens, np.int64), np.full(n, -1) if of is None else np.asarray(of, np.int64)
+    there = torch.is_tensor(tokens) and tokens.is_cuda
+    if there and tokens.dtype not in (torch.int32, torch.int64): raise ValueError(f"page_step: tokens are integers, not {tokens.dtype}")
+    if not there: tokens = np.asarray(tokens, np.int64)
+    of = np.full(n, -1) if of is None else np.asarray(of, np.int64)
     if tokens.shape != (n,) or of.shape != (n,): raise ValueError(f"page_step: {n} tokens and adapters")
     wide = np.full((n, self.pages), -1, np.int64)
     wide[:, :tab.shape[1]] = tab
-    ints = np.concatenate([tokens, places, of, wide.reshape(-1)]).astype(np.int32)
-    if ints.size <= PUT_MAX: ops.put_i32(ints, self._int)
-    else: self._int.copy_(torch.from_numpy(ints))
+    ints = np.concatenate(([] if there else [tokens]) + [places, of, wide.reshape(-1)]).astype(np.int32)
+    held = self._int[n:] if there else self._int
+    if ints.size <= PUT_MAX: ops.put_i32(ints, held)
+    else: held.copy_(torch.from_numpy(ints))
+    if there: self.ids.copy_(tokens)
 
   def step(self, tokens=None, places=None, tables=None, of=None, replay=True):
     """One step: the logits ([n][vocab] fp32) and greedy picks ([n] int32); a replayed step's are the graph's, as they are until the

@@ -4,6 +4,8 @@ import pytest
 import torch
 import seq_cases as S
 from test_gpu_23_paged import ints, ops
+from test_gpu_26_pages import VOCAB, config, decoder, pages_for
+from oracle import llama as OL
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +50,24 @@ def test_a_heads_norm_whose_squares_overflow(cuda, fmt, hd, x, T):
   else:  # -1: whole steps of 2^-6 or 2^-2 under the exponent of 1, two to a byte in bfp4
     m = c1[0][0, at]
     assert (c1[1][0, at] == 127).all() and (m == (256 - 64 if fmt == "bfp8" else 0xCC)).all()
+
+
+def test_a_decode_step_takes_its_own_picks(cuda):
+  # the picks of step_pages and of each step, int32 on the GPU, are the next step's tokens as they are
+  rng = np.random.default_rng(98)
+  dec = decoder(OL.random_weights(config()[0], rng), "bf16", 160, 3)
+  text = [[int(i) for i in rng.integers(0, VOCAB, n)] for n in (30, 7, 1)]
+  tables, places = pages_for(rng, [5] * 3, 30), [30, 7, 1]
+  picks = dec.step_pages(text, [0, 0, 0], tables, 16)[1]
+  step = dec.page_step(3, 5, 16)
+  for i in range(4):
+    tokens = picks.tolist()
+    logits, now = step.step(picks, places, tables)
+    got = (logits.clone(), now.clone())
+    want = step.step(tokens, places, tables)   # (the same tokens at the same places, from the host)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    also = step.step(got[1].new_tensor(tokens).long(), places, tables, replay=False)
+    assert torch.equal(also[0], got[0])
+    picks, places = want[1], [p + 1 for p in places]
+  for bad in (picks[:2], picks.view(3, 1), picks.float()):
+    with pytest.raises(ValueError, match="tokens"): step.step(bad, places, tables)
