@@ -505,6 +505,7 @@ class Decoder:
     return P
 
   def _check_adapters(self, what, adapters):
+    """The blocks' adapters (None: none), checked, in lists and dicts of their own: what a captured step reads is not the caller's to replace."""
     c, qkv = self.c, (self.c.heads * self.hd, self.c.kv * self.hd, self.c.kv * self.hd)
     shapes = dict(qkv=(c.dim, qkv), o=(c.heads * self.hd, (c.dim,)), gate_up=(c.dim, (c.ffn, c.ffn)), down=(c.ffn, (c.dim,)))
     if adapters is None or not any(adapters): return None
@@ -512,7 +513,7 @@ class Decoder:
     for ad in adapters:
       for name, a in ad.items():
         if name not in shapes or (a.a.shape[2], a.parts) != shapes[name]: raise ValueError(f"{what}: {name}'s adapters, [{a.a.shape[2]}] -> {a.parts}, are not of {shapes.get(name, 'qkv, o, gate_up or down')}")
-    return adapters
+    return [dict(ad) for ad in adapters]
 
   def step_pages(self, tokens, places, tables, page=64, adapters=None, of=None):
     """A step over sequences whose keys and values lie in pages of the cache (its slots * context rows cut into pages of `page`, 16, 32,
@@ -604,7 +605,8 @@ class Decoder:
 
 class PageStep:
   """A decode step of `n` sequences over a Decoder's cache in pages (Decoder.page_step), replayed as one HIP graph: their tokens, places,
-  pages and adapters are data. A sequence of the batch that nobody holds steps a page of its own."""
+  pages and which adapter each has are data. The adapters themselves are those it was made with: others take a step of their own, or go into
+  the same tensors in place. A sequence of the batch that nobody holds steps a page of its own."""
 
   def __init__(self, dec, n, pages, page, adapters):
     ops.attention_heads_ok(dec.c.heads, dec.c.kv, dec.hd)

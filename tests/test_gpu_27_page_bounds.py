@@ -4,7 +4,7 @@ import pytest
 import torch
 import seq_cases as S
 from test_gpu_23_paged import ints, ops
-from test_gpu_26_pages import VOCAB, config, decoder, pages_for
+from test_gpu_26_pages import LAYERS, VOCAB, adapters_of, close, config, decoder, pages_for
 from oracle import llama as OL
 
 pytestmark = pytest.mark.gpu
@@ -71,3 +71,23 @@ def test_a_decode_step_takes_its_own_picks(cuda):
     picks, places = want[1], [p + 1 for p in places]
   for bad in (picks[:2], picks.view(3, 1), picks.float()):
     with pytest.raises(ValueError, match="tokens"): step.step(bad, places, tables)
+
+
+def test_a_step_keeps_the_adapters_it_was_made_with(cuda):
+  # the caller puts others into its own lists after the step was made and captured, and their memory is given to something else
+  rng = np.random.default_rng(99)
+  dec = decoder(OL.random_weights(config()[0], rng), "bf16", 160, 2)
+  ads = adapters_of(rng, 2, ("qkv", "down"), 8)[0]
+  sizes = [(a.a.shape, a.b.shape) for ad in ads for a in ad.values()]
+  call = lambda s, **kw: s.step([5, 9], [0, 3], [[0, 1], [2, 3]], [1, 0], **kw)[0].clone()
+  step = dec.page_step(2, 2, 16, ads)
+  want = call(step)
+  other = adapters_of(rng, 2, ("qkv", "down", "gate_up"), 24)[0]
+  for l in range(LAYERS):
+    ads[l]["qkv"], ads[l]["down"], ads[l]["gate_up"] = other[l]["qkv"], other[l]["down"], other[l]["gate_up"]
+  ads.append({})
+  torch.cuda.synchronize()
+  junk = [torch.full(s, float("nan"), dtype=torch.bfloat16, device="cuda") for pair in sizes for s in pair for _ in range(4)]
+  torch.cuda.synchronize()
+  assert torch.equal(call(step), want) and torch.equal(call(step, replay=False), want) and len(junk)
+  assert not torch.equal(call(dec.page_step(2, 2, 16, ads[:LAYERS])), want)

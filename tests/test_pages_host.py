@@ -35,3 +35,14 @@ def test_q_over_rows_of_another_type_is_refused(kw):
   # (a wave's q would land on columns that another wave has not read, one row's too)
   lib.load()
   with pytest.raises(ValueError, match="qkv's own columns"): append(**kw)
+
+
+def test_a_step_keeps_the_adapters_it_was_made_with(decoder):
+  # the caller's list and dicts change after the step was made: what it reads stays, and stays alive
+  parts = (576, 192, 192)
+  ads = [dict(qkv=adapters(2, 576, parts)), dict(qkv=adapters(2, 576, parts))]
+  first = ads[0]["qkv"]
+  step = decoder.page_step(2, 2, 16, ads)
+  ads[0]["qkv"], ads[1]["gate_up"] = adapters(2, 576, parts, 16), adapters(2, 576, (1536, 1536))
+  ads.append({})
+  assert len(step.adapters) == 2 and step.adapters[0]["qkv"] is first and "gate_up" not in step.adapters[1]
