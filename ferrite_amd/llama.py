@@ -513,15 +513,25 @@ class Decoder:
     for ad in adapters:
       for name, a in ad.items():
         if name not in shapes or (a.a.shape[2], a.parts) != shapes[name]: raise ValueError(f"{what}: {name}'s adapters, [{a.a.shape[2]}] -> {a.parts}, are not of {shapes.get(name, 'qkv, o, gate_up or down')}")
+    if len({a.a.shape[0] for ad in adapters for a in ad.values()}) > 1: raise ValueError(f"{what}: as many adapters in every block and projection (an adapter's number is the same in all)")
     return [dict(ad) for ad in adapters]
+
+  @staticmethod
+  def _check_of(what, of, n, adapters):
+    """Each of n sequences' adapter, checked (None: none has one)."""
+    if of is None: return np.full(n, -1, np.int64)
+    of, count = np.asarray(of, np.int64), next((a.a.shape[0] for ad in adapters or () for a in ad.values()), 0)
+    if of.shape != (n,): raise ValueError(f"{what}: {n} sequences' adapters")
+    if ((of < -1) | (of >= count)).any(): raise ValueError(f"{what}: an adapter outside 0..{count - 1} (-1: none)" if count else f"{what}: an adapter where there are none")
+    return of
 
   def step_pages(self, tokens, places, tables, page=64, adapters=None, of=None):
     """A step over sequences whose keys and values lie in pages of the cache (its slots * context rows cut into pages of `page`, 16, 32,
     64, ...), as many tokens of each as there are: whole prompts, chunks of them and single tokens in one call. Sequence i's tokens
     are at places places[i], places[i] + 1, ..., its place p in page tables[i][p // page]; sequences may begin with the same pages (a common
     prompt), but what rows are put into is one's own. The pages are the caller's to hand out, and so are the rows of slots that
-    they lie in. adapters: for each block a dict of ops.Adapters, of any of "qkv" (parts q, k, v), "o", "gate_up" (gate, up) and "down"; of: each
-    sequence's (-1: none). Returns each sequence's last token's logits ([n][vocab] fp32) and greedy picks ([n] int32), within the
+    they lie in. adapters: for each block a dict of ops.Adapters, of any of "qkv" (parts q, k, v), "o", "gate_up" (gate, up) and "down", as many
+    in each (one that leaves a projection alone has zeros there); of: each sequence's (-1: none). Returns each sequence's last token's logits ([n][vocab] fp32) and greedy picks ([n] int32), within the
     rounding of bf16 rows and fp32 sums of prefill's."""
     c, what = self.c, "step_pages"
     ops.attention_heads_ok(c.heads, c.kv, self.hd)
@@ -531,9 +541,8 @@ class Decoder:
     places = np.asarray(places, np.int64)
     tab = self._page_layout(what, places, lens, tables, page)
     adapters = self._check_adapters(what, adapters)
+    of = self._check_of(what, of, n, adapters)
     T, starts = int(lens.sum()), np.concatenate([[0], np.cumsum(lens)])
-    of = np.full(n, -1, np.int64) if of is None else np.asarray(of, np.int64)
-    if of.shape != (n,): raise ValueError(f"{what}: {n} sequences' adapters")
     ints = np.concatenate([np.concatenate([np.asarray(t, np.int64) for t in tokens]), starts, places, starts[1:] - 1, np.repeat(of, lens), tab.reshape(-1)]).astype(np.int32)
     held = torch.empty(ints.size, dtype=torch.int32, device=self.device)
     if ints.size <= PUT_MAX: ops.put_i32(ints, held)
@@ -635,8 +644,8 @@ class PageStep:
     there = torch.is_tensor(tokens) and tokens.is_cuda
     if there and tokens.dtype not in (torch.int32, torch.int64): raise ValueError(f"page_step: tokens are integers, not {tokens.dtype}")
     if not there: tokens = np.asarray(tokens, np.int64)
-    of = np.full(n, -1) if of is None else np.asarray(of, np.int64)
-    if tokens.shape != (n,) or of.shape != (n,): raise ValueError(f"page_step: {n} tokens and adapters")
+    if tokens.shape != (n,): raise ValueError(f"page_step: {n} tokens, not {tuple(tokens.shape)}")
+    of = self.dec._check_of("page_step", of, n, self.adapters)
     wide = np.full((n, self.pages), -1, np.int64)
     wide[:, :tab.shape[1]] = tab
     ints = np.concatenate(([] if there else [tokens]) + [places, of, wide.reshape(-1)]).astype(np.int32)

@@ -46,3 +46,27 @@ def test_a_step_keeps_the_adapters_it_was_made_with(decoder):
   ads[0]["qkv"], ads[1]["gate_up"] = adapters(2, 576, parts, 16), adapters(2, 576, (1536, 1536))
   ads.append({})
   assert len(step.adapters) == 2 and step.adapters[0]["qkv"] is first and "gate_up" not in step.adapters[1]
+
+
+def test_an_adapter_that_is_not_there_is_refused(decoder):
+  # (the kernel takes an id past the adapters for none: a request would be answered by the base model, or in some blocks alone)
+  parts = (576, 192, 192)
+  ads = [dict(qkv=adapters(3, 576, parts)), dict(o=adapters(3, 576, (576,)), down=adapters(3, 1536, (576,), 16))]
+  ok = dict(tokens=[[1, 2], [3]], places=[0, 5], tables=[[0], [1]], page=16)
+  step = decoder.page_step(2, 2, 16, ads)
+  for of in ([0, 3], [-2, 0], [1 << 40, 0], [0], [0, 1, 2]):
+    with pytest.raises(ValueError, match="adapter"): decoder.step_pages(**ok, adapters=ads, of=of)
+    with pytest.raises(ValueError, match="adapter"): step.set([1, 2], [0, 5], [[0], [1]], of)
+  for none in (None, [], [{}, {}]):
+    with pytest.raises(ValueError, match="there are none"): decoder.step_pages(**ok, adapters=none, of=[-1, 0])
+  with pytest.raises(ValueError, match="there are none"): decoder.page_step(2, 2, 16).set([1, 2], [0, 5], [[0], [1]], [0, -1])
+  for other in (dict(o=adapters(2, 576, (576,))), dict(o=adapters(3, 576, (576,)), down=adapters(4, 1536, (576,)))):
+    with pytest.raises(ValueError, match="as many adapters"): decoder.step_pages(**ok, adapters=[ads[0], other], of=[0, 1])
+    with pytest.raises(ValueError, match="as many adapters"): decoder.page_step(2, 2, 16, [ads[0], other])
+  step.set([7, 8], [0, 20], [[4], [1, 2]], [2, -1])
+  assert step.ids.tolist() == [7, 8] and step.p0.tolist() == [0, 20] and step.of.tolist() == [2, -1] and step.tables.tolist() == [[4, -1], [1, 2]]
+  step.set([7, 8], [0, 20], [[4], [1, 2]])
+  assert step.of.tolist() == [-1, -1]
+  plain = decoder.page_step(2, 2, 16)
+  plain.set([7, 8], [0, 20], [[4], [1, 2]], [-1, -1])
+  assert plain.of.tolist() == [-1, -1]
