@@ -52,6 +52,39 @@ def test_a_heads_norm_whose_squares_overflow(cuda, fmt, hd, x, T):
     assert (c1[1][0, at] == 127).all() and (m == (256 - 64 if fmt == "bfp8" else 0xCC)).all()
 
 
+def mantissas(rng, *shape):
+  """fp32 values of 24 random bits each, 1 to 2 and their negatives."""
+  return torch.from_numpy(((rng.integers(1 << 23, 1 << 24, shape) | 1) * 2.0 ** -23 * rng.choice([-1.0, 1.0], shape)).astype(np.float32))
+
+
+@pytest.mark.parametrize("T,K,N,rank", [(9, 64, 96, 16), (70, 576, 192, 8), (130, 328, 264, 40), (33, 1000, 64, 128)])
+@pytest.mark.parametrize("x", ["fp32", "bf16"])
+@pytest.mark.parametrize("w", ["fp32", "bf16"])
+def test_fp32_adapters_to_their_last_term(cuda, T, K, N, rank, x, w):
+  # One value in each row of x, one in each column of A's product that meets it, one in each row of B: nothing is added but a product's own
+  # terms, so that what is left of the error is theirs. A value of 24 bits is its three terms' sum exactly (8 bits each, signed), and a product by a
+  # power of two is exact. Of two values of 24 bits a product's terms i + j > 2 are left out: twice 2^-8 2^-16 and 2^-32 of it; the 6 kept
+  # are added in 32 bits, at most 6 half steps (2^-24 of sums up to 1 + 2^-7 of it; twice that if the matrix core truncates). u and y
+  # are each such a product: (2 + 2 * 6) 2^-24 of it at u, the same at y and u's rounding to 24 bits.
+  print(f"lora terms {T} {K} {N} {rank} {x} {w}", flush=True)
+  rng = np.random.default_rng(96)
+  bf = lambda t, kind: t if kind == "fp32" else t.to(torch.bfloat16).float()
+  for full in ("x", "a", "b", "all"):
+    two = lambda *s: torch.from_numpy((2.0 ** rng.integers(-3, 4, s) * rng.choice([-1.0, 1.0], s)).astype(np.float32))
+    make = lambda name, *s: mantissas(rng, *s) if full in (name, "all") else two(*s)
+    k_of, r_of = rng.integers(0, K, T), rng.integers(0, rank, N)
+    xs = torch.zeros(T, K)
+    xs[torch.arange(T), torch.from_numpy(k_of)] = bf(make("x", T), x)
+    a, b = bf(make("a", 1, rank, K), w), torch.zeros(1, N, rank)
+    b[0, torch.arange(N), torch.from_numpy(r_of)] = bf(make("b", N), w)
+    ad = ops().Adapters(a.to(S.DTYPE[w]).cuda(), b.to(S.DTYPE[w]).cuda(), None, (N,))
+    got = ops().lora(xs.to(S.DTYPE[x]).cuda(), ad, ints([0] * T)).double().cpu()
+    want = (xs.double() @ a[0].double().T) @ b[0].double().T
+    tol = 0 if full != "all" else 30 * 2.0 ** -24
+    err = (got - want).abs() / want.abs().clamp(min=2.0 ** -100)
+    assert (want != 0).all() and float(err.max()) <= tol, (full, float(err.max()) * 2 ** 24)
+
+
 def test_a_decode_step_takes_its_own_picks(cuda):
   # the picks of step_pages and of each step, int32 on the GPU, are the next step's tokens as they are
   rng = np.random.default_rng(98)
