@@ -52,6 +52,37 @@ def test_a_heads_norm_whose_squares_overflow(cuda, fmt, hd, x, T):
     assert (c1[1][0, at] == 127).all() and (m == (256 - 64 if fmt == "bfp8" else 0xCC)).all()
 
 
+def far(seed, heads, kv, hd, lens, before, bound, fmt="bf16", q="fp32", o="bf16", page=1 << 12, cols=1 << 18):
+  """A call whose max_context is `bound`, over few pages that many sequences read, against the formula."""
+  rng = np.random.default_rng(seed)
+  n, some = len(lens), 3
+  cache, values = S.cache(rng, 2 * kv, some * page, hd, fmt)
+  pick = rng.integers(0, some, n)
+  tables = torch.full((n, cols), -5, dtype=torch.int32, device="cuda")
+  tables[:, 0] = ints(pick)
+  starts = np.concatenate([[0], np.cumsum(lens)])
+  qb = torch.from_numpy(rng.normal(0, 1.5, (int(starts[-1]), heads * hd)).astype(np.float32)).to(S.DTYPE[q])
+  assert max(a + b for a, b in zip(lens, before)) <= page and bound <= cols * page
+  got = ops().attention_paged(qb.cuda(), cache, heads, kv, hd, ints(starts), ints(before), tables, page, bound, out_dtype=S.DTYPE[o])
+  want, tol = torch.zeros(got.shape, dtype=torch.float64), torch.zeros(got.shape, dtype=torch.float64)
+  for s in range(n):
+    a, b, lo = lens[s], before[s], int(starts[s])
+    if a: want[lo:lo + a], tol[lo:lo + a] = S.attend(qb[lo:lo + a], values, pick[s] * page + torch.arange(a + b), b + 1 + np.arange(a), kv, hd, o == "bf16")
+  S.check(got, want, tol, (lens, bound, fmt))
+
+
+@pytest.mark.parametrize("bits", [24, 26, 28, 30])
+@pytest.mark.parametrize("heads,kv,hd,fmt,q,o", [(4, 2, 64, "bf16", "fp32", "bf16"), (4, 1, 128, "bfp8", "bf16", "fp32"), (2, 1, 64, "fp32", "fp32", "fp32"),
+                                                 (8, 1, 128, "bf16", "bf16", "bf16")])
+def test_costs_in_units(cuda, bits, heads, kv, hd, fmt, q, o):
+  # bounds so large that a call's costs go in units of 2 to 2^11 keys (tiles times max_context from 2^30 on): prompts of several tiles, chunks
+  # after many places, tokens beside them and single tokens alone
+  print(f"units {bits} {heads}/{kv} {hd} {fmt} {q} {o}", flush=True)
+  far(92, heads, kv, hd, [150, 1, 0, 129, 20, 1, 70], [0, 3000, 7, 1500, 2, 0, 3800], 1 << bits, fmt, q, o)
+  far(93, heads, kv, hd, [1] * 70, [int(b) for b in np.random.default_rng(1).integers(0, 2500, 70)], 1 << bits, fmt, q, o)
+  if bits == 30: far(94, heads, kv, hd, [1] * 900, [int(b) for b in np.random.default_rng(2).integers(0, 60, 900)], 1 << bits, fmt, q, o)
+
+
 def mantissas(rng, *shape):
   """fp32 values of 24 random bits each, 1 to 2 and their negatives."""
   return torch.from_numpy(((rng.integers(1 << 23, 1 << 24, shape) | 1) * 2.0 ** -23 * rng.choice([-1.0, 1.0], shape)).astype(np.float32))
