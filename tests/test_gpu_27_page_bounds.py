@@ -83,6 +83,26 @@ def test_costs_in_units(cuda, bits, heads, kv, hd, fmt, q, o):
   if bits == 30: far(94, heads, kv, hd, [1] * 900, [int(b) for b in np.random.default_rng(2).integers(0, 60, 900)], 1 << bits, fmt, q, o)
 
 
+@pytest.mark.parametrize("fmt,q,o", [("bfp8", "fp32", "bf16"), ("bfp4", "bf16", "bf16"), ("bfp8", "bf16", "fp32"), ("fp32", "fp32", "fp32")])
+def test_block_floats_and_fp32_repeat_their_bits(cuda, fmt, q, o):
+  # prompts, chunks and tokens cut over many workgroups: every call gives the same bits, on two streams at a time as well
+  rng = np.random.default_rng(95)
+  heads, kv, hd, n = 20, 4, 64, 11
+  cache, _ = S.cache(rng, 2 * kv, 32 * 300, hd, fmt)
+  lens = [250, 1, 130, 77, 0, 199, 1, 64, 128, 1, 90]
+  starts = ints(np.concatenate([[0], np.cumsum(lens)]))
+  x = torch.from_numpy(rng.normal(0, 1.5, (sum(lens), heads * hd)).astype(np.float32)).to(S.DTYPE[q]).cuda()
+  tables = torch.from_numpy(rng.integers(0, 300, (n, 40)).astype(np.int32)).cuda()
+  args = (x, cache, heads, kv, hd, starts, ints(rng.integers(0, 900, n)), tables, 32, 1200)
+  want = ops().attention_paged(*args, out_dtype=S.DTYPE[o])
+  torch.cuda.synchronize()
+  streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+  for i in range(24):
+    with torch.cuda.stream(streams[i % 2]): outs.append(ops().attention_paged(*args, out_dtype=S.DTYPE[o]))
+  torch.cuda.synchronize()
+  assert all(torch.equal(t, want) for t in outs)
+
+
 def mantissas(rng, *shape):
   """fp32 values of 24 random bits each, 1 to 2 and their negatives."""
   return torch.from_numpy(((rng.integers(1 << 23, 1 << 24, shape) | 1) * 2.0 ** -23 * rng.choice([-1.0, 1.0], shape)).astype(np.float32))
@@ -114,6 +134,40 @@ def test_fp32_adapters_to_their_last_term(cuda, T, K, N, rank, x, w):
     tol = 0 if full != "all" else 30 * 2.0 ** -24
     err = (got - want).abs() / want.abs().clamp(min=2.0 ** -100)
     assert (want != 0).all() and float(err.max()) <= tol, (full, float(err.max()) * 2 ** 24)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "bfp8", "bfp4", "fp32"])
+@pytest.mark.parametrize("hd,heads,kv", [(64, 4, 2), (128, 4, 1)])
+@pytest.mark.parametrize("tokens", [False, True])
+def test_fp32_attention_to_its_last_term(cuda, fmt, hd, heads, kv, tokens):
+  # One value in each row of q (24 bits) and of v, powers of 2 in k and v: a score is one product, its terms' sum exact, and each output one weight
+  # times a power of 2. What is left: the scale, two roundings and the constant's (2.5 half steps of |s|), the exponent's fma (one of at most 2 |s|) and its
+  # exp2 (2), once for the weight and once for the sum, whose n additions are a half step each, and 4 for the quotient and the
+  # output: (9 |s| + 8 + n) 2^-24. A third term left out of q moves a weight by up to 5e-5 where scores are 4 to 8 (allowed: 7e-6), out of a
+  # weight the output by up to 5e-6 (allowed: 3e-6 where scores are small).
+  print(f"attention terms {fmt} {hd} {heads}/{kv} {tokens}", flush=True)
+  rng, n = np.random.default_rng(100), 40
+  t = torch.arange(n)
+  for base, most in ((hd ** 0.5 * 4, 8.0), (hd ** 0.5 / 8, 0.25)):
+    base = 2.0 ** round(np.log2(base))
+    most *= base / (hd ** 0.5 * 4 if most == 8.0 else hd ** 0.5 / 8)
+    sign = lambda *s: torch.from_numpy(rng.choice([-1.0, 1.0], s).astype(np.float32))
+    q, k, v = torch.zeros(n, heads, hd), sign(n, kv, hd) * base * torch.from_numpy((2.0 ** -rng.integers(0, 3, (n, kv, hd))).astype(np.float32)), torch.zeros(n, kv, hd)
+    for h in range(heads): q[t, h, torch.from_numpy(rng.integers(0, hd, n))] = mantissas(rng, n)
+    for h in range(kv): v[t, h, t] = sign(n) * torch.from_numpy((2.0 ** rng.integers(-2, 3, n)).astype(np.float32))
+    cache = ops().kv_cache(2 * kv, 64, hd, fmt)
+    table, x = [[2, 0, 3]], torch.cat([q, k, v], 1).reshape(n, -1).cuda()
+    qx = ops().rope_append_paged(x, cache, heads, kv, hd, None, None, ints([0, n]), ints([0]), torch.tensor(table, dtype=torch.int32, device="cuda"), 16)
+    args = (ints(range(n + 1)), ints(range(n)), torch.tensor(table * n, dtype=torch.int32, device="cuda")) if tokens else (ints([0, n]), ints([0]), torch.tensor(table, dtype=torch.int32, device="cuda"))
+    got = ops().attention_paged(qx, cache, heads, kv, hd, *args, 16, n).double().cpu().view(n, heads, hd)
+    for h in range(heads):
+      g = h // (heads // kv)
+      s = (q[:, h].double() @ k[:, g].double().T) / np.sqrt(hd)
+      p = torch.softmax(s.masked_fill(t[None] > t[:, None], -np.inf), 1)
+      want = p @ v[:, g].double()
+      assert float(s.abs().max()) <= most
+      off = ((got[:, h] - want).abs() / want.abs().clamp(min=1e-30))[want != 0]
+      assert float(off.max()) <= (9 * most + 8 + n) * 2.0 ** -24 and (got[:, h][want == 0] == 0).all(), (h, base, float(off.max()) * 2 ** 24)
 
 
 def test_a_decode_step_takes_its_own_picks(cuda):
