@@ -170,6 +170,29 @@ def test_fp32_attention_to_its_last_term(cuda, fmt, hd, heads, kv, tokens):
       assert float(off.max()) <= (9 * most + 8 + n) * 2.0 ** -24 and (got[:, h][want == 0] == 0).all(), (h, base, float(off.max()) * 2 ** 24)
 
 
+def test_a_model_of_grouped_heads_of_128_dimensions(cuda):
+  # prompts, chunks and tokens in pages, then replayed steps, against its slots
+  from ferrite_amd import llama as G
+  cfg = dict(dim=512, heads=8, kv=2, head_dim=128, layers=2, eps=1e-5, theta=10000.0, vocab=1024, ffn=768, places=400)
+  for kv, page in (("bf16", 32), ("bfp8", 16)):
+    rng = np.random.default_rng(97)
+    slots = G.Decoder(G.model(**cfg), G.numpy_weights(OL.random_weights(OL.model(**cfg), rng)), mode="bfp8", kv=kv, batch=1, context=320, slots=3)
+    dec = G.Decoder(G.model(**cfg), None, mode="bfp8", kv=kv, batch=1, context=320, slots=3, share=slots)
+    text = [[int(i) for i in rng.integers(0, 1024, 300)] for _ in range(3)]
+    tables = pages_for(rng, [-(-300 // page)] * 3, 960 // page)
+    at = [0] * 3
+    def want(i, n): return slots.prefill(text[i][at[i]:at[i] + n], slot=i, p0=at[i])[0].clone()
+    for lens in ([170, 1, 33], [1, 90, 40], [20, 1, 1]):
+      got = dec.step_pages([text[i][at[i]:at[i] + n] for i, n in enumerate(lens)], at, tables, page)[0]
+      close(got, torch.cat([want(i, n) for i, n in enumerate(lens)]), (kv, lens))
+      at = [a + n for a, n in zip(at, lens)]
+    step = dec.page_step(3, -(-300 // page), page)
+    for _ in range(3):
+      got = step.step([text[i][at[i]] for i in range(3)], at, tables)[0]
+      close(got, torch.cat([want(i, 1) for i in range(3)]), (kv, "step"))
+      at = [a + 1 for a in at]
+
+
 def test_a_decode_step_takes_its_own_picks(cuda):
   # the picks of step_pages and of each step, int32 on the GPU, are the next step's tokens as they are
   rng = np.random.default_rng(98)
