@@ -7,8 +7,10 @@
 // A workgroup a row or two, HD / 8 lanes a head: a lane holds columns 4 l .. 4 l + 3 of each half, so that a pair turns in the lane, a
 // head's squares meet over 8 or 16 lanes, and a block float's run of 16 columns over 4. What a row waits for is a chain of loads (its
 // sequence, its place, its page's number and its row of the tables), so its own values are on their way before the first of them.
-// 3517 rows of 32 + 8 + 8 heads of 128, bf16, normed: 21.8 us for 89 MB, 4.1 TB/s where a copy reaches 5.1; 4 rows a workgroup 27, the
-// next row's values loaded behind this one's 27: fewer chains at a time. One row of 9 + 3 + 3 heads of 64: 2.5 us in a graph.
+// 3517 rows of 32 + 8 + 8 heads of 128, bf16, normed: 21.3-22.3 us for 89 MB, 4.1 TB/s where a copy reaches 5.15; 4 rows a workgroup 27, the
+// next row's values loaded behind this one's 27: fewer chains at a time. One row of 9 + 3 + 3 heads of 64: 2.9 us in a graph. Into bfp8,
+// 2444 rows of 20 + 4 + 4 heads of 64, normed: 10.1 us for 33 MB (6.3 at a copy's rate); its keys take 64 bits, and with 8 heads of 64 a wave
+// the waves that hold both q's and k's run both arithmetics, one after the other (here one of a row's four, all of its keys).
 #include <algorithm>
 #include <type_traits>
 #include "fh_common.h"

@@ -13,9 +13,11 @@
 // (v_mfma_f32_16x16x32_bf16): bf16 values go in as they are, fp32 ones (x, u, an fp32 adapter) as two bf16 terms for bf16 output
 // (2^-16 of themselves, less than the output's own rounding, 2^-8) and as three for fp32 output (2^-24).
 //
-// What bounds it (MI355X): the bytes, and for few rows the chain of loads. Beside an 8B model's gate and up, rank 32, 4096 rows of 4 adapters, bf16:
-// 136 us for 510 MB, 22 of them u, the rest y's 470 MB read and written at 4.2 TB/s where a copy reaches 5.1; 333 fp32 rows of 6 adapters by 3456
-// 20 us; beside its q, k and v, rank 16, 32 rows of 24 adapters 12.5 us for 11 MB, two launches of 5 and 7.
+// What bounds it (MI355X, calls in a replayed graph): the bytes, and for few rows the chain of loads. Beside an 8B model's gate and up, rank 32,
+// 4096 rows of 4 adapters, bf16: 133-137 us for 510 MB, 22 of them u (37 MB: 256 workgroups, one a CU, each wave with one round of 64 of K on its
+// way), the rest y's 470 MB read and written at 4.2 TB/s where a copy reaches 5.15; with an fp32 y 211 for 980 MB. 333 fp32 rows of 6 adapters by 3456
+// 20 us for 8 MB: fp32 x and A do not go through LDS, a lane's 32 bytes lie in rows K apart, and each of 210 workgroups adds 14 parts of K again;
+// beside its q, k and v, rank 16, 32 rows of 24 adapters 12.5 us for 11 MB, a chain of loads in each of two launches.
 #include <algorithm>
 #include "fh_common.h"
 
@@ -604,7 +606,8 @@ static void launch_lora(bool few, hipStream_t s, const LoraArgs& a) {
 }
 
 // silu(gate) up for rows whose gate and up are final only behind fh_lora (FH_EP_SILU_GATE does it in the product): a lane 8 columns, which
-// two loads and a store of 16 bytes each bound. 16 rows of 14336 out of fp32 into bf16 4 us (as a program of fh_map, decoded an element, 15).
+// two loads and a store of 16 bytes each bound. 16 rows of 14336 out of fp32 into bf16 4-5 us (as a program of fh_map, decoded an element, 15),
+// 4096 rows 107 for 587 MB, 5.5 TB/s.
 template <bool XB, bool YB>
 __global__ __launch_bounds__(256) void silu_gate_kernel(const void* x, int64_t ldx, int64_t rows, int64_t split, void* y, int64_t ldy) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, pieces = split / 8;

@@ -2,12 +2,16 @@
 // lies at row table[p / page] page + p % page of the cache, and a query at place p sees places 0 .. p:
 // o = sum_k softmax_k(q k / sqrt(hd)) v. Tiles of (row, head of a key head) pairs against tiles of keys with an online softmax, as
 // packed prompts have them (fh_seq.h); what is its own is the pages' reads, how the work is shared (SeqWalk) and token_kernel.
-// What bounds it (MI355X; 32 heads of 128, 8 key heads, bf16 cache; kernels alone): a decode step the reads, 48 tokens after up to
-// 8000 places 160 us (890 MB: 5.5 TB/s, a plain read's rate) and 5 the join of the shares' parts; with fewer keys the chain of a
-// table's page, its rows and the two products: 16 after up to 2000 18 us and 4 (53 MB, 10 at that rate), one launch for 4 short
-// ones 7.3. Prompts the products: 24 of up to 512 rows or single tokens after up to 4000 places 202 us (95 GF of pairs, 180 with the
-// weights' second term and the unseen pairs of a tile: 890 TFLOP/s) and 20 the join (58 MB of parts). A bfp8 cache's runs are decoded by
-// every workgroup that reads them: 11 of up to 250, 16 heads of 64, 28 us and 15.
+// What bounds it (MI355X; 32 heads of 128, 8 key heads, bf16 cache; whole calls in a replayed graph, and the kernels under a trace, which takes up to
+// a tenth longer): a decode step the reads, 48 tokens after up to 8000 places 169 us (890 MB: 5.25 TB/s, a plain read's rate; traced 164 and 6 the join
+// of the shares' parts); with fewer keys the chain of a table's page, its rows and the two products: 16 after up to 2000 22.4 us (traced 18 and 5;
+// 53 MB, 10 at that rate), 4 short ones in one launch 7.8. Prompts the products: 24 of up to 512 rows or single tokens after up to 4000
+// places 206-209 us (traced 201, 95 GF of pairs, 180 with the weights' second term and the unseen pairs of a tile: 895 TFLOP/s; and 20 the join, 58 MB of
+// parts). A bfp8 cache's runs are decoded by every workgroup that reads them: 11 of up to 250, 20 heads of 64, 42 us (traced 30 and 15).
+//
+// For bf16 output an fp32 q and the weights go in as two bf16 terms, as in the packed attention: in that bfp8 case 3.6e-6 off in the mean before the output's
+// own rounding of 1.6e-3, so that one value in 280 takes the other neighbour of the exact one (an fp32 computation: one in 1900; q in
+// three terms: one in 510).
 #include "fh_seq.h"
 
 namespace fh {
@@ -248,8 +252,9 @@ using namespace fh;
 // the cost from which a tile of 128 pairs of 128 dimensions is cut (its parts are 66 KB each, written and read: 16 prompts of up to 300 38 us,
 // with every tile cut 55). Prompts of tiles enough for every workgroup that the GPU holds, no sequence of which may outweigh the others' (PG_EACH:
 // rows a sequence times rounds of tiles against max_context), go a tile a workgroup as they come, a sequence's longest first, without cuts
-// or a join: 16 of 100 to 400 rows 54 -> 45 us, 4 of 1024 to 2048 185 -> 158, one of 2048 96 -> 85, 16 of 512 after up to 4000 places 600 -> 531;
-// but 8 of these 233 -> 243, 6 of them beside 24 tokens 272 -> 304, and over an fp32 cache 4 of up to 1500 575 -> 717.
+// or a join: with bf16 q, lengths and places evenly spaced in three mixed orders, 16 of 100 to 400 rows 53-61 -> 45-50 us, 4 of 1024 to 2048 170-178 -> 148-154,
+// one of 2048 86 -> 79, 16 of 512 after up to 4000 places 524-530 -> 462-487; but 8 of these 263-271 -> 261-297, 6 of them beside 24 tokens
+// 241-246 -> 265-292, and over an fp32 cache 4 of 512 to 1500 368 -> 370-429.
 constexpr int PG_WHOLE = 448, PG_WHOLE_FEW = 1024, PG_LEAST_TOKENS = 128, PG_LEAST = 256, PG_UNCUT = 512;
 constexpr int PG_EACH = 4;
 static int paged_slots(int head_dim) { return SQ_CUS * (head_dim == 64 ? 3 : 2); }

@@ -317,8 +317,8 @@ int fh_attention_decode_shared(const void* q, int q_dtype, const void* cache, in
  * through their RMSNorm x rsqrt(mean(x^2) + eps) w (w + 1 when centered), each head its own mean (q_norm, k_norm [head_dim]; each
  * NULL for none), and turned as FH_EP_ROPE_KV turns them by their place's row of cos_tab and sin_tab ([rope_rows][head_dim], a place
  * outside reads the nearest row; both NULL: not turned); q out (FH_F32 or FH_BF16), k and v into the cache at their place's row,
- * rounded as FH_EP_ROPE_KV's put. A place past the table or a page outside the cache writes no key or value; of rows with one cache row
- * in common any one's stays. For projections
+ * rounded as FH_EP_ROPE_KV's put. A place past the table or a page outside the cache writes no key or value; rows with one cache row in
+ * common leave values of each there (a block float's magnitudes and exponents of different ones, too). For projections
  * whose q, k and v are not final in the product (an adapter's part is added first), and for models with normed heads. q may be qkv's
  * own q columns (ldq = ldx, q_dtype = x_dtype). qkv's and q's rows are aligned to 4 values; norms, tables of angles and the cache to 16 bytes. */
 int fh_rope_append_paged(const void* qkv, int x_dtype, int64_t ldx, int64_t rows, int sequences, int heads, int kv_heads,
@@ -345,7 +345,8 @@ int fh_attention_paged(const void* q, int q_dtype, int64_t ldq, const void* cach
  * multiple of 8 up to 128, K and part_cols multiples of 8 (zeros behind what an adapter has of them). scale [adapters] (NULL: 1).
  * residual [rows][ldr] and y [rows][ldy] in y_dtype (FH_F32 or FH_BF16); residual may be y itself (then ldr = ldy), otherwise
  * they do not overlap, and y overlaps no other operand; NULL: zeros. x A^T, sums and the addition are fp32; products are bf16's, fp32 values in two terms for a bf16 y
- * (2^-16 of themselves) and three for an fp32 one (2^-24); a row with values that are not finite gives values that are not.
+ * (2^-16 of themselves) and three for an fp32 one (2^-24); a row with values that are not finite, or beyond what bf16
+ * holds (3.396e38, of fp32's 3.403e38), gives values that are not.
  * Everything 16-byte aligned, rows too. A call repeats its bits; one of other sizes may add K in other parts. Workspace: no
  * clearing, no state; one for some rows serves fewer. No counterpart in the reference. */
 size_t fh_lora_workspace_bytes(int64_t rows, int64_t K, int rank, int parts);
